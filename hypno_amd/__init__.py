@@ -38,6 +38,7 @@ from .kernels import (  # noqa: F401
     unregister_weight,
 )
 
+from .attention import append_kv, paged_attention  # noqa: F401
 from .model import FormatError, HypnoModel  # noqa: F401
 
 __version__ = "0.1.0"

@@ -52,6 +52,10 @@ SIGNATURES = {
     "hypno_hip_argmax_dev": (_i, [_vp, _vp, _sz, _vp]),
     "hypno_hip_sample_token_dev": (_i, [_vp, _vp, _vp, _sz, ctypes.c_float, ctypes.c_float,
                                         _sz, _vp]),
+    "hypno_hip_append_kv_dev": (_i, [_vp, _vp, _vp, _sz, _vp, _sz, _sz, _vp, _sz, _vp, _sz, _vp,
+                                     _sz, _u32, _vp]),
+    "hypno_hip_paged_attention_dev": (_i, [_vp, _vp, _sz, _sz, _vp, _vp, ctypes.c_float, _sz, _sz,
+                                           _vp]),
     "hypno_hip_model_open": (_i, [ctypes.c_char_p, _u32, ctypes.POINTER(_vp)]),
     "hypno_hip_model_close": (_i, [_vp]),
     "hypno_hip_model_header": (_i, [_vp, ctypes.POINTER(_u32), ctypes.POINTER(_u32),
@@ -77,6 +81,24 @@ class GemvPrologue(ctypes.Structure):
 
 
 PROLOGUE_NONE, PROLOGUE_RMS_NORM, PROLOGUE_SILU_MUL = 0, 1, 2
+
+
+class KvCache(ctypes.Structure):
+    """struct hypno_hip_kv_cache of include/hypno_hip.h."""
+    _fields_ = [("dtype", ctypes.c_uint32), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+                ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
+                ("pages", ctypes.c_size_t), ("kv_heads", ctypes.c_size_t),
+                ("page_size", ctypes.c_size_t), ("head_dim", ctypes.c_size_t),
+                ("k_page_stride", ctypes.c_size_t), ("v_page_stride", ctypes.c_size_t),
+                ("k_scale_page_stride", ctypes.c_size_t),
+                ("v_scale_page_stride", ctypes.c_size_t)]
+
+
+class KvBatch(ctypes.Structure):
+    """struct hypno_hip_kv_batch of include/hypno_hip.h."""
+    _fields_ = [("cu_q", ctypes.c_void_p), ("kv_lens", ctypes.c_void_p),
+                ("page_table", ctypes.c_void_p), ("batch", ctypes.c_size_t),
+                ("table_width", ctypes.c_size_t), ("tokens", ctypes.c_size_t)]
 
 
 class TensorInfo(ctypes.Structure):

@@ -19,6 +19,7 @@
 
 #include "../../include/hypno_hip.h"
 #include "common.hpp"
+#include "kv_cache.hpp"
 
 namespace {
 
@@ -753,6 +754,87 @@ int scratch_of_current_device(FixedScratch* out) {
   return HYPNO_HIP_OK;
 }
 
+// --- paged cache ----------------------------------------------------------------
+
+constexpr size_t kMaxInt = 0x7FFFFFFF;
+
+// Checks a cache and a batch and turns them into the kernels' form.
+int kv_args(const char* what, const hypno_hip_kv_cache* c, const hypno_hip_kv_batch* b,
+            KvCache* kc, KvBatch* kb) {
+  if (!c || !b) return fail(HYPNO_HIP_EINVAL, "%s: NULL cache or batch", what);
+  if (c->dtype != HYPNO_HIP_KV_FP16 && c->dtype != HYPNO_HIP_KV_INT8)
+    return fail(HYPNO_HIP_EINVAL, "%s: unknown cache dtype %u", what, c->dtype);
+  if (c->head_dim == 0 || c->head_dim % 8 || c->head_dim > 256)
+    return fail(HYPNO_HIP_EINVAL, "%s: head_dim %zu is no multiple of 8 up to 256", what,
+                c->head_dim);
+  if (c->page_size == 0 || (c->page_size & (c->page_size - 1)) || c->page_size > 65536)
+    return fail(HYPNO_HIP_EINVAL, "%s: page_size %zu is no power of two up to 65536", what,
+                c->page_size);
+  if (c->kv_heads == 0 || c->kv_heads > 65535 || c->pages > kMaxInt)
+    return fail(HYPNO_HIP_EINVAL, "%s: kv_heads or pages out of range", what);
+  if (b->batch > kMaxInt / 2 || b->tokens > kMaxInt || b->table_width > kMaxInt ||
+      mul_overflows(b->batch, b->table_width) || b->table_width * c->page_size > kMaxInt)
+    return fail(HYPNO_HIP_EINVAL, "%s: batch, tokens or table_width out of range", what);
+  const bool i8 = c->dtype == HYPNO_HIP_KV_INT8;
+  if (b->tokens && b->batch &&
+      (!b->cu_q || !b->kv_lens || (b->table_width && !b->page_table) ||
+       (c->pages && (!c->k || !c->v || (i8 && (!c->k_scale || !c->v_scale))))))
+    return fail(HYPNO_HIP_EINVAL, "%s: NULL pointer", what);
+  if (((uintptr_t)c->k | (uintptr_t)c->v) & 15)
+    return fail(HYPNO_HIP_EINVAL, "%s: k and v of the cache must be 16-byte aligned", what);
+  const size_t page = c->kv_heads * c->page_size * c->head_dim, sp = c->kv_heads * c->page_size;
+  *kc = KvCache{(int)c->dtype, c->k, c->v, c->k_scale, c->v_scale,
+                c->k_page_stride ? c->k_page_stride : page,
+                c->v_page_stride ? c->v_page_stride : page,
+                c->k_scale_page_stride ? c->k_scale_page_stride : sp,
+                c->v_scale_page_stride ? c->v_scale_page_stride : sp,
+                (int)c->pages, (int)c->kv_heads, __builtin_ctzll(c->page_size), (int)c->head_dim};
+  if (kc->k_page < page || kc->v_page < page || (i8 && (kc->ks_page < sp || kc->vs_page < sp)))
+    return fail(HYPNO_HIP_EINVAL, "%s: a page stride is smaller than a page", what);
+  if (c->k_page_stride % 8 || c->v_page_stride % 8)
+    return fail(HYPNO_HIP_EINVAL, "%s: page strides of k and v must be multiples of 8", what);
+  if (mul_overflows(c->pages, 4 * std::max(std::max(kc->k_page, kc->v_page),
+                                           std::max(kc->ks_page, kc->vs_page))))
+    return fail(HYPNO_HIP_EINVAL, "%s: cache size overflows", what);
+  *kb = KvBatch{b->cu_q, b->kv_lens, b->page_table, (int)b->batch, (int)b->table_width,
+                (int)b->tokens};
+  return HYPNO_HIP_OK;
+}
+
+// [p, p + bytes) shares memory with the cache or the batch's arrays.
+bool overlaps_kv(const void* p, size_t bytes, const KvCache& c, const KvBatch& b) {
+  const size_t item = c.dtype == kKvFp16 ? 2 : 1, sp = (size_t)c.kv_heads << c.page_shift;
+  auto span = [&](size_t stride, size_t page, size_t size) {
+    return c.pages ? ((c.pages - 1) * stride + page) * size : 0;
+  };
+  const size_t page = sp * c.head_dim, n = b.batch;
+  return overlaps(p, bytes, c.k, span(c.k_page, page, item)) ||
+         overlaps(p, bytes, c.v, span(c.v_page, page, item)) ||
+         overlaps(p, bytes, c.k_scale, span(c.ks_page, sp, 4)) ||
+         overlaps(p, bytes, c.v_scale, span(c.vs_page, sp, 4)) ||
+         overlaps(p, bytes, b.cu_q, (n + 1) * 4) || overlaps(p, bytes, b.kv_lens, n * 4) ||
+         overlaps(p, bytes, b.page_table, n * b.width * 4);
+}
+
+// Rows of wa floats from a and of wb from b share memory; parts of one fused
+// projection (both `stride` floats apart) lie between each other and share none.
+bool rows_overlap(const float* a, size_t na, size_t wa, size_t sa, const float* b, size_t nb,
+                  size_t wb, size_t sb) {
+  if (!overlaps(a, na, b, nb)) return false;
+  if (sa != sb) return true;
+  const size_t step = sa * 4, d = ((uintptr_t)b % step + step - (uintptr_t)a % step) % step;
+  return d < wa * 4 || d + wb * 4 > step;
+}
+
+// Rows of `width` floats, `stride` apart: their extent in bytes, or an error.
+int rows_bytes(const char* what, size_t rows, size_t width, size_t stride, size_t* bytes) {
+  if (stride < width) return fail(HYPNO_HIP_EINVAL, "%s: a stride is smaller than a row", what);
+  if (mul_overflows(rows, stride) || rows * stride > SIZE_MAX / 4)
+    return fail(HYPNO_HIP_EINVAL, "%s: shape overflows size_t", what);
+  *bytes = rows && width ? ((rows - 1) * stride + width) * 4 : 0;
+  return HYPNO_HIP_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -1292,6 +1374,79 @@ int hypno_hip_set_gemm_numerics(uint32_t mode) {
     return -HYPNO_HIP_EINVAL;
   }
   return (int)g_gemm_numerics.exchange(mode);
+}
+
+int hypno_hip_append_kv_dev(const hypno_hip_kv_cache* cache, const hypno_hip_kv_batch* batch,
+                            float* q_out, size_t q_out_stride, const float* q, size_t q_stride,
+                            size_t heads, const float* k, size_t k_stride, const float* v,
+                            size_t v_stride, const float* inv_freq, size_t rot_dim,
+                            uint32_t style, void* stream) {
+  KvCache c;
+  KvBatch b;
+  int st = kv_args("append_kv", cache, batch, &c, &b);
+  if (st) return st;
+  if (rot_dim % 2 || rot_dim > cache->head_dim)
+    return fail(HYPNO_HIP_EINVAL, "append_kv: rot_dim %zu is odd or above head_dim %zu", rot_dim,
+                cache->head_dim);
+  if (style > HYPNO_HIP_ROPE_PAIRS)
+    return fail(HYPNO_HIP_EINVAL, "append_kv: unknown rotation style %u", style);
+  if (heads > 65535 || mul_overflows(heads, batch->tokens))
+    return fail(HYPNO_HIP_EINVAL, "append_kv: heads out of range");
+  const size_t T = batch->tokens, D = cache->head_dim, KV = cache->kv_heads;
+  size_t qb = 0, ob = 0, kb = 0, vb = 0;
+  if (heads && (st = rows_bytes("append_kv", T, heads * D, q_stride, &qb))) return st;
+  if (heads && (st = rows_bytes("append_kv", T, heads * D, q_out_stride, &ob))) return st;
+  if ((st = rows_bytes("append_kv", T, KV * D, k_stride, &kb))) return st;
+  if ((st = rows_bytes("append_kv", T, KV * D, v_stride, &vb))) return st;
+  if (T == 0 || batch->batch == 0) return HYPNO_HIP_OK;
+  if (!k || !v || (heads && (!q || !q_out)) || (rot_dim && !inv_freq))
+    return fail(HYPNO_HIP_EINVAL, "append_kv: NULL pointer");
+  const bool in_place = q_out == q && q_out_stride == q_stride;
+  if ((!in_place && rows_overlap(q_out, ob, heads * D, q_out_stride, q, qb, heads * D, q_stride)) ||
+      rows_overlap(q_out, ob, heads * D, q_out_stride, k, kb, KV * D, k_stride) ||
+      rows_overlap(q_out, ob, heads * D, q_out_stride, v, vb, KV * D, v_stride) || overlaps(q_out, ob, inv_freq, rot_dim * 2) ||
+      overlaps_kv(q_out, ob, c, b))
+    return fail(HYPNO_HIP_EINVAL, "append_kv: q_out overlaps another buffer");
+  if (overlaps_kv(q, qb, c, b) || overlaps_kv(k, kb, c, b) || overlaps_kv(v, vb, c, b) ||
+      overlaps_kv(inv_freq, rot_dim * 2, c, b))
+    return fail(HYPNO_HIP_EINVAL, "append_kv: an input overlaps the cache or the batch");
+  DeviceState* ds = nullptr;
+  {
+    std::lock_guard<std::mutex> g(g_mu);
+    st = device_state(&ds);
+    if (st) return st;
+  }
+  hipError_t e = launch_append_kv(c, b, q_out, q_out_stride, q, q_stride, (int)heads, k, k_stride,
+                                  v, v_stride, inv_freq, (int)rot_dim,
+                                  style == HYPNO_HIP_ROPE_PAIRS, ds->cus, (hipStream_t)stream);
+  return e == hipSuccess ? HYPNO_HIP_OK : hip_fail(e, "append_kv launch");
+}
+
+int hypno_hip_paged_attention_dev(float* out, const float* q, size_t q_stride, size_t heads,
+                                  const hypno_hip_kv_cache* cache,
+                                  const hypno_hip_kv_batch* batch, float scale, size_t window,
+                                  size_t max_kv_len, void* stream) {
+  KvCache c;
+  KvBatch b;
+  int st = kv_args("paged_attention", cache, batch, &c, &b);
+  if (st) return st;
+  const size_t T = batch->tokens, D = cache->head_dim;
+  if (heads == 0 || heads % cache->kv_heads || heads > 65535)
+    return fail(HYPNO_HIP_EINVAL, "paged_attention: %zu heads are no multiple of %zu kv heads",
+                heads, cache->kv_heads);
+  if (T * heads > kMaxInt)
+    return fail(HYPNO_HIP_EINVAL, "paged_attention: tokens * heads out of range");
+  size_t qb = 0, ob = 0;
+  if ((st = rows_bytes("paged_attention", T, heads * D, q_stride, &qb))) return st;
+  if ((st = rows_bytes("paged_attention", T, heads * D, heads * D, &ob))) return st;
+  if (T == 0 || batch->batch == 0) return HYPNO_HIP_OK;
+  if (!out || !q) return fail(HYPNO_HIP_EINVAL, "paged_attention: NULL pointer");
+  if (overlaps(out, ob, q, qb) || overlaps_kv(out, ob, c, b))
+    return fail(HYPNO_HIP_EINVAL, "paged_attention: out overlaps an input");
+  (void)max_kv_len;
+  hipError_t e = launch_paged_attention(out, q, q_stride, (int)heads, c, b, scale,
+                                        (int)std::min(window, kMaxInt), (hipStream_t)stream);
+  return e == hipSuccess ? HYPNO_HIP_OK : hip_fail(e, "paged_attention launch");
 }
 
 int hypno_hip_stream_synchronize(void* stream) {

@@ -406,6 +406,84 @@ int hypno_hip_sample_token_dev(uint32_t* token, uint64_t* rng_state, const float
                                size_t n, float temperature, float top_p, size_t top_k,
                                void* stream);
 
+/* ---------------------------------------------------------------------------
+ * The step between the q/k/v projections and the output projection: rotated keys
+ * and values appended to a paged cache, and attention of the new tokens over it
+ * (in hypno a flat fp32 cache per layer, its rotation and its attention loop,
+ * transformer.rs:92-184,281-462, turbo.rs:145-185; the paged form, the types and
+ * the ragged batch have no counterpart there).  Device pointers, asynchronous on
+ * `stream`.
+ *
+ * A batch of sequences brings `tokens` new tokens, in rows of q, k and v: those of
+ * sequence b are the rows [cu_q[b], cu_q[b + 1]).  kv_lens[b] is what it holds with
+ * them, so that its i-th new token of n has position p = kv_lens[b] - n + i.  Its
+ * positions [j * page_size, (j + 1) * page_size) are in page page_table[b][j] of the
+ * cache.  The three arrays are read on the device.  What is wrong in them leads to no
+ * access out of the buffers: a row of q, k, v of no sequence is left alone; a token
+ * at a negative position, or in a page that is none of the cache's (-1, say) or past
+ * the table's width, is not stored; attention that reads such a page, or a sequence
+ * that is longer than its table row, is NaN.  Pages that no token of a batch sees
+ * (before the windows of all of a sequence's tokens) are not looked at.
+ * ------------------------------------------------------------------------- */
+typedef struct hypno_hip_kv_batch {
+  const int32_t* cu_q;        /* [batch + 1], ascending from 0 */
+  const int32_t* kv_lens;     /* [batch] */
+  const int32_t* page_table;  /* [batch][table_width] */
+  size_t batch, table_width;
+  size_t tokens;              /* rows of q, k, v: cu_q[batch] */
+} hypno_hip_kv_batch;
+
+/* Element types of a cache.  INT8: per (token, kv head) the codes c = round(x / s),
+ * halves away from zero, and one fp32 scale s = max|x| / 127 (a row of zeros, or one
+ * whose scale underflows: s = 0 and codes 0; one that holds an infinity or NaN: s =
+ * NaN and codes 0).  FP16: rounded to nearest (from 65520 on: infinity). */
+#define HYPNO_HIP_KV_FP16 0u
+#define HYPNO_HIP_KV_INT8 1u
+
+typedef struct hypno_hip_kv_cache {
+  uint32_t dtype;             /* HYPNO_HIP_KV_* */
+  void* k;                    /* [pages][kv_heads][page_size][head_dim], 16-byte aligned */
+  void* v;
+  float* k_scale;             /* INT8: [pages][kv_heads][page_size]; FP16: NULL */
+  float* v_scale;
+  size_t pages, kv_heads;
+  size_t page_size;           /* a power of two, at most 2^16 */
+  size_t head_dim;            /* a multiple of 8, at most 256 */
+  /* Elements from one page to the next, of k, v, k_scale and v_scale (0: no gap
+   * between pages; of k and v multiples of 8). */
+  size_t k_page_stride, v_page_stride, k_scale_page_stride, v_scale_page_stride;
+} hypno_hip_kv_cache;
+
+/* Which elements of a head make a pair (x0, x1): j and j + rot_dim / 2, or 2j and
+ * 2j + 1. */
+#define HYPNO_HIP_ROPE_HALVES 0u
+#define HYPNO_HIP_ROPE_PAIRS 1u
+
+/* Rotates pair j of the first rot_dim (even) elements of every head of q and k by p *
+ * inv_freq[j], (x0, x1) -> (x0 cos - x1 sin, x1 cos + x0 sin), angles and products in
+ * 64 bits, results rounded once to fp32; writes k and v to their places in the cache
+ * and q to q_out.  q [tokens][heads][head_dim], k and v [tokens][kv_heads][head_dim],
+ * q_out as q; *_stride: floats from one token to the next.  q_out may be q (with its
+ * stride).  heads = 0: k and v only.  rot_dim = 0: no rotation. */
+int hypno_hip_append_kv_dev(const hypno_hip_kv_cache* cache, const hypno_hip_kv_batch* batch,
+                            float* q_out, size_t q_out_stride, const float* q, size_t q_stride,
+                            size_t heads, const float* k, size_t k_stride, const float* v,
+                            size_t v_stride, const float* inv_freq, size_t rot_dim,
+                            uint32_t style, void* stream);
+
+/* out[t][h] = sum_p w_p v_p / sum_p w_p, w_p = exp(scale * q[t][h] . k_p), over the
+ * positions p <= the token's own (and, with window > 0, > its own - window) of kv head
+ * h / (heads / kv_heads).  Zeros where that leaves none, or no w_p but 0.  The cache's
+ * values are used exactly, sums and softmax statistics are fp32, and q and w are held
+ * to at least 22 bits: out is as near as an fp32 computation's.  out [tokens][heads]
+ * [head_dim], all of it fp32; it may not share memory with an input.  max_kv_len: an
+ * upper bound of kv_lens that the host knows (0: table_width * page_size); it sets how
+ * many work-groups share a sequence, never the result's range. */
+int hypno_hip_paged_attention_dev(float* out, const float* q, size_t q_stride, size_t heads,
+                                  const hypno_hip_kv_cache* cache,
+                                  const hypno_hip_kv_batch* batch, float scale, size_t window,
+                                  size_t max_kv_len, void* stream);
+
 /* Block until all work this library queued on `stream` is done. */
 int hypno_hip_stream_synchronize(void* stream);
 
