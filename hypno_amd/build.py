@@ -23,7 +23,7 @@ LIB_PATH = os.path.join(HERE, LIB_NAME)
 
 SOURCES = ["codec.hip", "gemv_q4_0.hip", "gemv_any.hip", "gemv_f16.hip", "gemm.hip", "gemm_q4.hip", "gemm_exact.hip",
            "gemm_block.hip", "gemm_pair.hip", "skinny_q4.hip", "prologue.hip", "gemv_col.hip", "gemm_q8_0.hip", "sample.hip",
-           "kv_append.hip", "attention.hip", "api.cpp", "model.cpp"]
+           "kv_append.hip", "attention.hip", "attention_few.hip", "attention_tile.hip", "api.cpp", "model.cpp"]
 
 ARCH = "gfx950"
 COMMON_FLAGS = [

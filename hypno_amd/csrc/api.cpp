@@ -1443,9 +1443,19 @@ int hypno_hip_paged_attention_dev(float* out, const float* q, size_t q_stride, s
   if (!out || !q) return fail(HYPNO_HIP_EINVAL, "paged_attention: NULL pointer");
   if (overlaps(out, ob, q, qb) || overlaps_kv(out, ob, c, b))
     return fail(HYPNO_HIP_EINVAL, "paged_attention: out overlaps an input");
-  (void)max_kv_len;
-  hipError_t e = launch_paged_attention(out, q, q_stride, (int)heads, c, b, scale,
-                                        (int)std::min(window, kMaxInt), (hipStream_t)stream);
+  DeviceState* ds = nullptr;
+  {
+    std::lock_guard<std::mutex> g(g_mu);
+    st = device_state(&ds);
+    if (st) return st;
+  }
+  const int win = (int)std::min(window, kMaxInt);
+  const AttnPlan p = attn_plan(c, b, (int)heads, win, (int64_t)std::min(max_kv_len, kMaxInt),
+                               ds->cus);
+  WsLock ws;
+  if (p.bytes) (void)try_workspace(ds, (hipStream_t)stream, p.bytes, ws);
+  hipError_t e = launch_paged_attention(p, out, q, q_stride, (int)heads, c, b, scale, win, ws.p,
+                                        (hipStream_t)stream);
   return e == hipSuccess ? HYPNO_HIP_OK : hip_fail(e, "paged_attention launch");
 }
 

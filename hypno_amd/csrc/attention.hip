@@ -1,92 +1,147 @@
-// Attention of each sequence's new tokens over its pages of the cache:
-//   o = sum_p w_p v_p / sum_p w_p,  w_p = exp(scale q.k_p - m)
-// over the positions p that the token sees, in one pass with the running maximum
-// m and sum.
-#include "kv_cache.hpp"
+// Attention of each sequence's new tokens over its pages of the cache: which kernels
+// a call takes, and the sum of what a row's ranges of positions gave.
+#include "attention.hpp"
 
 namespace hypno {
 
 namespace {
 
-struct AttnArgs {
-  KvCache c;
-  KvBatch b;
-  float* out;
-  const float* q;
-  size_t q_stride;
-  int heads, window;
-  float scale;
-};
-
-// One wave a (token, head).
-template <int kType>
+// One wave a (token, head): a row over no pages at all.
 __global__ void __launch_bounds__(64) attn_rows_kernel(AttnArgs a) {
-  const int t = blockIdx.x, h = blockIdx.y, lane = threadIdx.x;
-  const int D = a.c.head_dim, g = h / (a.heads / a.c.kv_heads);
+  const int t = blockIdx.x / a.heads, h = blockIdx.x % a.heads;
   const int b = find_seq(a.b, t, 0, 0);
   if (b < 0 || b >= a.b.batch) return;
-  const int first = cu_at(a.b, b), n = cu_at(a.b, b + 1) - first;
-  const int64_t kv = load_global<int>(a.b.kv_lens + b);
-  const int64_t pos = kv - n + (t - first);
-  const bool past = kv > ((int64_t)a.b.width << a.c.page_shift);
-  float q[4], m = -__builtin_inff();
-  double o[4] = {}, l = 0.0;  // (20000 additions of one value to an fp32 sum round one way)
-  for (int i = 0; i < 4; i++) {
-    const int e = lane + 64 * i;
-    q[i] = e < D ? a.q[(size_t)t * a.q_stride + (size_t)h * D + e] * a.scale : 0.0f;
-  }
-  const int64_t lo = a.window ? max(pos - a.window + 1, (int64_t)0) : 0;
-  for (int64_t p = lo; p <= pos && !past; p++) {
-    const int page = a.b.page_table[(size_t)b * a.b.width + (p >> a.c.page_shift)];
-    const bool there = page >= 0 && page < a.c.pages;
-    const size_t tok = ((size_t)g << a.c.page_shift) + (p & ((1 << a.c.page_shift) - 1));
-    const size_t ki = (size_t)page * a.c.k_page + tok * D, vi = (size_t)page * a.c.v_page + tok * D;
-    float s = 0.0f, v[4] = {};
-    if (there) {
-      for (int i = 0; i < 4; i++) {
-        const int e = lane + 64 * i;
-        if (e >= D) continue;
-        if (kType == kKvFp16) {
-          s = fmaf(q[i], (float)((const _Float16*)a.c.k)[ki + e], s);
-          v[i] = (float)((const _Float16*)a.c.v)[vi + e];
-        } else {
-          s = fmaf(q[i], (float)((const int8_t*)a.c.k)[ki + e], s);
-          v[i] = (float)((const int8_t*)a.c.v)[vi + e] *
-                 a.c.v_scale[(size_t)page * a.c.vs_page + tok];
-        }
-      }
-      s = wave_sum(s);
-      if (kType == kKvInt8) s *= a.c.k_scale[(size_t)page * a.c.ks_page + tok];
-    } else {
-      s = __builtin_nanf("");
-    }
-    const float mn = fmaxf(m, s);
-    const float ref = mn == -__builtin_inff() ? 0.0f : mn;
-    const float r = expf(m - ref), w = expf(s - ref);
-    m = mn;
-    l = l * r + w;
-    for (int i = 0; i < 4; i++) o[i] = o[i] * r + (double)w * v[i];
-  }
-  for (int i = 0; i < 4; i++) {
-    const int e = lane + 64 * i;
-    if (e < D)
-      a.out[((size_t)t * a.heads + h) * D + e] =
-          past ? __builtin_nanf("") : l == 0.0 ? 0.0f : (float)(o[i] / l);
-  }
+  const Seq sq = seq_of(a.b, b);
+  attn_row(a, sq, t - sq.first, h);
 }
+
+// One work-group a (token, head): the maxima, sums and outputs of its ranges; wave w
+// takes every fourth one from w, a lane four elements.
+__global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a) {
+  __shared__ float4 so[4][64];
+  __shared__ float2 sml[4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int t = blockIdx.x / a.heads, h = blockIdx.x % a.heads;
+  const int D = a.c.head_dim, G = a.group;
+  const int b = find_seq(a.b, t, 0, 0);
+  if (b < 0 || b >= a.b.batch) return;
+  const Seq sq = seq_of(a.b, b);
+  const int rows = sq.n * G, r = (t - sq.first) * G + h % G;
+  if (r < 0 || r >= rows) return;
+  const bool few = rows <= a.few;
+  const AttnSplit sp = few ? a.fs : a.ts;
+  if (sp.splits <= 1) return;  // written already
+  const int per = few ? 16 : a.tile_rows, r0 = r / per * per;
+  const bool past = too_long(a, sq);
+  const int n = past ? 0 : split_count(a, sq, sp, r0, min(r0 + per, rows));
+  const size_t row = (size_t)t * a.heads + h, step = (size_t)a.b.tokens * a.heads;
+  float m = -__builtin_inff(), l = 0.0f;
+  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int i = wave; i < n; i += 4) {
+    const float2 p = load_global<float2>(a.part_ml + i * step + row);
+    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (4 * lane < D) v = load_global<f32x4>(a.part_o + (i * step + row) * D + 4 * lane);
+    const float mn = fmaxf(m, p.x), ref = mn == -__builtin_inff() ? 0.0f : mn;
+    const float f = __builtin_amdgcn_exp2f(m - ref), w = __builtin_amdgcn_exp2f(p.x - ref);
+    m = mn;
+    l = l * f + p.y * w;
+    o.x = o.x * f + v[0] * w;
+    o.y = o.y * f + v[1] * w;
+    o.z = o.z * f + v[2] * w;
+    o.w = o.w * f + v[3] * w;
+  }
+  so[wave][lane] = o;
+  if (lane == 0) sml[wave] = make_float2(m, l);
+  __syncthreads();
+  if (wave) return;
+  for (int i = 1; i < 4; i++) {
+    const float2 p = sml[i];
+    const float4 v = so[i][lane];
+    const float mn = fmaxf(m, p.x), ref = mn == -__builtin_inff() ? 0.0f : mn;
+    const float f = __builtin_amdgcn_exp2f(m - ref), w = __builtin_amdgcn_exp2f(p.x - ref);
+    m = mn;
+    l = l * f + p.y * w;
+    o.x = o.x * f + v.x * w;
+    o.y = o.y * f + v.y * w;
+    o.z = o.z * f + v.z * w;
+    o.w = o.w * f + v.w * w;
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const f32x4 v = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
+  const float z = ((l + v[0]) + (v[1] + v[2]) + v[3]) * 0.0f;
+  const bool again = __any(!(z == 0.0f)) || past;
+  if (again)
+    attn_row(a, sq, t - sq.first, h);
+  else if (4 * lane < D)
+    *reinterpret_cast<f32x4*>(a.out + row * D + 4 * lane) = v;
+}
+
+int up(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
 }  // namespace
 
-hipError_t launch_paged_attention(float* out, const float* q, size_t q_stride, int heads,
-                                  const KvCache& c, const KvBatch& b, float scale, int window,
-                                  hipStream_t s) {
-  const AttnArgs a = {c, b, out, q, q_stride, heads, window, scale};
-  const dim3 grid(b.tokens, heads);
-  if (c.dtype == kKvFp16)
-    attn_rows_kernel<kKvFp16><<<grid, 64, 0, s>>>(a);
-  else
-    attn_rows_kernel<kKvInt8><<<grid, 64, 0, s>>>(a);
-  return hipGetLastError();
+AttnPlan attn_plan(const KvCache& c, const KvBatch& b, int heads, int window, int64_t max_kv,
+                   int num_cus) {
+  AttnPlan p = {};
+  const int G = heads / c.kv_heads;
+  const int64_t rows = (int64_t)b.tokens * G;
+  p.tile_rows = c.head_dim <= 128 ? 128 : 64;
+  // Single tokens, or one sequence of few rows: attn_few_kernel alone.  One sequence
+  // of many rows, or groups of more than 16: attn_tile_kernel alone.
+  const bool only_few = b.tokens <= b.batch || (b.batch == 1 && rows <= 16);
+  const bool only_tile = !only_few && (b.batch == 1 || G > 16);
+  p.few = only_few ? 0x7FFFFFFF : only_tile ? 0 : 16;
+  const int64_t room = (int64_t)b.width << c.page_shift;
+  const int64_t kv = std::max<int64_t>(1, max_kv ? std::min(max_kv, room) : room);
+  // Ranges so that there are about four work-groups for each one that the chip holds
+  // at a time, of 128 positions at least.
+  p.fs = {1, 0x7FFFFFFF};
+  if (p.few) {
+    const int64_t seen = window ? std::min<int64_t>(kv, (int64_t)window + 16) : kv;
+    const int64_t pairs = (int64_t)b.batch * c.kv_heads;
+    const int64_t want = std::max<int64_t>(1, 8 * num_cus / pairs);
+    const int64_t chunk = std::max<int64_t>(128, (up(seen, want) + 127) / 128 * 128);
+    p.fs.splits = up(seen, chunk);
+    p.fs.chunk = (int)std::min<int64_t>(chunk, 0x7FFFFFFF);
+  }
+  // Ranges while the work-groups do not fill the chip.
+  p.ts = {1, 0x7FFFFFFF};
+  if (p.few != 0x7FFFFFFF) {
+    const int64_t seen =
+        window ? std::min<int64_t>(kv, (int64_t)window + up(p.tile_rows, G)) : kv;
+    const int64_t groups = std::max<int64_t>(1, rows / p.tile_rows) * c.kv_heads;
+    const int64_t want = std::max<int64_t>(1, 2 * num_cus / groups);
+    const int64_t chunk = std::max<int64_t>(256, (up(seen, want) + 63) / 64 * 64);
+    p.ts.splits = up(seen, chunk);
+    p.ts.chunk = (int)std::min<int64_t>(chunk, 0x7FFFFFFF);
+  }
+  const int most = std::max(p.fs.splits, p.ts.splits);
+  p.ml_bytes = most > 1 ? ((size_t)most * b.tokens * heads * 8 + 255) / 256 * 256 : 0;
+  p.bytes = most > 1 ? p.ml_bytes + (size_t)most * b.tokens * heads * c.head_dim * 4 : 0;
+  return p;
+}
+
+hipError_t launch_paged_attention(const AttnPlan& p, float* out, const float* q, size_t q_stride,
+                                  int heads, const KvCache& c, const KvBatch& b, float scale,
+                                  int window, void* ws, hipStream_t s) {
+  AttnArgs a = {c, b, out, q, q_stride, heads, heads / c.kv_heads, window, scale,
+                p.few, p.tile_rows, p.fs, p.ts, nullptr, nullptr};
+  if (!ws) a.fs = a.ts = {1, 0x7FFFFFFF};
+  a.part_ml = reinterpret_cast<float2*>(ws);
+  a.part_o = reinterpret_cast<float*>((uint8_t*)ws + p.ml_bytes);
+  const unsigned rows = (unsigned)b.tokens * (unsigned)heads;
+  if (c.pages == 0) {
+    attn_rows_kernel<<<rows, 64, 0, s>>>(a);
+    return hipGetLastError();
+  }
+  hipError_t e = hipSuccess;
+  if (a.few != 0x7FFFFFFF) e = launch_attn_tile(a, s);
+  if (e == hipSuccess && a.few) e = launch_attn_few(a, s);
+  if (e == hipSuccess && (a.fs.splits > 1 || a.ts.splits > 1)) {
+    attn_join_kernel<<<rows, 256, 0, s>>>(a);
+    e = hipGetLastError();
+  }
+  return e;
 }
 
 }  // namespace hypno

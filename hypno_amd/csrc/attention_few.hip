@@ -1,0 +1,230 @@
+// Attention for sequences with few rows (single tokens, drafts): a work-group takes
+// one kv head of a sequence and a range of its positions; its four waves run through
+// tiles of 32 keys each on their own, 16 rows at a time, and add up at the end.
+#include "attention.hpp"
+
+namespace hypno {
+
+namespace {
+
+constexpr int kQ = 16, kKeys = 32;
+
+template <int kType, int DP>
+struct Few {
+  static constexpr int kBytes = kKeys * DP * 2;        // V of one tile in LDS
+  static constexpr int kN = kKeys * DP / 8 / 64;       // 16-byte pieces of it a lane
+  static constexpr int kBufs = kType == kKvFp16 ? 2 : 1;
+  // Per wave: V, 8-bit: scales of K and V; afterwards o of 16 rows, maxima and sums.
+  static constexpr int kStage = kBufs * kBytes + (kType == kKvInt8 ? 2 * kKeys * 4 : 0);
+  static constexpr int kOut = kQ * (DP + 4) * 4 + kQ * 8;
+  static constexpr int kWave = kStage > kOut ? kStage : kOut;
+};
+
+template <int kType, int DP>
+__global__ void __launch_bounds__(256, 2) attn_few_kernel(AttnArgs a) {
+  typedef Few<kType, DP> T;
+  typedef KvTile<DP> L;
+  typedef Rows<kType, kQ, DP, kKeys> R;
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  __shared__ uint32_t again;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int KV = a.c.kv_heads, G = a.group, D = a.c.head_dim;
+  int id = blockIdx.x;
+  const int g = id % KV;
+  id /= KV;
+  const int split = id % a.fs.splits;
+  const Seq sq = seq_of(a.b, id / a.fs.splits);
+  const int rows = sq.n * G, b = sq.b;
+  if (rows > a.few) return;
+  const bool past = too_long(a, sq);
+  const int grp = lane / kQ, col = lane % kQ;
+  uint8_t* const vbuf = smem + wave * T::kWave;
+  float* const ks = reinterpret_cast<float*>(vbuf + T::kBufs * T::kBytes);
+  float* const vs = ks + kKeys;
+
+  for (int r0 = 0; r0 < rows; r0 += kQ) {
+    const int r1 = min(r0 + kQ, rows);
+    int lo = first_seen(a, sq, r0 / G), hi = sq.kv - sq.n + (r1 - 1) / G + 1;
+    if (past || hi < lo) hi = lo;
+    if (a.fs.splits > 1) {
+      const int64_t start = lo + (int64_t)split * a.fs.chunk;
+      if (start >= hi && split) continue;
+      if (split + 1 < a.fs.splits) hi = (int)min((int64_t)hi, start + a.fs.chunk);
+      lo = (int)start;
+    }
+    const int row = min(r0 + col, rows - 1);
+    const int ti = row / G, h = g * G + row % G;
+    const int t = sq.first + ti;
+    const int seen_lo = first_seen(a, sq, ti), seen_hi = min(sq.kv - sq.n + ti, hi - 1);
+    const int all_lo = first_seen(a, sq, (r1 - 1) / G);
+    const int all_hi = min(sq.kv - sq.n + r0 / G, hi - 1);
+    R x;
+    x.init(r0 + col < rows ? a.q + (size_t)t * a.q_stride + (size_t)h * D : nullptr, D, a.scale);
+
+    bool bad = false;
+    int pid = 0;                 // page of key lane % 32 of the next tile
+    half8 kf[2][R::kSteps];      // K of the next tile: keys 16 i + col, pieces 4 s + grp
+    uint2 kc[2][R::kSteps], vc[T::kN];  // 8-bit: its codes, and V's
+    float kss = 0.0f, vss = 0.0f;
+    auto look_up = [&](int p0) __attribute__((always_inline)) {
+      pid = page_id(a, b, min(p0 + lane % kKeys, hi - 1));
+    };
+    auto issue = [&](int p0, int buf) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        const int r = kQ * i + col;
+        const Place pl = place(a, g, min(p0 + r, hi - 1), __shfl(pid, r, 64), bad);
+        const size_t ki = (size_t)pl.page * a.c.k_page + (size_t)pl.tok * D + 8 * grp;
+#pragma unroll
+        for (int s = 0; s < R::kSteps; s++) {
+          const bool in = 32 * s + 8 * grp < D;
+          if (kType == kKvFp16) {
+            kf[i][s] = half8{};
+            if (in) kf[i][s] = load_global<half8>((const _Float16*)a.c.k + ki + 32 * s);
+          } else {
+            kc[i][s] = make_uint2(0, 0);
+            if (in) kc[i][s] = load_global<uint2>((const int8_t*)a.c.k + ki + 32 * s);
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < T::kN; i++) {
+        const int r = (i * 64 + lane) / L::kCh, ch = ((i * 64 + lane) % L::kCh) ^ L::swz(r);
+        const Place pl = place(a, g, min(p0 + r, hi - 1), __shfl(pid, r, 64), bad);
+        const size_t vi = (size_t)pl.page * a.c.v_page + (size_t)pl.tok * D + 8 * ch;
+        const bool in = 8 * ch < D;
+        if (kType == kKvFp16) {
+          dma16(in ? (const void*)((const _Float16*)a.c.v + vi) : kZero16,
+                vbuf + buf * T::kBytes + i * 1024);
+        } else {
+          vc[i] = make_uint2(0, 0);
+          if (in) vc[i] = load_global<uint2>((const int8_t*)a.c.v + vi);
+        }
+      }
+      if (kType == kKvInt8) {
+        const Place pl = place(a, g, min(p0 + lane % kKeys, hi - 1), pid, bad);
+        kss = load_global<float>(a.c.k_scale + (size_t)pl.page * a.c.ks_page + pl.tok);
+        vss = load_global<float>(a.c.v_scale + (size_t)pl.page * a.c.vs_page + pl.tok);
+      }
+    };
+
+    const int step = 4 * kKeys;
+    if (lo + wave * kKeys < hi) {
+      look_up(lo + wave * kKeys);
+      issue(lo + wave * kKeys, 0);
+      look_up(lo + wave * kKeys + step);
+    }
+    int buf = 0;
+    for (int p0 = lo + wave * kKeys; p0 < hi; p0 += step, buf ^= T::kBufs - 1) {
+      half8 k[2][R::kSteps];
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+      for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (int s = 0; s < R::kSteps; s++)
+          k[i][s] = kType == kKvFp16 ? kf[i][s]
+                                     : __builtin_bit_cast(half8, codes_to_f16(kc[i][s]));
+      if (kType == kKvInt8) {
+#pragma unroll
+        for (int i = 0; i < T::kN; i++)
+          *reinterpret_cast<u32x4*>(vbuf + (i * 64 + lane) * 16) = codes_to_bf16(vc[i]);
+        ks[lane % kKeys] = kss;
+        vs[lane % kKeys] = vss;
+      }
+      if (p0 + step < hi) {
+        issue(p0 + step, buf ^ (T::kBufs - 1));
+        look_up(p0 + 2 * step);
+      }
+      typename R::acc s[2];
+      x.scores(s, [&](int i, int st) __attribute__((always_inline)) { return k[i][st]; });
+      if (p0 < all_lo || p0 + kKeys - 1 > all_hi)
+        x.template maximum<true>(s, seen_lo - p0, seen_hi - p0, ks);
+      else
+        x.template maximum<false>(s, 0, 0, ks);
+      x.values(s, vbuf + buf * T::kBytes, vs);
+    }
+    x.finish(__any(bad));
+
+    // The four waves' parts, then their sum: thread (row, piece) takes every sixteenth
+    // group of four elements.
+    float* const part = reinterpret_cast<float*>(vbuf);
+    float2* const ml = reinterpret_cast<float2*>(part + kQ * (DP + 4));
+#pragma unroll
+    for (int k = 0; k < R::kDt; k++)
+      *reinterpret_cast<f32x4*>(part + col * (DP + 4) + R::dim(k, 0)) =
+          f32x4{x.o[k][0], x.o[k][1], x.o[k][2], x.o[k][3]};
+    if (lane < kQ) ml[col] = make_float2(x.m, x.l);
+    if (tid == 0) again = 0;
+    __syncthreads();
+    const int or_ = tid / 16, piece = tid % 16;
+    float w[4], m = -__builtin_inff(), l = 0.0f;
+    const float* pw[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      pw[i] = reinterpret_cast<const float*>(smem + i * T::kWave);
+      const float2 v = reinterpret_cast<const float2*>(pw[i] + kQ * (DP + 4))[or_];
+      pw[i] += or_ * (DP + 4);
+      w[i] = v.x;
+      m = fmaxf(m, v.x);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      w[i] = w[i] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(w[i] - m);
+      const float2 v = reinterpret_cast<const float2*>(pw[i] - or_ * (DP + 4) + kQ * (DP + 4))[or_];
+      l += v.y * w[i];
+    }
+    const bool live = r0 + or_ < rows;
+    const int rr = min(r0 + or_, rows - 1);
+    const size_t orow = (size_t)(sq.first + rr / G) * a.heads + g * G + rr % G;
+    const size_t prow = (size_t)split * a.b.tokens * a.heads + orow;
+    const bool parts = a.fs.splits > 1;
+    const float inv = parts ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+    float* const dst = parts ? a.part_o + prow * D : a.out + orow * D;
+    float z = l * 0.0f;
+    if (live) {
+      for (int d = 4 * piece; d < D; d += 64) {
+        f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < 4; i++) v += *reinterpret_cast<const f32x4*>(pw[i] + d) * w[i];
+        v *= inv;
+#pragma unroll
+        for (int j = 0; j < 4; j++) z += v[j] * 0.0f;
+        *reinterpret_cast<f32x4*>(dst + d) = v;
+      }
+      if (parts && piece == 0) a.part_ml[prow] = make_float2(m, l);
+      if (!parts && (!(z == 0.0f) || past)) atomicOr(&again, 1u << or_);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (!parts)
+      attn_rows(a, sq, g, r0, again & (0x1111u << wave));  // (every fourth row a wave)
+    __syncthreads();
+  }
+}
+
+template <int kType, int DP>
+hipError_t run(const AttnArgs& a, hipStream_t s) {
+  const size_t grid = (size_t)a.b.batch * a.c.kv_heads * a.fs.splits;
+  if (grid > 0xFFFFFF) return hipErrorInvalidValue;
+  const hipError_t e = set_lds_limit((const void*)attn_few_kernel<kType, DP>, 4 * Few<kType, DP>::kWave);
+  if (e != hipSuccess) return e;
+  attn_few_kernel<kType, DP><<<(unsigned)grid, 256, 4 * Few<kType, DP>::kWave, s>>>(a);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_attn_few(const AttnArgs& a, hipStream_t s) {
+  const int D = a.c.head_dim;
+  if (a.c.dtype == kKvFp16)
+    return D <= 64    ? run<kKvFp16, 64>(a, s)
+           : D <= 96  ? run<kKvFp16, 96>(a, s)
+           : D <= 128 ? run<kKvFp16, 128>(a, s)
+                      : run<kKvFp16, 256>(a, s);
+  return D <= 64    ? run<kKvInt8, 64>(a, s)
+         : D <= 96  ? run<kKvInt8, 96>(a, s)
+         : D <= 128 ? run<kKvInt8, 128>(a, s)
+                    : run<kKvInt8, 256>(a, s);
+}
+
+}  // namespace hypno

@@ -1,0 +1,216 @@
+// Attention for sequences with many rows (prompts, chunks of them): a work-group
+// takes 4 NQ rows of one kv head, NQ a wave, and runs through their positions in
+// tiles of BK keys that all four waves read from LDS.
+#include "attention.hpp"
+
+namespace hypno {
+
+namespace {
+
+template <int kType, int NQ, int DP, int BK>
+struct Tile {
+  static constexpr int kRows = 4 * NQ;
+  static constexpr int kBytes = BK * DP * 2;          // K or V of one tile
+  static constexpr int kN = BK * DP / 8 / 256;        // 16-byte pieces of it a thread
+  // K and V twice; 8-bit: their scales twice.
+  static constexpr int kLds = 4 * kBytes + (kType == kKvInt8 ? 4 * BK * 4 : 0);
+};
+
+template <int kType, int NQ, int DP, int BK>
+__global__ void __launch_bounds__(256, 2) attn_tile_kernel(AttnArgs a) {
+  typedef Tile<kType, NQ, DP, BK> T;
+  typedef KvTile<DP> L;
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int KV = a.c.kv_heads, G = a.group, D = a.c.head_dim;
+  // The kv head goes fastest (work-groups of one head on one XCD, where it has
+  // eight), the rows with the most positions first.
+  int id = blockIdx.x;
+  const int g = id % KV;
+  id /= KV;
+  const int split = id % a.ts.splits;
+  const int slot = gridDim.x / (KV * a.ts.splits) - 1 - id / a.ts.splits;
+  const int b = find_seq(a.b, slot, G, T::kRows);
+  if (b < 0 || b >= a.b.batch) return;
+  const Seq sq = seq_of(a.b, b);
+  const int rows = sq.n * G;
+  const int r0 = (slot - ((int)((int64_t)sq.first * G / T::kRows) + b)) * T::kRows;
+  if (r0 < 0 || r0 >= rows || rows <= a.few) return;
+  const int r1 = min(r0 + T::kRows, rows);
+  const bool past = too_long(a, sq);
+  int lo = first_seen(a, sq, r0 / G), hi = sq.kv - sq.n + (r1 - 1) / G + 1;
+  if (past || hi < lo) hi = lo;
+  if (a.ts.splits > 1) {
+    const int64_t start = lo + (int64_t)split * a.ts.chunk;
+    if (start >= hi && split) return;
+    if (split + 1 < a.ts.splits) hi = (int)min((int64_t)hi, start + a.ts.chunk);
+    lo = (int)start;
+  }
+
+  // This wave's rows: lane % NQ of it, and the positions that it sees.
+  typedef Rows<kType, NQ, DP, BK> R;
+  const int w0 = r0 + wave * NQ, row = w0 + lane % NQ;
+  const bool live = row < rows;
+  const int ti = min(row, rows - 1) / G, h = g * G + min(row, rows - 1) % G;
+  const int t = sq.first + ti;
+  const int seen_lo = first_seen(a, sq, ti), seen_hi = min(sq.kv - sq.n + ti, hi - 1);
+  // of the wave's rows: the first and last position that any sees, those that all see
+  const int last = min(w0 + NQ, rows) - 1;
+  const bool some = w0 < rows;
+  const int any_lo = some ? first_seen(a, sq, w0 / G) : 0;
+  const int any_hi = some ? min(sq.kv - sq.n + last / G, hi - 1) : -1;
+  const int all_lo = some ? first_seen(a, sq, last / G) : 0;
+  const int all_hi = some ? min(sq.kv - sq.n + w0 / G, hi - 1) : -1;
+  R x;
+  x.init(live ? a.q + (size_t)t * a.q_stride + (size_t)h * D : nullptr, D, a.scale);
+
+  bool bad = false;
+  uint8_t* const kbuf = smem;
+  uint8_t* const vbuf = smem + 2 * T::kBytes;
+  float* const scales = reinterpret_cast<float*>(smem + 4 * T::kBytes);
+  int ids[T::kN], sid = 0;      // pages of this thread's pieces; of its scale
+  uint2 kr[T::kN], vr[T::kN];   // 8-bit codes on their way
+  float sr = 0.0f;
+  auto look_up = [&](int p0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < T::kN; i++)
+      ids[i] = page_id(a, b, min(p0 + (i * 256 + tid) / L::kCh, hi - 1));
+    if (kType == kKvInt8) sid = page_id(a, b, min(p0 + tid % BK, hi - 1));
+  };
+  auto issue = [&](int p0, int buf) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < T::kN; i++) {
+      const int r = (i * 256 + tid) / L::kCh, ch = ((i * 256 + tid) % L::kCh) ^ L::swz(r);
+      const Place pl = place(a, g, min(p0 + r, hi - 1), ids[i], bad);
+      const size_t ki = (size_t)pl.page * a.c.k_page + (size_t)pl.tok * D + 8 * ch;
+      const size_t vi = (size_t)pl.page * a.c.v_page + (size_t)pl.tok * D + 8 * ch;
+      const bool in = 8 * ch < D;
+      if (kType == kKvFp16) {
+        const int at = (i * 256 + wave * 64) * 16 + buf * T::kBytes;
+        dma16(in ? (const void*)((const _Float16*)a.c.k + ki) : kZero16, kbuf + at);
+        dma16(in ? (const void*)((const _Float16*)a.c.v + vi) : kZero16, vbuf + at);
+      } else {
+        kr[i] = vr[i] = make_uint2(0, 0);
+        if (in) {
+          kr[i] = load_global<uint2>((const int8_t*)a.c.k + ki);
+          vr[i] = load_global<uint2>((const int8_t*)a.c.v + vi);
+        }
+      }
+    }
+    if (kType == kKvInt8 && tid < 2 * BK) {
+      const Place pl = place(a, g, min(p0 + tid % BK, hi - 1), sid, bad);
+      sr = tid < BK ? load_global<float>(a.c.k_scale + (size_t)pl.page * a.c.ks_page + pl.tok)
+                    : load_global<float>(a.c.v_scale + (size_t)pl.page * a.c.vs_page + pl.tok);
+    }
+  };
+  auto store = [&](int buf) __attribute__((always_inline)) {  // 8-bit: what `issue` loaded
+#pragma unroll
+    for (int i = 0; i < T::kN; i++) {
+      const int at = (i * 256 + tid) * 16 + buf * T::kBytes;
+      *reinterpret_cast<u32x4*>(kbuf + at) = codes_to_f16(kr[i]);
+      *reinterpret_cast<u32x4*>(vbuf + at) = codes_to_bf16(vr[i]);
+    }
+    if (tid < 2 * BK) scales[buf * 2 * BK + tid] = sr;
+  };
+
+  const int tiles = (hi - lo + BK - 1) / BK;
+  if (tiles > 0) {
+    look_up(lo);
+    issue(lo, 0);
+    if (kType == kKvInt8) store(0);
+    look_up(lo + BK);
+  }
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  for (int i = 0; i < tiles; i++) {
+    const int p0 = lo + i * BK, buf = i & 1;
+    if (i + 1 < tiles) {
+      issue(p0 + BK, buf ^ 1);
+      look_up(p0 + 2 * BK);
+    }
+    if (p0 <= any_hi && p0 + BK > any_lo) {
+      const uint8_t* kt = kbuf + buf * T::kBytes;
+      typename R::acc s[BK / NQ];
+      x.scores(s, [&](int kt_i, int st) __attribute__((always_inline)) {
+        const int r = NQ * kt_i + lane % NQ;
+        return *reinterpret_cast<const half8*>(kt + L::at(r, R::NG * st + lane / NQ));
+      });
+      const float* ks = scales + buf * 2 * BK;
+      if (p0 < all_lo || p0 + BK - 1 > all_hi)
+        x.template maximum<true>(s, seen_lo - p0, seen_hi - p0, ks);
+      else
+        x.template maximum<false>(s, 0, 0, ks);
+      x.values(s, vbuf + buf * T::kBytes, ks + BK);
+    }
+    if (kType == kKvInt8 && i + 1 < tiles) store(buf ^ 1);
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  }
+  x.finish(__syncthreads_or(bad));
+
+  const size_t orow = (size_t)t * a.heads + h;
+  if (a.ts.splits > 1) {
+    if (!live) return;
+    const size_t part = (size_t)split * a.b.tokens * a.heads + orow;
+    float* po = a.part_o + part * D;
+#pragma unroll
+    for (int k = 0; k < R::kDt; k++)
+#pragma unroll
+      for (int i = 0; i < R::kAcc; i += 4) {
+        const int d = R::dim(k, i);
+        if (d < D)
+          *reinterpret_cast<f32x4*>(po + d) =
+              f32x4{x.o[k][i], x.o[k][i + 1], x.o[k][i + 2], x.o[k][i + 3]};
+      }
+    if (lane < NQ) a.part_ml[part] = make_float2(x.m, x.l);
+    return;
+  }
+  const float inv = x.l == 0.0f ? 0.0f : 1.0f / x.l;
+  float z = x.l * 0.0f;
+#pragma unroll
+  for (int k = 0; k < R::kDt; k++)
+#pragma unroll
+    for (int i = 0; i < R::kAcc; i += 4) {
+      const int d = R::dim(k, i);
+      f32x4 v;
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        z += x.o[k][i + j] * 0.0f;
+        v[j] = x.o[k][i + j] * inv;
+      }
+      if (live && d < D) *reinterpret_cast<f32x4*>(a.out + orow * D + d) = v;
+    }
+  uint64_t again = __ballot(live && (!(z == 0.0f) || past));
+  again |= again >> 32;
+  if (NQ == 16) again |= again >> 16;
+  // (the stores above, by other lanes, come first)
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  attn_rows(a, sq, g, w0, again & ((1ull << NQ) - 1));
+}
+
+template <int kType, int NQ, int DP, int BK>
+hipError_t run(const AttnArgs& a, hipStream_t s) {
+  typedef Tile<kType, NQ, DP, BK> T;
+  const size_t slots = (size_t)a.b.tokens * a.group / T::kRows + a.b.batch;
+  const size_t grid = slots * a.c.kv_heads * a.ts.splits;
+  if (grid > 0xFFFFFF) return hipErrorInvalidValue;
+  const hipError_t e = set_lds_limit((const void*)attn_tile_kernel<kType, NQ, DP, BK>, T::kLds);
+  if (e != hipSuccess) return e;
+  attn_tile_kernel<kType, NQ, DP, BK><<<(unsigned)grid, 256, T::kLds, s>>>(a);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_attn_tile(const AttnArgs& a, hipStream_t s) {
+  const int D = a.c.head_dim;
+  if (a.c.dtype == kKvFp16)
+    return D <= 64    ? run<kKvFp16, 32, 64, 64>(a, s)
+           : D <= 96  ? run<kKvFp16, 32, 96, 64>(a, s)
+           : D <= 128 ? run<kKvFp16, 32, 128, 64>(a, s)
+                      : run<kKvFp16, 16, 256, 32>(a, s);
+  return D <= 64    ? run<kKvInt8, 32, 64, 64>(a, s)
+         : D <= 96  ? run<kKvInt8, 32, 96, 64>(a, s)
+         : D <= 128 ? run<kKvInt8, 32, 128, 64>(a, s)
+                    : run<kKvInt8, 16, 256, 32>(a, s);
+}
+
+}  // namespace hypno

@@ -65,8 +65,24 @@ hipError_t launch_append_kv(const KvCache& c, const KvBatch& b, float* q_out, si
                             const float* inv_freq, int rot, bool pairs, int num_cus,
                             hipStream_t s);
 
-hipError_t launch_paged_attention(float* out, const float* q, size_t q_stride, int heads,
-                                  const KvCache& c, const KvBatch& b, float scale, int window,
-                                  hipStream_t s);
+// How the positions of a tile of rows are split: into ranges of `chunk`, the last
+// one of `splits` taking what is left.
+struct AttnSplit {
+  int splits, chunk;
+};
+
+// How a call's rows and positions are split, and the workspace that takes.
+struct AttnPlan {
+  int few;        // sequences of at most so many rows go to attn_few_kernel
+  int tile_rows;  // rows of a work-group of attn_tile_kernel
+  AttnSplit fs, ts;
+  size_t bytes, ml_bytes;
+};
+AttnPlan attn_plan(const KvCache& c, const KvBatch& b, int heads, int window, int64_t max_kv,
+                   int num_cus);
+// ws: plan.bytes, 256-byte aligned, or NULL (no range is split then).
+hipError_t launch_paged_attention(const AttnPlan& p, float* out, const float* q, size_t q_stride,
+                                  int heads, const KvCache& c, const KvBatch& b, float scale,
+                                  int window, void* ws, hipStream_t s);
 
 }  // namespace hypno
