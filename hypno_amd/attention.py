@@ -24,107 +24,130 @@ HypnoHipError.
 """
 from __future__ import annotations
 
-import ctypes
 import math
+import struct
 
-from ._lib import KvBatch, KvCache, check, load
+from ._lib import check, load
 
 __all__ = ["append_kv", "paged_attention"]
 
 _STYLES = {"halves": 0, "pairs": 1}  # HYPNO_HIP_ROPE_*
 
+# The structs of include/hypno_hip.h (as _lib.KvCache and _lib.KvBatch, packed at once:
+# a call of one token takes the GPU 5 us, and its checks should not take longer).
+_CACHE = struct.Struct("=I4x12Q")
+_BATCH = struct.Struct("=6Q")
+
+torch = None
+
 
 def _torch():
-    import torch
+    """(imported by the first call: the rest of the package works without it)"""
+    global torch
+    if torch is None:
+        import torch
     return torch
 
 
-def _rows(t, what: str, heads=None, head_dim=None):
-    """A [tokens, heads, head_dim] float32 tensor whose heads are contiguous: its
-    floats from one token to the next."""
-    torch = _torch()
+def _rows(t, what: str):
+    """A [tokens, heads, head_dim] float32 tensor whose heads are contiguous: its shape,
+    the floats from one token to the next and its device's index."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise ValueError(f"{what} must be a GPU tensor")
-    if t.dtype != torch.float32 or t.dim() != 3:
+    shape = t.shape
+    if t.dtype is not torch.float32 or len(shape) != 3:
         raise ValueError(f"{what} must be float32 [tokens, heads, head_dim], got {t.dtype} "
-                         f"{list(t.shape)}")
-    n, h, d = t.shape
-    if (heads is not None and h != heads) or (head_dim is not None and d != head_dim):
-        raise ValueError(f"{what} is {list(t.shape)}, expected [tokens, {heads}, {head_dim}]")
-    if t.numel() and ((d > 1 and t.stride(2) != 1) or (h > 1 and t.stride(1) != d)):
-        raise ValueError(f"{what}: the heads of a token must be contiguous")
-    if n <= 1 or not t.numel():
-        return h * d
-    if t.stride(0) < h * d:
-        raise ValueError(f"{what}: tokens overlap")
-    return t.stride(0)
+                         f"{list(shape)}")
+    n, h, d = shape
+    s, sh, sd = t.stride()
+    if n and h and d:
+        if (sd != 1 and d > 1) or (sh != d and h > 1):
+            raise ValueError(f"{what}: the heads of a token must be contiguous")
+        if n == 1:
+            s = h * d
+        elif s < h * d:
+            raise ValueError(f"{what}: tokens overlap")
+    else:
+        s = h * d
+    return n, h, d, s, t.get_device()
+
+
+def _empty(q):
+    """(contiguous, whatever q's strides are)"""
+    return torch.empty_like(q) if q.is_contiguous() else q.new_empty(q.shape)
 
 
 def _page_stride(t, what: str) -> int:
     """Elements from one page to the next, 0 if there is one page or none."""
     inner = 1
-    for i in range(t.dim() - 1, 0, -1):
-        if t.shape[i] > 1 and t.stride(i) != inner:
+    shape, stride = t.shape, t.stride()
+    for i in range(len(shape) - 1, 0, -1):
+        if shape[i] > 1 and stride[i] != inner:
             raise ValueError(f"{what}: the elements of a page must be contiguous")
-        inner *= t.shape[i]
-    if t.shape[0] <= 1 or t.stride(0) == inner:
+        inner *= shape[i]
+    if shape[0] <= 1 or stride[0] == inner:
         return 0
-    if t.stride(0) < inner:
+    if stride[0] < inner:
         raise ValueError(f"{what}: pages overlap")
-    return t.stride(0)
+    return stride[0]
 
 
-def _cache(k_cache, v_cache, k_scale, v_scale, device):
-    torch = _torch()
-    for t, what in ((k_cache, "k_cache"), (v_cache, "v_cache")):
-        if not isinstance(t, torch.Tensor) or t.device != device:
-            raise ValueError(f"{what} must be a tensor on {device}")
+def _cache(k_cache, v_cache, k_scale, v_scale, dev: int):
+    """The packed cache, its kv heads and head_dim."""
+    if not isinstance(k_cache, torch.Tensor) or not isinstance(v_cache, torch.Tensor) or \
+            k_cache.get_device() != dev or v_cache.get_device() != dev:
+        raise ValueError(f"k_cache and v_cache must be tensors on GPU {dev}")
     dtype, shape = k_cache.dtype, k_cache.shape
-    if dtype not in (torch.float16, torch.int8):
+    int8 = dtype is torch.int8
+    if not int8 and dtype is not torch.float16:
         raise ValueError(f"k_cache must be float16 or int8, got {dtype}")
-    if len(shape) != 4 or v_cache.shape != shape or v_cache.dtype != dtype:
+    if len(shape) != 4 or v_cache.shape != shape or v_cache.dtype is not dtype:
         raise ValueError("k_cache and v_cache must be [pages, kv_heads, page_size, head_dim] of "
                          "one type")
-    strides = [_page_stride(k_cache, "k_cache"), _page_stride(v_cache, "v_cache"), 0, 0]
-    ks = vs = None
-    if dtype == torch.int8:
-        for i, (t, what) in enumerate(((k_scale, "k_scale"), (v_scale, "v_scale"))):
-            if not isinstance(t, torch.Tensor) or t.device != device or \
-                    t.dtype != torch.float32 or t.shape != shape[:3]:
+    pages, heads, size, dim = shape
+    ks = vs = kss = vss = 0
+    if int8:
+        for t, what in ((k_scale, "k_scale"), (v_scale, "v_scale")):
+            if not isinstance(t, torch.Tensor) or t.get_device() != dev or \
+                    t.dtype is not torch.float32 or t.shape != shape[:3]:
                 raise ValueError(f"{what} must be float32 [pages, kv_heads, page_size] on "
-                                 f"{device} beside an int8 cache")
-            strides[2 + i] = _page_stride(t, what)
-        ks, vs = k_scale.data_ptr(), v_scale.data_ptr()
+                                 f"GPU {dev} beside an int8 cache")
+        ks, kss = k_scale.data_ptr(), _page_stride(k_scale, "k_scale")
+        vs, vss = v_scale.data_ptr(), _page_stride(v_scale, "v_scale")
     elif k_scale is not None or v_scale is not None:
         raise ValueError("a float16 cache has no scales")
-    return KvCache(int(dtype == torch.int8), k_cache.data_ptr(), v_cache.data_ptr(), ks, vs,
-                   *shape, *strides)
+    return _CACHE.pack(int8, k_cache.data_ptr(), v_cache.data_ptr(), ks, vs, pages, heads,
+                       size, dim,
+                       0 if k_cache.is_contiguous() else _page_stride(k_cache, "k_cache"),
+                       0 if v_cache.is_contiguous() else _page_stride(v_cache, "v_cache"),
+                       kss, vss), heads, dim
 
 
-def _batch(page_table, kv_lens, cu_q, tokens: int, device):
-    torch = _torch()
-    for t, what, dim in ((page_table, "page_table", 2), (kv_lens, "kv_lens", 1),
-                         (cu_q, "cu_q", 1)):
-        if not isinstance(t, torch.Tensor) or t.device != device or t.dtype != torch.int32 or \
-                t.dim() != dim or not t.is_contiguous():
-            raise ValueError(f"{what} must be a contiguous int32 tensor of {dim} dimension(s) on "
-                             f"{device}")
-    n = kv_lens.shape[0]
-    if page_table.shape[0] != n or cu_q.shape[0] != n + 1:
-        raise ValueError(f"page_table {list(page_table.shape)}, kv_lens [{n}] and cu_q "
-                         f"[{cu_q.shape[0]}] are not of one batch")
-    return KvBatch(cu_q.data_ptr(), kv_lens.data_ptr(), page_table.data_ptr(), n,
-                   page_table.shape[1], tokens)
+def _batch(page_table, kv_lens, cu_q, tokens: int, dev: int):
+    try:
+        n, width = page_table.shape
+        (lens,), (cus,) = kv_lens.shape, cu_q.shape
+        int32 = torch.int32
+        if page_table.dtype is int32 and kv_lens.dtype is int32 and cu_q.dtype is int32 and \
+                page_table.get_device() == dev and kv_lens.get_device() == dev and \
+                cu_q.get_device() == dev and page_table.is_contiguous() and \
+                kv_lens.is_contiguous() and cu_q.is_contiguous() and lens == n and cus == n + 1:
+            return _BATCH.pack(cu_q.data_ptr(), kv_lens.data_ptr(), page_table.data_ptr(), n,
+                               width, tokens)
+    except (AttributeError, TypeError, ValueError):
+        pass
+    raise ValueError("page_table [sequences, width], kv_lens [sequences] and cu_q [sequences + 1] "
+                     f"must be contiguous int32 tensors on GPU {dev}")
 
 
-def _call(fn, where: str, device, *args) -> None:
-    torch = _torch()
-    stream = torch.cuda.current_stream(device).cuda_stream
-    if torch.cuda.current_device() == device.index:
-        check(fn(*args, stream), where)
+def _call(fn, where: str, dev: int, *args) -> None:
+    if torch.cuda.current_device() == dev:
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
     else:
-        with torch.cuda.device(device):
-            check(fn(*args, stream), where)
+        with torch.cuda.device(dev):
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if status:
+        check(status, where)
 
 
 def append_kv(q, k, v, k_cache, v_cache, page_table, kv_lens, cu_q, inv_freq=None,
@@ -135,46 +158,43 @@ def append_kv(q, k, v, k_cache, v_cache, page_table, kv_lens, cu_q, inv_freq=Non
     None: no rotation.  style "halves": pair j is elements j and j + rot_dim / 2;
     "pairs": 2j and 2j + 1.  q may be None (k and v only).  int8 caches: see
     include/hypno_hip.h for the codes."""
-    torch = _torch()
+    _torch()
     if style not in _STYLES:
         raise ValueError(f"style must be 'halves' or 'pairs', got {style!r}")
-    k_stride = _rows(k, "k")
-    tokens, kv_heads, dim = k.shape
-    device = k.device
-    v_stride = _rows(v, "v", kv_heads, dim)
-    heads = q_stride = o_stride = 0
+    tokens, kv_heads, dim, k_stride, dev = _rows(k, "k")
+    n, vh, vd, v_stride, vdev = _rows(v, "v")
+    if n != tokens or vh != kv_heads or vd != dim or vdev != dev:
+        raise ValueError("k and v differ in shape or device")
+    heads = q_stride = o_stride = rot = 0
     qp = op = fp = None
-    rot = 0
     if q is not None:
-        q_stride = _rows(q, "q", None, dim)
-        heads = q.shape[1]
+        n, heads, qd, q_stride, qdev = _rows(q, "q")
+        if n != tokens or qd != dim or qdev != dev:
+            raise ValueError("q and k differ in tokens, head_dim or device")
         if out is None:
-            out = torch.empty((tokens, heads, dim), dtype=torch.float32, device=device)
-        o_stride = _rows(out, "out", heads, dim)
-        if q.shape[0] != tokens or out.shape[0] != tokens or q.device != device or \
-                out.device != device:
-            raise ValueError("q, k and out differ in tokens or device")
+            out = _empty(q)
+            o_stride = heads * dim
+        else:
+            n, oh, od, o_stride, odev = _rows(out, "out")
+            if n != tokens or oh != heads or od != dim or odev != dev:
+                raise ValueError("q and out differ in shape or device")
         qp, op = q.data_ptr(), out.data_ptr()
     elif out is not None:
         raise ValueError("out without q")
-    if v.shape[0] != tokens or v.device != device:
-        raise ValueError("k and v differ in tokens or device")
     if inv_freq is not None:
-        if not isinstance(inv_freq, torch.Tensor) or inv_freq.device != device or \
-                inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or \
+        if not isinstance(inv_freq, torch.Tensor) or inv_freq.get_device() != dev or \
+                inv_freq.dtype is not torch.float32 or inv_freq.dim() != 1 or \
                 not inv_freq.is_contiguous():
-            raise ValueError(f"inv_freq must be a contiguous float32 [rot_dim / 2] on {device}")
+            raise ValueError(f"inv_freq must be a contiguous float32 [rot_dim / 2] on GPU {dev}")
         rot, fp = 2 * inv_freq.shape[0], inv_freq.data_ptr()
         if rot > dim:
             raise ValueError(f"inv_freq has {rot // 2} values for a head_dim of {dim}")
-    cache = _cache(k_cache, v_cache, k_scale, v_scale, device)
-    if cache.kv_heads != kv_heads or cache.head_dim != dim:
-        raise ValueError(f"k is {list(k.shape)} for a cache of {cache.kv_heads} kv heads of "
-                         f"{cache.head_dim}")
-    batch = _batch(page_table, kv_lens, cu_q, tokens, device)
-    _call(load().hypno_hip_append_kv_dev, "append_kv", device, ctypes.byref(cache),
-          ctypes.byref(batch), op, o_stride, qp, q_stride, heads, k.data_ptr(), k_stride,
-          v.data_ptr(), v_stride, fp, rot, _STYLES[style])
+    cache, ch, cd = _cache(k_cache, v_cache, k_scale, v_scale, dev)
+    if ch != kv_heads or cd != dim:
+        raise ValueError(f"k is {list(k.shape)} for a cache of {ch} kv heads of {cd}")
+    _call(load().hypno_hip_append_kv_dev, "append_kv", dev, cache,
+          _batch(page_table, kv_lens, cu_q, tokens, dev), op, o_stride, qp, q_stride, heads,
+          k.data_ptr(), k_stride, v.data_ptr(), v_stride, fp, rot, _STYLES[style])
     return out
 
 
@@ -187,27 +207,25 @@ def paged_attention(q, k_cache, v_cache, page_table, kv_lens, cu_q, scale=None, 
     scores, by default head_dim ** -0.5.  max_kv_len: an upper bound of kv_lens, if the
     host knows one (default: what page_table has room for); it decides how many
     work-groups share a sequence."""
-    torch = _torch()
-    q_stride = _rows(q, "q")
-    tokens, heads, dim = q.shape
-    device = q.device
-    cache = _cache(k_cache, v_cache, k_scale, v_scale, device)
-    if cache.head_dim != dim or not cache.kv_heads or heads % cache.kv_heads:
-        raise ValueError(f"q is {list(q.shape)} for a cache of {cache.kv_heads} kv heads of "
-                         f"{cache.head_dim}")
+    _torch()
+    tokens, heads, dim, q_stride, dev = _rows(q, "q")
+    cache, kv_heads, cd = _cache(k_cache, v_cache, k_scale, v_scale, dev)
+    if cd != dim or not kv_heads or heads % kv_heads:
+        raise ValueError(f"q is {list(q.shape)} for a cache of {kv_heads} kv heads of {cd}")
     if window < 0:
         raise ValueError("window must not be negative")
-    if max_kv_len is not None and max_kv_len < 0:
+    if max_kv_len is None:
+        max_kv_len = 0
+    elif max_kv_len < 0:
         raise ValueError("max_kv_len must not be negative")
     if scale is None:
         scale = 1.0 / math.sqrt(dim)
     if out is None:
-        out = torch.empty((tokens, heads, dim), dtype=torch.float32, device=device)
-    elif not isinstance(out, torch.Tensor) or out.device != device or \
-            out.dtype != torch.float32 or out.shape != q.shape or not out.is_contiguous():
-        raise ValueError(f"out must be a contiguous float32 {list(q.shape)} on {device}")
-    batch = _batch(page_table, kv_lens, cu_q, tokens, device)
-    _call(load().hypno_hip_paged_attention_dev, "paged_attention", device, out.data_ptr(),
-          q.data_ptr(), q_stride, heads, ctypes.byref(cache), ctypes.byref(batch), float(scale),
-          int(window), int(max_kv_len or 0))
+        out = _empty(q)
+    elif not isinstance(out, torch.Tensor) or out.get_device() != dev or \
+            out.dtype is not torch.float32 or out.shape != q.shape or not out.is_contiguous():
+        raise ValueError(f"out must be a contiguous float32 {list(q.shape)} on GPU {dev}")
+    _call(load().hypno_hip_paged_attention_dev, "paged_attention", dev, out.data_ptr(),
+          q.data_ptr(), q_stride, heads, cache, _batch(page_table, kv_lens, cu_q, tokens, dev),
+          scale, window, max_kv_len)
     return out
