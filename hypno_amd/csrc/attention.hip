@@ -15,15 +15,19 @@ __global__ void __launch_bounds__(64) attn_rows_kernel(AttnArgs a) {
   attn_row(a, sq, t - sq.first, h);
 }
 
-// One work-group a (token, head): the maxima, sums and outputs of its ranges; wave w
-// takes every fourth one from w, a lane four elements.
+// One (token, head): the maxima, sums and outputs of its ranges, by kWaves waves (one
+// where rows are many), each on a part of the ranges.  A lane holds one range's maximum
+// and sum, then four elements of the output in every (64 / lanes)th range.
+template <int kWaves>
 __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a) {
-  __shared__ float4 so[4][64];
+  __shared__ f32x4 so[4][64];
   __shared__ float2 sml[4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int t = blockIdx.x / a.heads, h = blockIdx.x % a.heads;
+  const int part = wave % kWaves;
+  const size_t row = (size_t)blockIdx.x * (4 / kWaves) + wave / kWaves;
+  const int t = (int)(row / a.heads), h = (int)(row % a.heads);
   const int D = a.c.head_dim, G = a.group;
-  const int b = find_seq(a.b, t, 0, 0);
+  const int b = t < a.b.tokens ? find_seq(a.b, t, 0, 0) : -1;
   if (b < 0 || b >= a.b.batch) return;
   const Seq sq = seq_of(a.b, b);
   const int rows = sq.n * G, r = (t - sq.first) * G + h % G;
@@ -33,48 +37,69 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a) {
   if (sp.splits <= 1) return;  // written already
   const int per = few ? 16 : a.tile_rows, r0 = r / per * per;
   const bool past = too_long(a, sq);
-  const int n = past ? 0 : split_count(a, sq, sp, r0, min(r0 + per, rows));
-  const size_t row = (size_t)t * a.heads + h, step = (size_t)a.b.tokens * a.heads;
+  const int all = past ? 0 : split_count(a, sq, sp, r0, min(r0 + per, rows));
+  const int first = all * part / kWaves, n = all * (part + 1) / kWaves - first;
+  const float2* ml = a.part_ml + row * a.row_parts + first;
+  const int lanes = D <= 64 ? 16 : D <= 128 ? 32 : 64, sub = lane / lanes, d = lane % lanes * 4;
+  const float* po = a.part_o + (row * a.row_parts + first) * D + d;
   float m = -__builtin_inff(), l = 0.0f;
-  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  for (int i = wave; i < n; i += 4) {
-    const float2 p = load_global<float2>(a.part_ml + i * step + row);
-    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (4 * lane < D) v = load_global<f32x4>(a.part_o + (i * step + row) * D + 4 * lane);
-    const float mn = fmaxf(m, p.x), ref = mn == -__builtin_inff() ? 0.0f : mn;
+  f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int i0 = 0; i0 < n; i0 += 64) {
+    float2 p = make_float2(-__builtin_inff(), 0.0f);
+    if (i0 + lane < n) p = load_global<float2>(ml + i0 + lane);
+    float top = fmaxf(m, p.x);
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+    const float ref = top == -__builtin_inff() ? 0.0f : top;
     const float f = __builtin_amdgcn_exp2f(m - ref), w = __builtin_amdgcn_exp2f(p.x - ref);
-    m = mn;
-    l = l * f + p.y * w;
-    o.x = o.x * f + v[0] * w;
-    o.y = o.y * f + v[1] * w;
-    o.z = o.z * f + v[2] * w;
-    o.w = o.w * f + v[3] * w;
+    m = top;
+    l = l * f + wave_sum(p.y * w);
+    o *= f;
+    constexpr int kFly = 8;
+    const int cnt = min(64, n - i0), step = 64 / lanes;
+    for (int i = sub; i < cnt; i += kFly * step) {
+      f32x4 v[kFly];
+#pragma unroll
+      for (int j = 0; j < kFly; j++)
+        if (i + j * step < cnt && d < D)
+          v[j] = load_global<f32x4>(po + (size_t)(i0 + i + j * step) * D);
+#pragma unroll
+      for (int j = 0; j < kFly; j++) {
+        const float wj = __shfl(w, min(i + j * step, 63), 64);
+        if (i + j * step < cnt && d < D) o += v[j] * wj;
+      }
+    }
   }
-  so[wave][lane] = o;
-  if (lane == 0) sml[wave] = make_float2(m, l);
-  __syncthreads();
-  if (wave) return;
-  for (int i = 1; i < 4; i++) {
-    const float2 p = sml[i];
-    const float4 v = so[i][lane];
-    const float mn = fmaxf(m, p.x), ref = mn == -__builtin_inff() ? 0.0f : mn;
-    const float f = __builtin_amdgcn_exp2f(m - ref), w = __builtin_amdgcn_exp2f(p.x - ref);
-    m = mn;
-    l = l * f + p.y * w;
-    o.x = o.x * f + v.x * w;
-    o.y = o.y * f + v.y * w;
-    o.z = o.z * f + v.z * w;
-    o.w = o.w * f + v.w * w;
+  for (int off = lanes; off < 64; off *= 2)
+#pragma unroll
+    for (int j = 0; j < 4; j++) o[j] += __shfl_xor(o[j], off, 64);
+  if (kWaves > 1) {
+    so[wave][lane] = o;
+    if (lane == 0) sml[wave] = make_float2(m, l);
+    __syncthreads();
+    if (wave) return;
+    float top = m;
+    for (int i = 1; i < kWaves; i++) top = fmaxf(top, sml[i].x);
+    const float ref = top == -__builtin_inff() ? 0.0f : top;
+    l = 0.0f;
+    o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i = 0; i < kWaves; i++) {
+      const float w = __builtin_amdgcn_exp2f(sml[i].x - ref);
+      l += sml[i].y * w;
+      o += so[i][lane] * w;
+    }
   }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  const f32x4 v = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
+  const f32x4 v = o * (l == 0.0f ? 0.0f : 1.0f / l);
   const float z = ((l + v[0]) + (v[1] + v[2]) + v[3]) * 0.0f;
   const bool again = __any(!(z == 0.0f)) || past;
   if (again)
     attn_row(a, sq, t - sq.first, h);
-  else if (4 * lane < D)
-    *reinterpret_cast<f32x4*>(a.out + row * D + 4 * lane) = v;
+  else if (sub == 0 && d < D)
+    *reinterpret_cast<f32x4*>(a.out + row * D + d) = v;
 }
+
+// From here on a wave a row, not four.
+constexpr unsigned kJoinRows = 1024;
 
 int up(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
@@ -99,7 +124,7 @@ AttnPlan attn_plan(const KvCache& c, const KvBatch& b, int heads, int window, in
   if (p.few) {
     const int64_t seen = window ? std::min<int64_t>(kv, (int64_t)window + 16) : kv;
     const int64_t pairs = (int64_t)b.batch * c.kv_heads;
-    const int64_t want = std::max<int64_t>(1, 8 * num_cus / pairs);
+    const int64_t want = std::max<int64_t>(1, (b.batch > 1 ? 8 : 2) * num_cus / pairs);
     const int64_t chunk = std::max<int64_t>(128, (up(seen, want) + 127) / 128 * 128);
     p.fs.splits = up(seen, chunk);
     p.fs.chunk = (int)std::min<int64_t>(chunk, 0x7FFFFFFF);
@@ -125,7 +150,8 @@ hipError_t launch_paged_attention(const AttnPlan& p, float* out, const float* q,
                                   int heads, const KvCache& c, const KvBatch& b, float scale,
                                   int window, void* ws, hipStream_t s) {
   AttnArgs a = {c, b, out, q, q_stride, heads, heads / c.kv_heads, window, scale,
-                p.few, p.tile_rows, p.fs, p.ts, nullptr, nullptr};
+                p.few, p.tile_rows, p.fs, p.ts, std::max(p.fs.splits, p.ts.splits),
+                nullptr, nullptr};
   if (!ws) a.fs = a.ts = {1, 0x7FFFFFFF};
   a.part_ml = reinterpret_cast<float2*>(ws);
   a.part_o = reinterpret_cast<float*>((uint8_t*)ws + p.ml_bytes);
@@ -138,7 +164,10 @@ hipError_t launch_paged_attention(const AttnPlan& p, float* out, const float* q,
   if (a.few != 0x7FFFFFFF) e = launch_attn_tile(a, s);
   if (e == hipSuccess && a.few) e = launch_attn_few(a, s);
   if (e == hipSuccess && (a.fs.splits > 1 || a.ts.splits > 1)) {
-    attn_join_kernel<<<rows, 256, 0, s>>>(a);
+    if (rows < kJoinRows)
+      attn_join_kernel<4><<<rows, 256, 0, s>>>(a);
+    else
+      attn_join_kernel<1><<<(rows + 3) / 4, 256, 0, s>>>(a);
     e = hipGetLastError();
   }
   return e;

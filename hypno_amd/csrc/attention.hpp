@@ -39,8 +39,9 @@ struct AttnArgs {
   int few;                // sequences of at most so many rows are attn_few_kernel's
   int tile_rows;          // rows of a work-group of the other
   AttnSplit fs, ts;       // of attn_few_kernel and attn_tile_kernel
-  float* part_o;          // [split][token][head][head_dim], if some split is above 1
-  float2* part_ml;        // [split][token][head]: maximum (log2), sum
+  int row_parts;          // the larger of both splits
+  float* part_o;          // [token][head][row_parts][head_dim], if that is above 1
+  float2* part_ml;        // [token][head][row_parts]: maximum (log2), sum
 };
 
 // The new tokens of a sequence and what it holds (both at least 0).

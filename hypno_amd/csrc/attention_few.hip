@@ -176,7 +176,7 @@ __global__ void __launch_bounds__(256, 2) attn_few_kernel(AttnArgs a) {
     const bool live = r0 + or_ < rows;
     const int rr = min(r0 + or_, rows - 1);
     const size_t orow = (size_t)(sq.first + rr / G) * a.heads + g * G + rr % G;
-    const size_t prow = (size_t)split * a.b.tokens * a.heads + orow;
+    const size_t prow = orow * a.row_parts + split;
     const bool parts = a.fs.splits > 1;
     const float inv = parts ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
     float* const dst = parts ? a.part_o + prow * D : a.out + orow * D;

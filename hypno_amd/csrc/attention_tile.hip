@@ -149,7 +149,7 @@ __global__ void __launch_bounds__(256, 2) attn_tile_kernel(AttnArgs a) {
   const size_t orow = (size_t)t * a.heads + h;
   if (a.ts.splits > 1) {
     if (!live) return;
-    const size_t part = (size_t)split * a.b.tokens * a.heads + orow;
+    const size_t part = orow * a.row_parts + split;
     float* po = a.part_o + part * D;
 #pragma unroll
     for (int k = 0; k < R::kDt; k++)
