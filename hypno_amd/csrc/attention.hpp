@@ -161,10 +161,11 @@ __device__ __forceinline__ void dma16(const void* src, uint8_t* lds) {
 __device__ __forceinline__ half8 f16x8(u32x4 x) { return __builtin_bit_cast(half8, x); }
 __device__ __forceinline__ bf8 bf16x8(u32x4 x) { return __builtin_bit_cast(bf8, x); }
 
-// Two fp32 -> their fp16 roundings, and those of what these are off by.
-__device__ __forceinline__ void split_f16(float x, float y, uint32_t& h, uint32_t& l) {
-  const half2v a = {(_Float16)x, (_Float16)y};
-  const half2v b = {(_Float16)fmaf((float)a[0], -1.0f, x), (_Float16)fmaf((float)a[1], -1.0f, y)};
+// Two fp32 -> fp16 each (toward zero), and what these leave in fp16.  `neg`: -1 that
+// the compiler does not see (it then takes fp16 and fp32 into one instruction).
+__device__ __forceinline__ void split_f16(float x, float y, float neg, uint32_t& h, uint32_t& l) {
+  const half2v a = __builtin_bit_cast(half2v, __builtin_amdgcn_cvt_pkrtz(x, y));
+  const half2v b = {(_Float16)fmaf((float)a[0], neg, x), (_Float16)fmaf((float)a[1], neg, y)};
   h = __builtin_bit_cast(uint32_t, a);
   l = __builtin_bit_cast(uint32_t, b);
 }
@@ -369,7 +370,8 @@ struct Rows {
     const int row0 = 4 * grp + l16 / 4;
     const int col = (NQ == 32 ? (lane >> 4 & 1) * 2 : 0) + (l16 & 3) / 2;
     const float off = kTop - (m == -__builtin_inff() ? 0.0f : m);
-    float sum = 0.0f;
+    float sum = 0.0f, neg = -1.0f;
+    asm("" : "+s"(neg));
 #pragma unroll
     for (int p = 0; p < kPv; p++) {
       uint32_t w1[4], w2[4], w3[4];  // the weights' parts, two a register
@@ -390,7 +392,7 @@ struct Rows {
         for (int r = 0; r < 4; r += 2) {
           const int i = 2 * q + r / 2;
           if (kType == kKvFp16)
-            split_f16(w[r], w[r + 1], w1[i], w2[i]);
+            split_f16(w[r], w[r + 1], neg, w1[i], w2[i]);
           else
             split_bf16(w[r], w[r + 1], w1[i], w2[i], w3[i]);
         }

@@ -1,6 +1,8 @@
 // Attention for sequences with many rows (prompts, chunks of them): a work-group
 // takes 4 NQ rows of one kv head, NQ a wave, and runs through their positions in
 // tiles of BK keys that all four waves read from LDS.
+#include <type_traits>
+
 #include "attention.hpp"
 
 namespace hypno {
@@ -121,13 +123,15 @@ __global__ void __launch_bounds__(256, 2) attn_tile_kernel(AttnArgs a) {
     look_up(lo + BK);
   }
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-  for (int i = 0; i < tiles; i++) {
+  // Tiles that all of the wave's rows see whole need no mask; each wave goes through
+  // its own runs of the two kinds, tile by tile with the others.
+  auto step = [&](auto masked, int i) __attribute__((always_inline)) {
     const int p0 = lo + i * BK, buf = i & 1;
     if (i + 1 < tiles) {
       issue(p0 + BK, buf ^ 1);
       look_up(p0 + 2 * BK);
     }
-    if (p0 <= any_hi && p0 + BK > any_lo) {
+    if (!masked || (p0 <= any_hi && p0 + BK > any_lo)) {
       const uint8_t* kt = kbuf + buf * T::kBytes;
       typename R::acc s[BK / NQ];
       x.scores(s, [&](int kt_i, int st) __attribute__((always_inline)) {
@@ -135,14 +139,18 @@ __global__ void __launch_bounds__(256, 2) attn_tile_kernel(AttnArgs a) {
         return *reinterpret_cast<const half8*>(kt + L::at(r, R::NG * st + lane / NQ));
       });
       const float* ks = scales + buf * 2 * BK;
-      if (p0 < all_lo || p0 + BK - 1 > all_hi)
-        x.template maximum<true>(s, seen_lo - p0, seen_hi - p0, ks);
-      else
-        x.template maximum<false>(s, 0, 0, ks);
+      x.template maximum<masked>(s, seen_lo - p0, seen_hi - p0, ks);
       x.values(s, vbuf + buf * T::kBytes, ks + BK);
     }
     if (kType == kKvInt8 && i + 1 < tiles) store(buf ^ 1);
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  };
+  const int full0 = some ? min(max(all_lo - lo + BK - 1, 0) / BK, tiles) : tiles;
+  const int full1 = some ? max(full0, (all_hi + 1 - lo) / BK) : tiles;
+  for (int i = 0, run = 0; run < 2; run++) {
+    if (run)
+      for (; i < full1; i++) step(std::false_type(), i);
+    for (const int end = run ? tiles : full0; i < end; i++) step(std::true_type(), i);
   }
   x.finish(__syncthreads_or(bad));
 
