@@ -151,11 +151,17 @@ struct KvTile {
 
 __device__ inline const uint32_t kZero16[4] __attribute__((aligned(16))) = {0, 0, 0, 0};
 
-// Lane i's 16 bytes at `src` to lds + 16 i, asynchronously.
+// Lane i's 16 bytes at `src` to lds + 16 i, asynchronously; counted by vmcnt, which the
+// caller waits for.  (Not the builtin: the compiler then has every transposing read of
+// LDS wait for all such copies, the next tile's too.)
 __device__ __forceinline__ void dma16(const void* src, uint8_t* lds) {
-  __builtin_amdgcn_global_load_lds(
-      (const __attribute__((address_space(1))) void*)(uintptr_t)src,
-      (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
+#if defined(__HIP_DEVICE_COMPILE__)
+  const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)lds;
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+               :
+               : "{m0}"(at), "v"(src)
+               : "memory");
+#endif
 }
 
 __device__ __forceinline__ half8 f16x8(u32x4 x) { return __builtin_bit_cast(half8, x); }
@@ -312,19 +318,29 @@ struct Rows {
     for (int t = 0; t < kDt; t++) o[t] = acc{};
   }
 
-  // Scores of BK keys; key(t, s): the operand of step s for keys NQ t + lane % NQ.
+  // Scores of BK keys; key(t, s): the operand of step s for keys NQ t + lane % NQ.  (The
+  // scheduling barriers keep a step's reads ahead of the products before it: the
+  // compiler puts them right before their use.)
   template <typename F>
   __device__ __forceinline__ void scores(acc (&s)[BK / NQ], F&& key) {
 #pragma unroll
     for (int t = 0; t < BK / NQ; t++) s[t] = acc{};
+    half8 k[2][BK / NQ];
 #pragma unroll
-    for (int st = 0; st < kSteps; st++)
+    for (int t = 0; t < BK / NQ; t++) k[0][t] = key(t, 0);
 #pragma unroll
-      for (int t = 0; t < BK / NQ; t++) {
-        const half8 k = key(t, st);
-        s[t] = Mfma<NQ>::mul(k, qh[st], s[t]);
-        s[t] = Mfma<NQ>::mul(k, ql[st], s[t]);
+    for (int st = 0; st < kSteps; st++) {
+      if (st + 1 < kSteps) {
+#pragma unroll
+        for (int t = 0; t < BK / NQ; t++) k[(st + 1) & 1][t] = key(t, st + 1);
       }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int t = 0; t < BK / NQ; t++) s[t] = Mfma<NQ>::mul(k[st & 1][t], qh[st], s[t]);
+#pragma unroll
+      for (int t = 0; t < BK / NQ; t++) s[t] = Mfma<NQ>::mul(k[st & 1][t], ql[st], s[t]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
   }
 
   // Scores times the keys' scales (8-bit keys: `ks`, the tile's in LDS), -inf where a
@@ -362,7 +378,8 @@ struct Rows {
   }
 
   // Scores to weights, and o += V^T w over a tile of V rows in LDS (KvTile; fp16, or
-  // 8-bit codes as bf16 with the values' scales in `vs`).
+  // 8-bit codes as bf16 with the values' scales in `vs`).  While a step's products run,
+  // the next step's weights are computed, two at a time.
   __device__ __forceinline__ void values(acc (&s)[BK / NQ], const uint8_t* tile,
                                          const float* vs) {
     constexpr int kPer = kAcc / 4;
@@ -370,60 +387,67 @@ struct Rows {
     const int row0 = 4 * grp + l16 / 4;
     const int col = (NQ == 32 ? (lane >> 4 & 1) * 2 : 0) + (l16 & 3) / 2;
     const float off = kTop - (m == -__builtin_inff() ? 0.0f : m);
-    float sum = 0.0f, neg = -1.0f;
+    float neg = -1.0f;
     asm("" : "+s"(neg));
+    u32x4 w[2][3];  // the weights' parts of this step and the next, two a register
+    auto pair = [&](int p, int i) __attribute__((always_inline)) {
+      const int u = 2 * p + i / 2, r = i % 2 * 2;
+      float x[2];
 #pragma unroll
-    for (int p = 0; p < kPv; p++) {
-      uint32_t w1[4], w2[4], w3[4];  // the weights' parts, two a register
+      for (int j = 0; j < 2; j++)
+        x[j] = __builtin_amdgcn_exp2f(fmaf(s[u / kPer][u % kPer * 4 + r + j], c, off));
+      l += x[0] + x[1];
+      uint32_t a, b, d = 0;
+      if (kType == kKvFp16) {
+        split_f16(x[0], x[1], neg, a, b);
+      } else {
+        const float* v = vs + 4 * NG * u + 4 * grp + r;
+        split_bf16(x[0] * v[0], x[1] * v[1], a, b, d);
+      }
+      w[p & 1][0][i] = a;
+      w[p & 1][1][i] = b;
+      w[p & 1][2][i] = d;
+    };
+    auto value = [&](int p, int t) __attribute__((always_inline)) {
+      u32x4 v;
 #pragma unroll
       for (int q = 0; q < 2; q++) {
-        const int u = 2 * p + q;
-        float w[4];
-#pragma unroll
-        for (int r = 0; r < 4; r++)
-          w[r] = __builtin_amdgcn_exp2f(fmaf(s[u / kPer][u % kPer * 4 + r], c, off));
-        sum += (w[0] + w[1]) + (w[2] + w[3]);
-        if (kType == kKvInt8) {
-          const f32x4 v4 = *reinterpret_cast<const f32x4*>(vs + 4 * NG * u + 4 * grp);
-#pragma unroll
-          for (int r = 0; r < 4; r++) w[r] *= v4[r];
-        }
-#pragma unroll
-        for (int r = 0; r < 4; r += 2) {
-          const int i = 2 * q + r / 2;
-          if (kType == kKvFp16)
-            split_f16(w[r], w[r + 1], neg, w1[i], w2[i]);
-          else
-            split_bf16(w[r], w[r + 1], w1[i], w2[i], w3[i]);
-        }
+        const int row = 4 * NG * (2 * p + q) + row0;
+        const uint8_t* src = tile + KvTile<DP>::at(row, NQ / 8 * t + col) + (l16 & 1) * 8;
+        typedef short short4v __attribute__((ext_vector_type(4)));
+        const auto x = __builtin_bit_cast(
+            uint2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                         (__attribute__((address_space(3))) short4v*)src));
+        v[2 * q] = x[0];
+        v[2 * q + 1] = x[1];
       }
+      return v;
+    };
+    u32x4 v[2];
+    v[0] = value(0, 0);
+#pragma unroll
+    for (int i = 0; i < 4; i++) pair(0, i);
+#pragma unroll
+    for (int p = 0; p < kPv; p++)
 #pragma unroll
       for (int t = 0; t < kDt; t++) {
-        u32x4 v;
-#pragma unroll
-        for (int q = 0; q < 2; q++) {
-          const int row = 4 * NG * (2 * p + q) + row0;
-          const uint8_t* src = tile + KvTile<DP>::at(row, NQ / 8 * t + col) + (l16 & 1) * 8;
-          typedef short short4v __attribute__((ext_vector_type(4)));
-          const auto x = __builtin_bit_cast(
-              uint2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                           (__attribute__((address_space(3))) short4v*)src));
-          v[2 * q] = x[0];
-          v[2 * q + 1] = x[1];
-        }
-        const u32x4 a1 = {w1[0], w1[1], w1[2], w1[3]}, a2 = {w2[0], w2[1], w2[2], w2[3]};
+        const int at = p * kDt + t;
+        if (at + 1 < kPv * kDt) v[(at + 1) & 1] = value((at + 1) / kDt, (at + 1) % kDt);
+        __builtin_amdgcn_sched_barrier(0);
+        const u32x4 x = v[at & 1], *y = w[p & 1];
         if (kType == kKvFp16) {
-          o[t] = Mfma<NQ>::mul(f16x8(v), f16x8(a1), o[t]);
-          o[t] = Mfma<NQ>::mul(f16x8(v), f16x8(a2), o[t]);
+          o[t] = Mfma<NQ>::mul(f16x8(x), f16x8(y[0]), o[t]);
+          o[t] = Mfma<NQ>::mul(f16x8(x), f16x8(y[1]), o[t]);
         } else {
-          const u32x4 a3 = {w3[0], w3[1], w3[2], w3[3]};
-          o[t] = Mfma<NQ>::mul(bf16x8(v), bf16x8(a1), o[t]);
-          o[t] = Mfma<NQ>::mul(bf16x8(v), bf16x8(a2), o[t]);
-          o[t] = Mfma<NQ>::mul(bf16x8(v), bf16x8(a3), o[t]);
+          o[t] = Mfma<NQ>::mul(bf16x8(x), bf16x8(y[0]), o[t]);
+          o[t] = Mfma<NQ>::mul(bf16x8(x), bf16x8(y[1]), o[t]);
+          o[t] = Mfma<NQ>::mul(bf16x8(x), bf16x8(y[2]), o[t]);
         }
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          if (p + 1 < kPv && i * kDt / 4 == t) pair(p + 1, i);
+        __builtin_amdgcn_sched_barrier(0);
       }
-    }
-    l += sum;
   }
 
   // Ends the pass: this lane's row sum, NaN where the tiles held pages that are none.
