@@ -37,7 +37,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a) {
   if (sp.splits <= 1) return;  // written already
   const int per = few ? 16 : a.tile_rows, r0 = r / per * per;
   const bool past = too_long(a, sq);
-  const int all = past ? 0 : split_count(a, sq, sp, r0, min(r0 + per, rows));
+  const int all = past ? 0 : split_count(sp, span_of(a, sq, r0, min(r0 + per, rows)));
   const int first = all * part / kWaves, n = all * (part + 1) / kWaves - first;
   const float2* ml = a.part_ml + row * a.row_parts + first;
   const int lanes = D <= 64 ? 16 : D <= 128 ? 32 : 64, sub = lane / lanes, d = lane % lanes * 4;

@@ -11,7 +11,7 @@
 //
 // Arithmetic: the cache's values are fp16 or 8-bit codes, both exact as MFMA operands.
 // q (scaled by a power of two per row) goes in as two fp16, 22 bits, every product
-// twice.  The weights go in as two fp16 beside fp16 values (22 bits, or 2^-40 of the
+// twice.  The weights go in as two fp16 beside fp16 values (22 bits, or 2^-37 of the
 // row's largest), and times the values' scale as three bf16, all of an fp32, beside
 // 8-bit ones: a code of 0 beside the largest weight leaves an element to the smallest.
 // Sums are fp32.  What this cannot hold (infinities and NaN anywhere in a tile, masked
@@ -49,9 +49,12 @@ struct Seq {
   int b, first, n, kv;
 };
 
+// (the same in all lanes)
 __device__ __forceinline__ Seq seq_of(const KvBatch& b, int i) {
-  const int first = cu_at(b, i);
-  return {i, first, max(cu_at(b, i + 1) - first, 0), max(load_global<int>(b.kv_lens + i), 0)};
+  const int first = __builtin_amdgcn_readfirstlane(cu_at(b, i));
+  const int end = __builtin_amdgcn_readfirstlane(cu_at(b, i + 1));
+  const int kv = __builtin_amdgcn_readfirstlane(load_global<int>(b.kv_lens + i));
+  return {i, first, max(end - first, 0), max(kv, 0)};
 }
 
 // A sequence longer than its table row: its tokens are NaN.
@@ -64,11 +67,24 @@ __device__ __forceinline__ int first_seen(const AttnArgs& a, const Seq& s, int i
   return a.window ? (int)max((int64_t)s.kv - s.n + i - a.window + 1, (int64_t)0) : 0;
 }
 
-// Ranges that the rows [r0, r1) of a sequence are split into (0: they see nothing).
-__device__ __forceinline__ int split_count(const AttnArgs& a, const Seq& s, const AttnSplit& sp,
-                                           int r0, int r1) {
+// A run of kRun positions from a multiple of it lies in one page, if pages have as many.
+constexpr int kRunShift = 4, kRun = 1 << kRunShift;
+
+// Positions that the rows [r0, r1) of a sequence read, from the start of a run (of the
+// page's start, where pages are shorter): those before the first that is seen are in its
+// page.
+struct Span {
+  int lo, hi;
+};
+__device__ __forceinline__ Span span_of(const AttnArgs& a, const Seq& s, int r0, int r1) {
   const int lo = first_seen(a, s, r0 / a.group), hi = s.kv - s.n + (r1 - 1) / a.group + 1;
-  return hi <= lo ? 0 : min(sp.splits, (hi - lo - 1) / sp.chunk + 1);
+  if (hi <= lo) return {0, 0};
+  return {lo & -(1 << min(a.c.page_shift, kRunShift)), hi};
+}
+
+// Ranges that a span is split into (0: nothing is seen).
+__device__ __forceinline__ int split_count(const AttnSplit& sp, const Span& x) {
+  return x.hi <= x.lo ? 0 : min(sp.splits, (x.hi - x.lo - 1) / sp.chunk + 1);
 }
 
 // One row by a wave, plainly, sums in 64 bits.
@@ -149,11 +165,18 @@ struct KvTile {
   __device__ static __forceinline__ int at(int r, int c) { return r * kPitch + ((c ^ swz(r)) << 4); }
 };
 
-__device__ inline const uint32_t kZero16[4] __attribute__((aligned(16))) = {0, 0, 0, 0};
-
-// Lane i's 16 bytes at `src` to lds + 16 i, asynchronously; counted by vmcnt, which the
-// caller waits for.  (Not the builtin: the compiler then has every transposing read of
-// LDS wait for all such copies, the next tile's too.)
+// Lane i's 16 bytes at base + off to lds + 16 i, asynchronously; counted by vmcnt, which
+// the caller waits for.  (Not the builtin: the compiler then has every transposing read
+// of LDS wait for all such copies, the next tile's too.)
+__device__ __forceinline__ void dma16(const void* base, uint32_t off, uint8_t* lds) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)lds;
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+               :
+               : "{m0}"(at), "v"(off), "s"(base)
+               : "memory");
+#endif
+}
 __device__ __forceinline__ void dma16(const void* src, uint8_t* lds) {
 #if defined(__HIP_DEVICE_COMPILE__)
   const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)lds;
@@ -205,17 +228,14 @@ __device__ __forceinline__ u32x4 codes_to_f16(uint2 x) {
   return unpack8_bytes(x.x ^ 0x80808080u, x.y ^ 0x80808080u);
 }
 
-// Where a position's row lies: its page (0 for one that is none, with *bad set).
-struct Place {
-  int page, tok;  // tok: row within the page
-};
-__device__ __forceinline__ Place place(const AttnArgs& a, int g, int p, int id, bool& bad) {
-  const bool ok = id >= 0 && id < a.c.pages;
-  bad |= !ok;
-  return {ok ? id : 0, (g << a.c.page_shift) + (p & ((1 << a.c.page_shift) - 1))};
-}
 __device__ __forceinline__ int page_id(const AttnArgs& a, int b, int p) {
   return load_global<int>(a.b.page_table + (size_t)b * a.b.width + (p >> a.c.page_shift));
+}
+// The page to read for an entry of the table: 0, with *bad set, where it is none.
+__device__ __forceinline__ int page_of(const AttnArgs& a, int id, bool& bad) {
+  const bool ok = id >= 0 && id < a.c.pages;
+  bad |= !ok;
+  return ok ? id : 0;
 }
 
 // --- one wave's rows ------------------------------------------------------------------
@@ -261,8 +281,9 @@ struct Mfma<16> {
 };
 
 // The weights go in as 2^kTop at a row's largest score when its reference was last
-// moved, and at most as 2^(kTop + kSlack): with fp16 values up to fp16's end, as its
-// smallest step then is 2^-40 of the largest weight.
+// moved, and at most as 2^(kTop + kSlack), where fp16 ends (its smallest step is then
+// between 2^-36 and 2^-40 of the largest weight).  The more slack, the fewer moves, each
+// of which takes o times a factor.
 
 template <int kType, int NQ, int DP, int BK>
 struct Rows {
@@ -272,7 +293,8 @@ struct Rows {
   static constexpr int kQuads = BK / (4 * NG);  // of keys a lane holds: 4 NG u + 4 group + 0..3
   static constexpr int kPv = kQuads / 2;      // steps of the second product
   static constexpr int kDt = DP / NQ;
-  static constexpr float kTop = kType == kKvFp16 ? 15.0f : 0.0f, kSlack = 0.9f;
+  static constexpr float kTop = kType == kKvFp16 ? 12.0f : 0.0f;
+  static constexpr float kSlack = kType == kKvFp16 ? 3.9f : 16.0f;
   typedef typename Mfma<NQ>::acc acc;
 
   half8 qh[kSteps], ql[kSteps];

@@ -44,8 +44,8 @@ __global__ void __launch_bounds__(256, 2) attn_few_kernel(AttnArgs a) {
 
   for (int r0 = 0; r0 < rows; r0 += kQ) {
     const int r1 = min(r0 + kQ, rows);
-    int lo = first_seen(a, sq, r0 / G), hi = sq.kv - sq.n + (r1 - 1) / G + 1;
-    if (past || hi < lo) hi = lo;
+    const Span span = span_of(a, sq, r0, r1);
+    int lo = past ? 0 : span.lo, hi = past ? 0 : span.hi;
     if (a.fs.splits > 1) {
       const int64_t start = lo + (int64_t)split * a.fs.chunk;
       if (start >= hi && split) continue;
@@ -70,41 +70,41 @@ __global__ void __launch_bounds__(256, 2) attn_few_kernel(AttnArgs a) {
       pid = page_id(a, b, min(p0 + lane % kKeys, hi - 1));
     };
     auto issue = [&](int p0, int buf) __attribute__((always_inline)) {
+      const int mask = (1 << a.c.page_shift) - 1, item = kType == kKvFp16 ? 2 : 1;
 #pragma unroll
       for (int i = 0; i < 2; i++) {
         const int r = kQ * i + col;
-        const Place pl = place(a, g, min(p0 + r, hi - 1), __shfl(pid, r, 64), bad);
-        const size_t ki = (size_t)pl.page * a.c.k_page + (size_t)pl.tok * D + 8 * grp;
+        const int pg = page_of(a, __shfl(pid, r, 64), bad);
+        const uint8_t* src = (const uint8_t*)a.c.k +
+                             (((size_t)g << a.c.page_shift) * D + (size_t)pg * a.c.k_page) * item +
+                             __umul24(min(p0 + r, hi - 1) & mask, D) * item;
 #pragma unroll
         for (int s = 0; s < R::kSteps; s++) {
-          const bool in = 32 * s + 8 * grp < D;
-          if (kType == kKvFp16) {
-            kf[i][s] = half8{};
-            if (in) kf[i][s] = load_global<half8>((const _Float16*)a.c.k + ki + 32 * s);
-          } else {
-            kc[i][s] = make_uint2(0, 0);
-            if (in) kc[i][s] = load_global<uint2>((const int8_t*)a.c.k + ki + 32 * s);
-          }
+          const int d = 32 * s + 8 * grp < D ? 32 * s + 8 * grp : 0;  // (products with zeros)
+          if (kType == kKvFp16)
+            kf[i][s] = load_global<half8>(src + 2 * d);
+          else
+            kc[i][s] = load_global<uint2>(src + d);
         }
       }
 #pragma unroll
       for (int i = 0; i < T::kN; i++) {
-        const int r = (i * 64 + lane) / L::kCh, ch = ((i * 64 + lane) % L::kCh) ^ L::swz(r);
-        const Place pl = place(a, g, min(p0 + r, hi - 1), __shfl(pid, r, 64), bad);
-        const size_t vi = (size_t)pl.page * a.c.v_page + (size_t)pl.tok * D + 8 * ch;
-        const bool in = 8 * ch < D;
-        if (kType == kKvFp16) {
-          dma16(in ? (const void*)((const _Float16*)a.c.v + vi) : kZero16,
-                vbuf + buf * T::kBytes + i * 1024);
-        } else {
-          vc[i] = make_uint2(0, 0);
-          if (in) vc[i] = load_global<uint2>((const int8_t*)a.c.v + vi);
-        }
+        const int r = (i * 64 + lane) / L::kCh;
+        const int ch = 8 * (((i * 64 + lane) % L::kCh) ^ L::swz(r));
+        const int pg = page_of(a, __shfl(pid, r, 64), bad);
+        const uint8_t* src = (const uint8_t*)a.c.v +
+                             (((size_t)g << a.c.page_shift) * D + (size_t)pg * a.c.v_page) * item +
+                             (__umul24(min(p0 + r, hi - 1) & mask, D) + (ch < D ? ch : 0)) * item;
+        if (kType == kKvFp16)
+          dma16(src, vbuf + buf * T::kBytes + i * 1024);
+        else
+          vc[i] = load_global<uint2>(src);
       }
       if (kType == kKvInt8) {
-        const Place pl = place(a, g, min(p0 + lane % kKeys, hi - 1), pid, bad);
-        kss = load_global<float>(a.c.k_scale + (size_t)pl.page * a.c.ks_page + pl.tok);
-        vss = load_global<float>(a.c.v_scale + (size_t)pl.page * a.c.vs_page + pl.tok);
+        const int pg = page_of(a, pid, bad);
+        const int tok = (g << a.c.page_shift) + (min(p0 + lane % kKeys, hi - 1) & mask);
+        kss = load_global<float>(a.c.k_scale + (size_t)pg * a.c.ks_page + tok);
+        vss = load_global<float>(a.c.v_scale + (size_t)pg * a.c.vs_page + tok);
       }
     };
 

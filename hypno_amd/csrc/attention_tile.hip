@@ -27,11 +27,8 @@ __global__ void __launch_bounds__(256, 2) attn_tile_kernel(AttnArgs a) {
   const int KV = a.c.kv_heads, G = a.group, D = a.c.head_dim;
   // The kv head goes fastest (work-groups of one head on one XCD, where it has
   // eight), the rows with the most positions first.
-  int id = blockIdx.x;
-  const int g = id % KV;
-  id /= KV;
-  const int split = id % a.ts.splits;
-  const int slot = gridDim.x / (KV * a.ts.splits) - 1 - id / a.ts.splits;
+  const int g = blockIdx.x % KV, split = blockIdx.x / KV % a.ts.splits;
+  const int slot = (gridDim.x - 1 - blockIdx.x) / (KV * a.ts.splits);
   const int b = find_seq(a.b, slot, G, T::kRows);
   if (b < 0 || b >= a.b.batch) return;
   const Seq sq = seq_of(a.b, b);
@@ -40,8 +37,8 @@ __global__ void __launch_bounds__(256, 2) attn_tile_kernel(AttnArgs a) {
   if (r0 < 0 || r0 >= rows || rows <= a.few) return;
   const int r1 = min(r0 + T::kRows, rows);
   const bool past = too_long(a, sq);
-  int lo = first_seen(a, sq, r0 / G), hi = sq.kv - sq.n + (r1 - 1) / G + 1;
-  if (past || hi < lo) hi = lo;
+  const Span span = span_of(a, sq, r0, r1);
+  int lo = past ? 0 : span.lo, hi = past ? 0 : span.hi;
   if (a.ts.splits > 1) {
     const int64_t start = lo + (int64_t)split * a.ts.chunk;
     if (start >= hi && split) return;
@@ -70,49 +67,90 @@ __global__ void __launch_bounds__(256, 2) attn_tile_kernel(AttnArgs a) {
   uint8_t* const kbuf = smem;
   uint8_t* const vbuf = smem + 2 * T::kBytes;
   float* const scales = reinterpret_cast<float*>(smem + 4 * T::kBytes);
-  int ids[T::kN], sid = 0;      // pages of this thread's pieces; of its scale
+  // Wave w brings rows BK / 4 w and on of a tile, 16-byte piece by piece.  Where pages
+  // are no shorter, these lie in one, `id`; otherwise each piece's page is in `ids`.
+  // (Rows past the end: the last row again, whose weights are 0.)
+  constexpr int kMine = BK / 4;
+  const bool one = (1 << a.c.page_shift) >= kRun;
+  const int mask = (1 << a.c.page_shift) - 1, item = kType == kKvFp16 ? 2 : 1;
+  int id = 0, ids[T::kN];  // (with `ids`, id: of the lane's scale)
   uint2 kr[T::kN], vr[T::kN];   // 8-bit codes on their way
   float sr = 0.0f;
+  const int srow = wave * kMine + lane % kMine;
+  const bool sk = lane < kMine;
+  int rr[T::kN], ch[T::kN];
+#pragma unroll
+  for (int i = 0; i < T::kN; i++) {
+    const int j = (wave * T::kN + i) * 64 + lane;
+    rr[i] = j / L::kCh;
+    ch[i] = 8 * ((j % L::kCh) ^ L::swz(rr[i]));
+    if (ch[i] >= D) ch[i] = 0;  // (columns past D: products with zeros, outputs not used)
+  }
   auto look_up = [&](int p0) __attribute__((always_inline)) {
+    if (one) {
+      id = load_const<int>(a.b.page_table + (size_t)b * a.b.width +
+                            (min(p0 + wave * kMine, hi - 1) >> a.c.page_shift));
+    } else {
+#pragma unroll
+      for (int i = 0; i < T::kN; i++) ids[i] = page_id(a, b, min(p0 + rr[i], hi - 1));
+      if (kType == kKvInt8) id = page_id(a, b, min(p0 + srow, hi - 1));
+    }
+  };
+  const uint8_t* const kg = (const uint8_t*)a.c.k + ((size_t)g << a.c.page_shift) * D * item;
+  const uint8_t* const vg = (const uint8_t*)a.c.v + ((size_t)g << a.c.page_shift) * D * item;
+  const float* const ksg = a.c.k_scale + ((size_t)g << a.c.page_shift);
+  const float* const vsg = a.c.v_scale + ((size_t)g << a.c.page_shift);
+  auto issue = [&](int p0, int buf) __attribute__((always_inline)) {
+    const int page = kType == kKvInt8 || one ? page_of(a, id, bad) : 0;
+    uint32_t off[T::kN];
 #pragma unroll
     for (int i = 0; i < T::kN; i++)
-      ids[i] = page_id(a, b, min(p0 + (i * 256 + tid) / L::kCh, hi - 1));
-    if (kType == kKvInt8) sid = page_id(a, b, min(p0 + tid % BK, hi - 1));
-  };
-  auto issue = [&](int p0, int buf) __attribute__((always_inline)) {
+      off[i] = (__umul24(min(p0 + rr[i], hi - 1) & mask, D) + ch[i]) * item;
+    uint8_t* const kd = kbuf + buf * T::kBytes + wave * T::kN * 1024;
+    uint8_t* const vd = kd + 2 * T::kBytes;
+    if (one) {
+      const int pg = __builtin_amdgcn_readfirstlane(page);
+      const uint8_t* const kp = kg + (size_t)pg * a.c.k_page * item;
+      const uint8_t* const vp = vg + (size_t)pg * a.c.v_page * item;
 #pragma unroll
-    for (int i = 0; i < T::kN; i++) {
-      const int r = (i * 256 + tid) / L::kCh, ch = ((i * 256 + tid) % L::kCh) ^ L::swz(r);
-      const Place pl = place(a, g, min(p0 + r, hi - 1), ids[i], bad);
-      const size_t ki = (size_t)pl.page * a.c.k_page + (size_t)pl.tok * D + 8 * ch;
-      const size_t vi = (size_t)pl.page * a.c.v_page + (size_t)pl.tok * D + 8 * ch;
-      const bool in = 8 * ch < D;
-      if (kType == kKvFp16) {
-        const int at = (i * 256 + wave * 64) * 16 + buf * T::kBytes;
-        dma16(in ? (const void*)((const _Float16*)a.c.k + ki) : kZero16, kbuf + at);
-        dma16(in ? (const void*)((const _Float16*)a.c.v + vi) : kZero16, vbuf + at);
-      } else {
-        kr[i] = vr[i] = make_uint2(0, 0);
-        if (in) {
-          kr[i] = load_global<uint2>((const int8_t*)a.c.k + ki);
-          vr[i] = load_global<uint2>((const int8_t*)a.c.v + vi);
+      for (int i = 0; i < T::kN; i++) {
+        if (kType == kKvFp16) {
+          dma16(kp, off[i], kd + i * 1024);
+          dma16(vp, off[i], vd + i * 1024);
+        } else {
+          kr[i] = load_global<uint2>(kp + off[i]);
+          vr[i] = load_global<uint2>(vp + off[i]);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < T::kN; i++) {
+        const int pg = page_of(a, ids[i], bad);
+        const uint8_t* const kp = kg + (size_t)pg * a.c.k_page * item + off[i];
+        const uint8_t* const vp = vg + (size_t)pg * a.c.v_page * item + off[i];
+        if (kType == kKvFp16) {
+          dma16(kp, kd + i * 1024);
+          dma16(vp, vd + i * 1024);
+        } else {
+          kr[i] = load_global<uint2>(kp);
+          vr[i] = load_global<uint2>(vp);
         }
       }
     }
-    if (kType == kKvInt8 && tid < 2 * BK) {
-      const Place pl = place(a, g, min(p0 + tid % BK, hi - 1), sid, bad);
-      sr = tid < BK ? load_global<float>(a.c.k_scale + (size_t)pl.page * a.c.ks_page + pl.tok)
-                    : load_global<float>(a.c.v_scale + (size_t)pl.page * a.c.vs_page + pl.tok);
+    if (kType == kKvInt8 && lane < 2 * kMine) {
+      const int tok = min(p0 + srow, hi - 1) & mask;
+      sr = load_global<float>((sk ? ksg + (size_t)page * a.c.ks_page
+                                  : vsg + (size_t)page * a.c.vs_page) + tok);
     }
   };
   auto store = [&](int buf) __attribute__((always_inline)) {  // 8-bit: what `issue` loaded
 #pragma unroll
     for (int i = 0; i < T::kN; i++) {
-      const int at = (i * 256 + tid) * 16 + buf * T::kBytes;
+      const int at = ((wave * T::kN + i) * 64 + lane) * 16 + buf * T::kBytes;
       *reinterpret_cast<u32x4*>(kbuf + at) = codes_to_f16(kr[i]);
       *reinterpret_cast<u32x4*>(vbuf + at) = codes_to_bf16(vr[i]);
     }
-    if (tid < 2 * BK) scales[buf * 2 * BK + tid] = sr;
+    if (lane < 2 * kMine) scales[(buf * 2 + !sk) * BK + srow] = sr;
   };
 
   const int tiles = (hi - lo + BK - 1) / BK;
@@ -146,7 +184,7 @@ __global__ void __launch_bounds__(256, 2) attn_tile_kernel(AttnArgs a) {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
   };
   const int full0 = some ? min(max(all_lo - lo + BK - 1, 0) / BK, tiles) : tiles;
-  const int full1 = some ? max(full0, (all_hi + 1 - lo) / BK) : tiles;
+  const int full1 = some ? max(full0, min((all_hi + 1 - lo) / BK, tiles)) : tiles;
   for (int i = 0, run = 0; run < 2; run++) {
     if (run)
       for (; i < full1; i++) step(std::false_type(), i);
