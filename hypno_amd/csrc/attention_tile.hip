@@ -18,7 +18,8 @@ struct Tile {
   static constexpr int kLds = 4 * kBytes + (kType == kKvInt8 ? 4 * BK * 4 : 0);
 };
 
-template <int kType, int NQ, int DP, int BK>
+// kOne: pages have kRun positions or more.
+template <int kType, int NQ, int DP, int BK, bool kOne>
 __global__ void __launch_bounds__(256, 2) attn_tile_kernel(AttnArgs a) {
   typedef Tile<kType, NQ, DP, BK> T;
   typedef KvTile<DP> L;
@@ -67,11 +68,10 @@ __global__ void __launch_bounds__(256, 2) attn_tile_kernel(AttnArgs a) {
   uint8_t* const kbuf = smem;
   uint8_t* const vbuf = smem + 2 * T::kBytes;
   float* const scales = reinterpret_cast<float*>(smem + 4 * T::kBytes);
-  // Wave w brings rows BK / 4 w and on of a tile, 16-byte piece by piece.  Where pages
-  // are no shorter, these lie in one, `id`; otherwise each piece's page is in `ids`.
+  // Wave w brings rows BK / 4 w and on of a tile, 16-byte piece by piece.  With
+  // kOne these lie in one page, `id`; otherwise each piece's page is in `ids`.
   // (Rows past the end: the last row again, whose weights are 0.)
   constexpr int kMine = BK / 4;
-  const bool one = (1 << a.c.page_shift) >= kRun;
   const int mask = (1 << a.c.page_shift) - 1, item = kType == kKvFp16 ? 2 : 1;
   int id = 0, ids[T::kN];  // (with `ids`, id: of the lane's scale)
   uint2 kr[T::kN], vr[T::kN];   // 8-bit codes on their way
@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(256, 2) attn_tile_kernel(AttnArgs a) {
     if (ch[i] >= D) ch[i] = 0;  // (columns past D: products with zeros, outputs not used)
   }
   auto look_up = [&](int p0) __attribute__((always_inline)) {
-    if (one) {
+    if (kOne) {
       id = load_const<int>(a.b.page_table + (size_t)b * a.b.width +
                             (min(p0 + wave * kMine, hi - 1) >> a.c.page_shift));
     } else {
@@ -101,14 +101,14 @@ __global__ void __launch_bounds__(256, 2) attn_tile_kernel(AttnArgs a) {
   const float* const ksg = a.c.k_scale + ((size_t)g << a.c.page_shift);
   const float* const vsg = a.c.v_scale + ((size_t)g << a.c.page_shift);
   auto issue = [&](int p0, int buf) __attribute__((always_inline)) {
-    const int page = kType == kKvInt8 || one ? page_of(a, id, bad) : 0;
+    const int page = kType == kKvInt8 || kOne ? page_of(a, id, bad) : 0;
     uint32_t off[T::kN];
 #pragma unroll
     for (int i = 0; i < T::kN; i++)
       off[i] = (__umul24(min(p0 + rr[i], hi - 1) & mask, D) + ch[i]) * item;
     uint8_t* const kd = kbuf + buf * T::kBytes + wave * T::kN * 1024;
     uint8_t* const vd = kd + 2 * T::kBytes;
-    if (one) {
+    if (kOne) {
       const int pg = __builtin_amdgcn_readfirstlane(page);
       const uint8_t* const kp = kg + (size_t)pg * a.c.k_page * item;
       const uint8_t* const vp = vg + (size_t)pg * a.c.v_page * item;
@@ -232,16 +232,22 @@ __global__ void __launch_bounds__(256, 2) attn_tile_kernel(AttnArgs a) {
   attn_rows(a, sq, g, w0, again & ((1ull << NQ) - 1));
 }
 
-template <int kType, int NQ, int DP, int BK>
-hipError_t run(const AttnArgs& a, hipStream_t s) {
+template <int kType, int NQ, int DP, int BK, bool kOne>
+hipError_t launch(const AttnArgs& a, hipStream_t s) {
   typedef Tile<kType, NQ, DP, BK> T;
   const size_t slots = (size_t)a.b.tokens * a.group / T::kRows + a.b.batch;
   const size_t grid = slots * a.c.kv_heads * a.ts.splits;
   if (grid > 0xFFFFFF) return hipErrorInvalidValue;
-  const hipError_t e = set_lds_limit((const void*)attn_tile_kernel<kType, NQ, DP, BK>, T::kLds);
+  const hipError_t e = set_lds_limit((const void*)attn_tile_kernel<kType, NQ, DP, BK, kOne>, T::kLds);
   if (e != hipSuccess) return e;
-  attn_tile_kernel<kType, NQ, DP, BK><<<(unsigned)grid, 256, T::kLds, s>>>(a);
+  attn_tile_kernel<kType, NQ, DP, BK, kOne><<<(unsigned)grid, 256, T::kLds, s>>>(a);
   return hipGetLastError();
+}
+
+template <int kType, int NQ, int DP, int BK>
+hipError_t run(const AttnArgs& a, hipStream_t s) {
+  return a.c.page_shift >= kRunShift ? launch<kType, NQ, DP, BK, true>(a, s)
+                                     : launch<kType, NQ, DP, BK, false>(a, s);
 }
 
 }  // namespace
