@@ -108,6 +108,7 @@ int up(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 AttnPlan attn_plan(const KvCache& c, const KvBatch& b, int heads, int window, int64_t max_kv,
                    int num_cus) {
   AttnPlan p = {};
+  p.cus = num_cus;
   const int G = heads / c.kv_heads;
   const int64_t rows = (int64_t)b.tokens * G;
   p.tile_rows = c.head_dim <= 128 ? 128 : 64;
@@ -150,7 +151,7 @@ hipError_t launch_paged_attention(const AttnPlan& p, float* out, const float* q,
                                   int heads, const KvCache& c, const KvBatch& b, float scale,
                                   int window, void* ws, hipStream_t s) {
   AttnArgs a = {c, b, out, q, q_stride, heads, heads / c.kv_heads, window, scale,
-                p.few, p.tile_rows, p.fs, p.ts, std::max(p.fs.splits, p.ts.splits),
+                p.few, p.tile_rows, p.fs, p.ts, p.cus, std::max(p.fs.splits, p.ts.splits),
                 nullptr, nullptr};
   if (!ws) a.fs = a.ts = {1, 0x7FFFFFFF};
   a.part_ml = reinterpret_cast<float2*>(ws);

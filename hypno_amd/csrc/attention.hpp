@@ -39,6 +39,7 @@ struct AttnArgs {
   int few;                // sequences of at most so many rows are attn_few_kernel's
   int tile_rows;          // rows of a work-group of the other
   AttnSplit fs, ts;       // of attn_few_kernel and attn_tile_kernel
+  int cus;
   int row_parts;          // the larger of both splits
   float* part_o;          // [token][head][row_parts][head_dim], if that is above 1
   float2* part_ml;        // [token][head][row_parts]: maximum (log2), sum
@@ -445,29 +446,37 @@ struct Rows {
       }
       return v;
     };
-    u32x4 v[2];
-    v[0] = value(0, 0);
+    // (two accumulators in turn: a product on the one before it would wait for it)
+    constexpr int kGroups = (kDt + 1) / 2;
+    u32x4 v[2][2];
+    auto values_of = [&](int at) __attribute__((always_inline)) {
+#pragma unroll
+      for (int j = 0; j < 2; j++)
+        if (at % kGroups * 2 + j < kDt) v[at & 1][j] = value(at / kGroups, at % kGroups * 2 + j);
+    };
+    values_of(0);
 #pragma unroll
     for (int i = 0; i < 4; i++) pair(0, i);
 #pragma unroll
     for (int p = 0; p < kPv; p++)
 #pragma unroll
-      for (int t = 0; t < kDt; t++) {
-        const int at = p * kDt + t;
-        if (at + 1 < kPv * kDt) v[(at + 1) & 1] = value((at + 1) / kDt, (at + 1) % kDt);
+      for (int g = 0; g < kGroups; g++) {
+        const int at = p * kGroups + g;
+        if (at + 1 < kPv * kGroups) values_of(at + 1);
         __builtin_amdgcn_sched_barrier(0);
-        const u32x4 x = v[at & 1], *y = w[p & 1];
-        if (kType == kKvFp16) {
-          o[t] = Mfma<NQ>::mul(f16x8(x), f16x8(y[0]), o[t]);
-          o[t] = Mfma<NQ>::mul(f16x8(x), f16x8(y[1]), o[t]);
-        } else {
-          o[t] = Mfma<NQ>::mul(bf16x8(x), bf16x8(y[0]), o[t]);
-          o[t] = Mfma<NQ>::mul(bf16x8(x), bf16x8(y[1]), o[t]);
-          o[t] = Mfma<NQ>::mul(bf16x8(x), bf16x8(y[2]), o[t]);
-        }
+#pragma unroll
+        for (int part = 0; part < (kType == kKvFp16 ? 2 : 3); part++)
+#pragma unroll
+          for (int j = 0; j < 2; j++) {
+            const int t = 2 * g + j;
+            if (t >= kDt) continue;
+            const u32x4 x = v[at & 1][j], y = w[p & 1][part];
+            o[t] = kType == kKvFp16 ? Mfma<NQ>::mul(f16x8(x), f16x8(y), o[t])
+                                    : Mfma<NQ>::mul(bf16x8(x), bf16x8(y), o[t]);
+          }
 #pragma unroll
         for (int i = 0; i < 4; i++)
-          if (p + 1 < kPv && i * kDt / 4 == t) pair(p + 1, i);
+          if (p + 1 < kPv && i * kGroups / 4 == g) pair(p + 1, i);
         __builtin_amdgcn_sched_barrier(0);
       }
   }

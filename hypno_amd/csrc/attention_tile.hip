@@ -26,10 +26,13 @@ __global__ void __launch_bounds__(256, 2) attn_tile_kernel(AttnArgs a) {
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int KV = a.c.kv_heads, G = a.group, D = a.c.head_dim;
-  // The kv head goes fastest (work-groups of one head on one XCD, where it has
-  // eight), the rows with the most positions first.
-  const int g = blockIdx.x % KV, split = blockIdx.x / KV % a.ts.splits;
-  const int slot = (gridDim.x - 1 - blockIdx.x) / (KV * a.ts.splits);
+  // The kv head goes fastest (work-groups of one head on one XCD, where it has eight),
+  // the rows with the most positions first.  Where all work-groups run at once, two a
+  // CU, the second half goes up again: a long one beside a short one.
+  const int g = blockIdx.x % KV, all = gridDim.x / KV, half = a.cus / KV;
+  int at = blockIdx.x / KV;
+  if (all - a.b.batch * a.ts.splits <= 2 * half && at >= half) at = all - 1 - (at - half);
+  const int split = at % a.ts.splits, slot = (all - 1 - at) / a.ts.splits;
   const int b = find_seq(a.b, slot, G, T::kRows);
   if (b < 0 || b >= a.b.batch) return;
   const Seq sq = seq_of(a.b, b);

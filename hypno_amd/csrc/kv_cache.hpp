@@ -75,6 +75,7 @@ struct AttnSplit {
 struct AttnPlan {
   int few;        // sequences of at most so many rows go to attn_few_kernel
   int tile_rows;  // rows of a work-group of attn_tile_kernel
+  int cus;
   AttnSplit fs, ts;
   size_t bytes, ml_bytes;
 };
