@@ -119,13 +119,13 @@ AttnPlan attn_plan(const KvCache& c, const KvBatch& b, int heads, int window, in
   p.few = only_few ? 0x7FFFFFFF : only_tile ? 0 : 16;
   const int64_t room = (int64_t)b.width << c.page_shift;
   const int64_t kv = std::max<int64_t>(1, max_kv ? std::min(max_kv, room) : room);
-  // Ranges so that there are about four work-groups for each one that the chip holds
-  // at a time, of 128 positions at least.
+  // Ranges of 128 positions at least, so that one sequence has a work-group for each one
+  // that the chip holds at a time, and several up to eight, for lengths that differ.
   p.fs = {1, 0x7FFFFFFF};
   if (p.few) {
     const int64_t seen = window ? std::min<int64_t>(kv, (int64_t)window + 16) : kv;
     const int64_t pairs = (int64_t)b.batch * c.kv_heads;
-    const int64_t want = std::max<int64_t>(1, (b.batch > 1 ? 8 : 2) * num_cus / pairs);
+    const int64_t want = std::max<int64_t>(1, (b.batch > 1 ? 16 : 2) * num_cus / pairs);
     const int64_t chunk = std::max<int64_t>(128, (up(seen, want) + 127) / 128 * 128);
     p.fs.splits = up(seen, chunk);
     p.fs.chunk = (int)std::min<int64_t>(chunk, 0x7FFFFFFF);

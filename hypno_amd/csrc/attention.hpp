@@ -217,8 +217,8 @@ __device__ __forceinline__ u32x4 codes_to_bf16(uint2 x) {
   u32x4 r;
 #pragma unroll
   for (int i = 0; i < 4; i++) {
-    const uint32_t u = ((i < 2 ? x.x : x.y) ^ 0x80808080u) >> 16 * (i % 2);
-    const float a = (float)(u & 0xFFu) - 128.0f, b = (float)(u >> 8 & 0xFFu) - 128.0f;
+    const int u = (int)((i < 2 ? x.x : x.y) >> 16 * (i % 2));
+    const float a = (float)(int8_t)u, b = (float)(int8_t)(u >> 8);
     r[i] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
   }
   return r;

@@ -1,16 +1,19 @@
 // Attention for sequences with few rows (single tokens, drafts): a work-group takes
 // one kv head of a sequence and a range of its positions; its four waves run through
-// tiles of 32 keys each on their own, 16 rows at a time, and add up at the end.
+// tiles of keys on their own, 16 rows at a time, and add up at the end.
 #include "attention.hpp"
 
 namespace hypno {
 
 namespace {
 
-constexpr int kQ = 16, kKeys = 32;
+constexpr int kQ = 16;
 
 template <int kType, int DP>
 struct Few {
+  static constexpr int kKeys = 32;
+  static constexpr int kGroups = DP > 128 ? 1 : 2;  // a CU
+  static constexpr int kRuns = kKeys / kRun;
   static constexpr int kBytes = kKeys * DP * 2;        // V of one tile in LDS
   static constexpr int kN = kKeys * DP / 8 / 64;       // 16-byte pieces of it a lane
   static constexpr int kBufs = kType == kKvFp16 ? 2 : 1;
@@ -20,20 +23,21 @@ struct Few {
   static constexpr int kWave = kStage > kOut ? kStage : kOut;
 };
 
-template <int kType, int DP>
-__global__ void __launch_bounds__(256, 2) attn_few_kernel(AttnArgs a) {
+// kOne: pages have kRun positions or more.
+template <int kType, int DP, bool kOne>
+__global__ void __launch_bounds__(256, (Few<kType, DP>::kGroups)) attn_few_kernel(AttnArgs a) {
   typedef Few<kType, DP> T;
+  constexpr int kKeys = T::kKeys, kRuns = T::kRuns, kVs = T::kN / kRuns;
   typedef KvTile<DP> L;
   typedef Rows<kType, kQ, DP, kKeys> R;
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   __shared__ uint32_t again;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int KV = a.c.kv_heads, G = a.group, D = a.c.head_dim;
-  int id = blockIdx.x;
-  const int g = id % KV;
-  id /= KV;
-  const int split = id % a.fs.splits;
-  const Seq sq = seq_of(a.b, id / a.fs.splits);
+  // The kv head goes fastest and the range slowest: the last ranges, which the shorter
+  // sequences do not have, come last.
+  const int g = blockIdx.x % KV, split = blockIdx.x / KV / a.b.batch;
+  const Seq sq = seq_of(a.b, blockIdx.x / KV % a.b.batch);
   const int rows = sq.n * G, b = sq.b;
   if (rows > a.few) return;
   const bool past = too_long(a, sq);
@@ -41,6 +45,21 @@ __global__ void __launch_bounds__(256, 2) attn_few_kernel(AttnArgs a) {
   uint8_t* const vbuf = smem + wave * T::kWave;
   float* const ks = reinterpret_cast<float*>(vbuf + T::kBufs * T::kBytes);
   float* const vs = ks + kKeys;
+
+  const int mask = (1 << a.c.page_shift) - 1, item = kType == kKvFp16 ? 2 : 1;
+  const uint8_t* const kg = (const uint8_t*)a.c.k + ((size_t)g << a.c.page_shift) * D * item;
+  const uint8_t* const vg = (const uint8_t*)a.c.v + ((size_t)g << a.c.page_shift) * D * item;
+  // A lane's columns of a K row, and its rows and columns of 16 V rows (those past D: the
+  // row's first, whose products are with zeros or not used).
+  int kcol[R::kSteps], vrow[kVs], vcol[kVs];
+#pragma unroll
+  for (int s = 0; s < R::kSteps; s++) kcol[s] = 32 * s + 8 * grp < D ? 32 * s + 8 * grp : 0;
+#pragma unroll
+  for (int i = 0; i < kVs; i++) {
+    vrow[i] = (i * 64 + lane) / L::kCh;
+    const int c = 8 * (((i * 64 + lane) % L::kCh) ^ L::swz(vrow[i]));
+    vcol[i] = c < D ? c : 0;
+  }
 
   for (int r0 = 0; r0 < rows; r0 += kQ) {
     const int r1 = min(r0 + kQ, rows);
@@ -58,53 +77,76 @@ __global__ void __launch_bounds__(256, 2) attn_few_kernel(AttnArgs a) {
     const int seen_lo = first_seen(a, sq, ti), seen_hi = min(sq.kv - sq.n + ti, hi - 1);
     const int all_lo = first_seen(a, sq, (r1 - 1) / G);
     const int all_hi = min(sq.kv - sq.n + r0 / G, hi - 1);
-    R x;
-    x.init(r0 + col < rows ? a.q + (size_t)t * a.q_stride + (size_t)h * D : nullptr, D, a.scale);
-
     bool bad = false;
-    int pid = 0;                 // page of key lane % 32 of the next tile
-    half8 kf[2][R::kSteps];      // K of the next tile: keys 16 i + col, pieces 4 s + grp
-    uint2 kc[2][R::kSteps], vc[T::kN];  // 8-bit: its codes, and V's
+    // Pages of the next tile's keys: kOne: of its runs; else the lane's.
+    int pid[kRuns] = {};
+    half8 kf[kRuns][R::kSteps];     // K of the next tile: keys 16 i + col, columns kcol
+    uint2 kc[kRuns][R::kSteps], vc[T::kN];  // 8-bit: its codes, and V's
     float kss = 0.0f, vss = 0.0f;
     auto look_up = [&](int p0) __attribute__((always_inline)) {
-      pid = page_id(a, b, min(p0 + lane % kKeys, hi - 1));
+      if (kOne) {
+#pragma unroll
+        for (int i = 0; i < kRuns; i++)
+          pid[i] = load_const<int>(a.b.page_table + (size_t)b * a.b.width +
+                                   (min(p0 + kRun * i, hi - 1) >> a.c.page_shift));
+      } else {
+        pid[0] = page_id(a, b, min(p0 + lane % kKeys, hi - 1));
+      }
     };
     auto issue = [&](int p0, int buf) __attribute__((always_inline)) {
-      const int mask = (1 << a.c.page_shift) - 1, item = kType == kKvFp16 ? 2 : 1;
+      int pg[kRuns] = {};
 #pragma unroll
-      for (int i = 0; i < 2; i++) {
-        const int r = kQ * i + col;
-        const int pg = page_of(a, __shfl(pid, r, 64), bad);
-        const uint8_t* src = (const uint8_t*)a.c.k +
-                             (((size_t)g << a.c.page_shift) * D + (size_t)pg * a.c.k_page) * item +
-                             __umul24(min(p0 + r, hi - 1) & mask, D) * item;
+      for (int i = 0; i < kRuns; i++) {
+        // (kOne: a run past the end is the last one again, rows past it the last row)
+        const int start = min(p0 + kRun * i, (hi - 1) & -kRun), last = hi - 1 - start;
+        if (kOne) pg[i] = __builtin_amdgcn_readfirstlane(page_of(a, pid[i], bad));
+        {
+          const uint8_t* src;
+          uint32_t off;
+          if (kOne) {
+            src = kg + ((size_t)pg[i] * a.c.k_page + (uint32_t)((start & mask) * D)) * item;
+            off = __umul24(min(col, last), D) * item;
+          } else {
+            src = kg + (size_t)page_of(a, __shfl(pid[0], kQ * i + col, 64), bad) * a.c.k_page *
+                           item;
+            off = __umul24(min(p0 + kQ * i + col, hi - 1) & mask, D) * item;
+          }
 #pragma unroll
-        for (int s = 0; s < R::kSteps; s++) {
-          const int d = 32 * s + 8 * grp < D ? 32 * s + 8 * grp : 0;  // (products with zeros)
-          if (kType == kKvFp16)
-            kf[i][s] = load_global<half8>(src + 2 * d);
+          for (int s = 0; s < R::kSteps; s++) {
+            if (kType == kKvFp16)
+              kf[i][s] = load_global<half8>(src + (off + kcol[s] * 2));
+            else
+              kc[i][s] = load_global<uint2>(src + (off + kcol[s]));
+          }
+        }
+        uint8_t* const dst = vbuf + buf * T::kBytes + i * (T::kBytes / kRuns);
+        const uint8_t* vp =
+            vg + ((size_t)pg[i] * a.c.v_page + (uint32_t)((start & mask) * D)) * item;
+#pragma unroll
+        for (int j = 0; j < kVs; j++) {
+          uint32_t off = (__umul24(min(vrow[j], last), D) + vcol[j]) * item;
+          if (!kOne) {
+            const int r = kQ * i + vrow[j];
+            vp = vg + (size_t)page_of(a, __shfl(pid[0], r, 64), bad) * a.c.v_page * item;
+            off = (__umul24(min(p0 + r, hi - 1) & mask, D) + vcol[j]) * item;
+          }
+          if (kType == kKvInt8)
+            vc[i * kVs + j] = load_global<uint2>(vp + off);
+          else if (kOne)
+            dma16(vp, off, dst + j * 1024);
           else
-            kc[i][s] = load_global<uint2>(src + d);
+            dma16(vp + off, dst + j * 1024);
         }
       }
-#pragma unroll
-      for (int i = 0; i < T::kN; i++) {
-        const int r = (i * 64 + lane) / L::kCh;
-        const int ch = 8 * (((i * 64 + lane) % L::kCh) ^ L::swz(r));
-        const int pg = page_of(a, __shfl(pid, r, 64), bad);
-        const uint8_t* src = (const uint8_t*)a.c.v +
-                             (((size_t)g << a.c.page_shift) * D + (size_t)pg * a.c.v_page) * item +
-                             (__umul24(min(p0 + r, hi - 1) & mask, D) + (ch < D ? ch : 0)) * item;
-        if (kType == kKvFp16)
-          dma16(src, vbuf + buf * T::kBytes + i * 1024);
-        else
-          vc[i] = load_global<uint2>(src);
-      }
       if (kType == kKvInt8) {
-        const int pg = page_of(a, pid, bad);
+        int page = kOne ? pg[0] : page_of(a, pid[0], bad);
+        if (kOne) {
+#pragma unroll
+          for (int i = 1; i < kRuns; i++) page = lane % kKeys / kRun == i ? pg[i] : page;
+        }
         const int tok = (g << a.c.page_shift) + (min(p0 + lane % kKeys, hi - 1) & mask);
-        kss = load_global<float>(a.c.k_scale + (size_t)pg * a.c.ks_page + tok);
-        vss = load_global<float>(a.c.v_scale + (size_t)pg * a.c.vs_page + tok);
+        kss = load_global<float>(a.c.k_scale + (size_t)page * a.c.ks_page + tok);
+        vss = load_global<float>(a.c.v_scale + (size_t)page * a.c.vs_page + tok);
       }
     };
 
@@ -114,29 +156,39 @@ __global__ void __launch_bounds__(256, 2) attn_few_kernel(AttnArgs a) {
       issue(lo + wave * kKeys, 0);
       look_up(lo + wave * kKeys + step);
     }
+    R x;
+    x.init(r0 + col < rows ? a.q + (size_t)t * a.q_stride + (size_t)h * D : nullptr, D, a.scale);
     int buf = 0;
     for (int p0 = lo + wave * kKeys; p0 < hi; p0 += step, buf ^= T::kBufs - 1) {
-      half8 k[2][R::kSteps];
+      typename R::acc s[kRuns];
+      auto next = [&]() __attribute__((always_inline)) {
+        if (p0 + step < hi) {
+          issue(p0 + step, buf ^ (T::kBufs - 1));
+          look_up(p0 + 2 * step);
+        }
+      };
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      if (kType == kKvFp16) {
+        half8 k[kRuns][R::kSteps];
 #pragma unroll
-      for (int i = 0; i < 2; i++)
+        for (int i = 0; i < kRuns; i++)
 #pragma unroll
-        for (int s = 0; s < R::kSteps; s++)
-          k[i][s] = kType == kKvFp16 ? kf[i][s]
-                                     : __builtin_bit_cast(half8, codes_to_f16(kc[i][s]));
-      if (kType == kKvInt8) {
+          for (int st = 0; st < R::kSteps; st++) k[i][st] = kf[i][st];
+        next();
+        x.scores(s, [&](int i, int st) __attribute__((always_inline)) { return k[i][st]; });
+      } else {
+        // (the next tile's codes come into the registers of this one's: with a third of
+        // the registers less, three work-groups a CU and not two)
 #pragma unroll
         for (int i = 0; i < T::kN; i++)
           *reinterpret_cast<u32x4*>(vbuf + (i * 64 + lane) * 16) = codes_to_bf16(vc[i]);
         ks[lane % kKeys] = kss;
         vs[lane % kKeys] = vss;
+        x.scores(s, [&](int i, int st) __attribute__((always_inline)) {
+          return f16x8(codes_to_f16(kc[i][st]));
+        });
+        next();
       }
-      if (p0 + step < hi) {
-        issue(p0 + step, buf ^ (T::kBufs - 1));
-        look_up(p0 + 2 * step);
-      }
-      typename R::acc s[2];
-      x.scores(s, [&](int i, int st) __attribute__((always_inline)) { return k[i][st]; });
       if (p0 < all_lo || p0 + kKeys - 1 > all_hi)
         x.template maximum<true>(s, seen_lo - p0, seen_hi - p0, ks);
       else
@@ -202,14 +254,20 @@ __global__ void __launch_bounds__(256, 2) attn_few_kernel(AttnArgs a) {
   }
 }
 
-template <int kType, int DP>
-hipError_t run(const AttnArgs& a, hipStream_t s) {
+template <int kType, int DP, bool kOne>
+hipError_t launch(const AttnArgs& a, hipStream_t s) {
   const size_t grid = (size_t)a.b.batch * a.c.kv_heads * a.fs.splits;
   if (grid > 0xFFFFFF) return hipErrorInvalidValue;
-  const hipError_t e = set_lds_limit((const void*)attn_few_kernel<kType, DP>, 4 * Few<kType, DP>::kWave);
+  const hipError_t e = set_lds_limit((const void*)attn_few_kernel<kType, DP, kOne>, 4 * Few<kType, DP>::kWave);
   if (e != hipSuccess) return e;
-  attn_few_kernel<kType, DP><<<(unsigned)grid, 256, 4 * Few<kType, DP>::kWave, s>>>(a);
+  attn_few_kernel<kType, DP, kOne><<<(unsigned)grid, 256, 4 * Few<kType, DP>::kWave, s>>>(a);
   return hipGetLastError();
+}
+
+template <int kType, int DP>
+hipError_t run(const AttnArgs& a, hipStream_t s) {
+  return a.c.page_shift >= kRunShift ? launch<kType, DP, true>(a, s)
+                                     : launch<kType, DP, false>(a, s);
 }
 
 }  // namespace

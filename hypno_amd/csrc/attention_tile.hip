@@ -64,9 +64,6 @@ __global__ void __launch_bounds__(256, 2) attn_tile_kernel(AttnArgs a) {
   const int any_hi = some ? min(sq.kv - sq.n + last / G, hi - 1) : -1;
   const int all_lo = some ? first_seen(a, sq, last / G) : 0;
   const int all_hi = some ? min(sq.kv - sq.n + w0 / G, hi - 1) : -1;
-  R x;
-  x.init(live ? a.q + (size_t)t * a.q_stride + (size_t)h * D : nullptr, D, a.scale);
-
   bool bad = false;
   uint8_t* const kbuf = smem;
   uint8_t* const vbuf = smem + 2 * T::kBytes;
@@ -163,6 +160,8 @@ __global__ void __launch_bounds__(256, 2) attn_tile_kernel(AttnArgs a) {
     if (kType == kKvInt8) store(0);
     look_up(lo + BK);
   }
+  R x;
+  x.init(live ? a.q + (size_t)t * a.q_stride + (size_t)h * D : nullptr, D, a.scale);
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
   // Tiles that all of the wave's rows see whole need no mask; each wave goes through
   // its own runs of the two kinds, tile by tile with the others.
