@@ -1,5 +1,7 @@
 // Attention of each sequence's new tokens over its pages of the cache: which kernels
 // a call takes, and the sum of what a row's ranges of positions gave.
+#include <cmath>
+
 #include "attention.hpp"
 
 namespace hypno {
@@ -119,16 +121,29 @@ AttnPlan attn_plan(const KvCache& c, const KvBatch& b, int heads, int window, in
   p.few = only_few ? 0x7FFFFFFF : only_tile ? 0 : 16;
   const int64_t room = (int64_t)b.width << c.page_shift;
   const int64_t kv = std::max<int64_t>(1, max_kv ? std::min(max_kv, room) : room);
-  // Ranges of 128 positions at least, so that one sequence has a work-group for each one
-  // that the chip holds at a time, and several up to eight, for lengths that differ.
+  // Up to 1024 positions (2048 where sequences and heads alone fill the chip) a
+  // work-group takes them all: the kernel that joins ranges costs 4 us and its launch.
+  // Beyond, one sequence gets a work-group for each one that the chip holds at a time.
+  // Lengths of several may differ, so that the last range to end counts: against the
+  // start of a range (about 130 positions' time) the best length grows with the root of
+  // all work.  (us at 32/8 heads of 128, ranges of 128 / 256 / 512 / none: one sequence
+  // of 3000: 11.1 / 12.0 / 14.1 / -; 8 of up to 6000: 44 / 35 / 32 / -; 64 of up to 2000:
+  // - / 67 / 58 / 53.)
   p.fs = {1, 0x7FFFFFFF};
+  p.few_waves = 4;
   if (p.few) {
     const int64_t seen = window ? std::min<int64_t>(kv, (int64_t)window + 16) : kv;
-    const int64_t pairs = (int64_t)b.batch * c.kv_heads;
-    const int64_t want = std::max<int64_t>(1, (b.batch > 1 ? 16 : 2) * num_cus / pairs);
-    const int64_t chunk = std::max<int64_t>(128, (up(seen, want) + 127) / 128 * 128);
-    p.fs.splits = up(seen, chunk);
-    p.fs.chunk = (int)std::min<int64_t>(chunk, 0x7FFFFFFF);
+    const int64_t pairs = (int64_t)b.batch * c.kv_heads, slots = 2 * num_cus;
+    if (seen > (pairs >= slots ? 2048 : 1024)) {
+      const double each = (double)pairs * seen / slots;
+      const double best = b.batch > 1 ? std::sqrt(128.0 * each) : each;
+      const int64_t least = std::min<int64_t>(std::max<int64_t>(8 * pairs, 128), 512);
+      const int64_t chunk = std::max(least, ((int64_t)best + 127) / 128 * 128);
+      p.fs.splits = up(seen, chunk);
+      p.fs.chunk = (int)std::min<int64_t>(chunk, 0x7FFFFFFF);
+    } else if (pairs <= num_cus && seen > 128) {
+      p.few_waves = 8;
+    }
   }
   // Ranges while the work-groups do not fill the chip.
   p.ts = {1, 0x7FFFFFFF};
@@ -151,7 +166,7 @@ hipError_t launch_paged_attention(const AttnPlan& p, float* out, const float* q,
                                   int heads, const KvCache& c, const KvBatch& b, float scale,
                                   int window, void* ws, hipStream_t s) {
   AttnArgs a = {c, b, out, q, q_stride, heads, heads / c.kv_heads, window, scale,
-                p.few, p.tile_rows, p.fs, p.ts, p.cus, std::max(p.fs.splits, p.ts.splits),
+                p.few, p.few_waves, p.tile_rows, p.fs, p.ts, p.cus, std::max(p.fs.splits, p.ts.splits),
                 nullptr, nullptr};
   if (!ws) a.fs = a.ts = {1, 0x7FFFFFFF};
   a.part_ml = reinterpret_cast<float2*>(ws);

@@ -37,6 +37,7 @@ struct AttnArgs {
   int heads, group, window;
   float scale;
   int few;                // sequences of at most so many rows are attn_few_kernel's
+  int few_waves;          // of its work-groups (4 or 8)
   int tile_rows;          // rows of a work-group of the other
   AttnSplit fs, ts;       // of attn_few_kernel and attn_tile_kernel
   int cus;

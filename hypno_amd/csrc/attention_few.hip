@@ -23,9 +23,11 @@ struct Few {
   static constexpr int kWave = kStage > kOut ? kStage : kOut;
 };
 
-// kOne: pages have kRun positions or more.
-template <int kType, int DP, bool kOne>
-__global__ void __launch_bounds__(256, (Few<kType, DP>::kGroups)) attn_few_kernel(AttnArgs a) {
+// kOne: pages have kRun positions or more.  kWaves: 4, or 8 where a work-group takes all
+// positions and these are few: half the tiles one after the other.
+template <int kType, int DP, bool kOne, int kWaves>
+__global__ void __launch_bounds__(64 * kWaves, (kWaves == 8 ? 1 : Few<kType, DP>::kGroups))
+    attn_few_kernel(AttnArgs a) {
   typedef Few<kType, DP> T;
   constexpr int kKeys = T::kKeys, kRuns = T::kRuns, kVs = T::kN / kRuns;
   typedef KvTile<DP> L;
@@ -150,7 +152,7 @@ __global__ void __launch_bounds__(256, (Few<kType, DP>::kGroups)) attn_few_kerne
       }
     };
 
-    const int step = 4 * kKeys;
+    const int step = kWaves * kKeys;
     if (lo + wave * kKeys < hi) {
       look_up(lo + wave * kKeys);
       issue(lo + wave * kKeys, 0);
@@ -197,8 +199,7 @@ __global__ void __launch_bounds__(256, (Few<kType, DP>::kGroups)) attn_few_kerne
     }
     x.finish(__any(bad));
 
-    // The four waves' parts, then their sum: thread (row, piece) takes every sixteenth
-    // group of four elements.
+    // The waves' parts, then their sum: thread (row, piece) takes four elements.
     float* const part = reinterpret_cast<float*>(vbuf);
     float2* const ml = reinterpret_cast<float2*>(part + kQ * (DP + 4));
 #pragma unroll
@@ -208,22 +209,21 @@ __global__ void __launch_bounds__(256, (Few<kType, DP>::kGroups)) attn_few_kerne
     if (lane < kQ) ml[col] = make_float2(x.m, x.l);
     if (tid == 0) again = 0;
     __syncthreads();
-    const int or_ = tid / 16, piece = tid % 16;
-    float w[4], m = -__builtin_inff(), l = 0.0f;
-    const float* pw[4];
+    const int or_ = tid / (4 * kWaves), piece = tid % (4 * kWaves);
+    float w[kWaves], m = -__builtin_inff(), l = 0.0f;
+    auto row_of = [&](int i) { return reinterpret_cast<const float*>(smem + i * T::kWave) + or_ * (DP + 4); };
+    auto ml_of = [&](int i) {
+      return reinterpret_cast<const float2*>(smem + i * T::kWave + kQ * (DP + 4) * 4)[or_];
+    };
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      pw[i] = reinterpret_cast<const float*>(smem + i * T::kWave);
-      const float2 v = reinterpret_cast<const float2*>(pw[i] + kQ * (DP + 4))[or_];
-      pw[i] += or_ * (DP + 4);
-      w[i] = v.x;
-      m = fmaxf(m, v.x);
+    for (int i = 0; i < kWaves; i++) {
+      w[i] = ml_of(i).x;
+      m = fmaxf(m, w[i]);
     }
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
+    for (int i = 0; i < kWaves; i++) {
       w[i] = w[i] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(w[i] - m);
-      const float2 v = reinterpret_cast<const float2*>(pw[i] - or_ * (DP + 4) + kQ * (DP + 4))[or_];
-      l += v.y * w[i];
+      l += ml_of(i).y * w[i];
     }
     const bool live = r0 + or_ < rows;
     const int rr = min(r0 + or_, rows - 1);
@@ -234,10 +234,11 @@ __global__ void __launch_bounds__(256, (Few<kType, DP>::kGroups)) attn_few_kerne
     float* const dst = parts ? a.part_o + prow * D : a.out + orow * D;
     float z = l * 0.0f;
     if (live) {
-      for (int d = 4 * piece; d < D; d += 64) {
+      for (int d = 4 * piece; d < D; d += 16 * kWaves) {
         f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int i = 0; i < 4; i++) v += *reinterpret_cast<const f32x4*>(pw[i] + d) * w[i];
+        for (int i = 0; i < kWaves; i++)
+          v += *reinterpret_cast<const f32x4*>(row_of(i) + d) * w[i];
         v *= inv;
 #pragma unroll
         for (int j = 0; j < 4; j++) z += v[j] * 0.0f;
@@ -249,25 +250,31 @@ __global__ void __launch_bounds__(256, (Few<kType, DP>::kGroups)) attn_few_kerne
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (!parts)
-      attn_rows(a, sq, g, r0, again & (0x1111u << wave));  // (every fourth row a wave)
+      attn_rows(a, sq, g, r0, again & ((kWaves == 8 ? 0x0101u : 0x1111u) << wave));
     __syncthreads();
   }
 }
 
-template <int kType, int DP, bool kOne>
+template <int kType, int DP, bool kOne, int kWaves>
 hipError_t launch(const AttnArgs& a, hipStream_t s) {
+  constexpr int kLds = kWaves * Few<kType, DP>::kWave;
   const size_t grid = (size_t)a.b.batch * a.c.kv_heads * a.fs.splits;
   if (grid > 0xFFFFFF) return hipErrorInvalidValue;
-  const hipError_t e = set_lds_limit((const void*)attn_few_kernel<kType, DP, kOne>, 4 * Few<kType, DP>::kWave);
+  const void* kernel = (const void*)attn_few_kernel<kType, DP, kOne, kWaves>;
+  const hipError_t e = set_lds_limit(kernel, kLds);
   if (e != hipSuccess) return e;
-  attn_few_kernel<kType, DP, kOne><<<(unsigned)grid, 256, 4 * Few<kType, DP>::kWave, s>>>(a);
+  attn_few_kernel<kType, DP, kOne, kWaves><<<(unsigned)grid, 64 * kWaves, kLds, s>>>(a);
   return hipGetLastError();
 }
 
 template <int kType, int DP>
 hipError_t run(const AttnArgs& a, hipStream_t s) {
-  return a.c.page_shift >= kRunShift ? launch<kType, DP, true>(a, s)
-                                     : launch<kType, DP, false>(a, s);
+  const bool one = a.c.page_shift >= kRunShift;
+  if constexpr (DP <= 128) {
+    if (a.few_waves == 8)
+      return one ? launch<kType, DP, true, 8>(a, s) : launch<kType, DP, false, 8>(a, s);
+  }
+  return one ? launch<kType, DP, true, 4>(a, s) : launch<kType, DP, false, 4>(a, s);
 }
 
 }  // namespace

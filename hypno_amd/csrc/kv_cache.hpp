@@ -74,6 +74,7 @@ struct AttnSplit {
 // How a call's rows and positions are split, and the workspace that takes.
 struct AttnPlan {
   int few;        // sequences of at most so many rows go to attn_few_kernel
+  int few_waves;  // of its work-groups
   int tile_rows;  // rows of a work-group of attn_tile_kernel
   int cus;
   AttnSplit fs, ts;
