@@ -114,10 +114,11 @@ AttnPlan attn_plan(const KvCache& c, const KvBatch& b, int heads, int window, in
   const int G = heads / c.kv_heads;
   const int64_t rows = (int64_t)b.tokens * G;
   p.tile_rows = c.head_dim <= 128 ? 128 : 64;
-  // Single tokens, or one sequence of few rows: attn_few_kernel alone.  One sequence
-  // of many rows, or groups of more than 16: attn_tile_kernel alone.
+  // Single tokens, or one sequence of few rows: attn_few_kernel alone.  Few sequences, or
+  // groups of more than 16: attn_tile_kernel alone (single tokens among them then run
+  // beside the others, which costs less than a second kernel after them).
   const bool only_few = b.tokens <= b.batch || (b.batch == 1 && rows <= 16);
-  const bool only_tile = !only_few && (b.batch == 1 || G > 16);
+  const bool only_tile = !only_few && (b.batch <= 8 || G > 16);
   p.few = only_few ? 0x7FFFFFFF : only_tile ? 0 : 16;
   const int64_t room = (int64_t)b.width << c.page_shift;
   const int64_t kv = std::max<int64_t>(1, max_kv ? std::min(max_kv, room) : room);
@@ -145,16 +146,31 @@ AttnPlan attn_plan(const KvCache& c, const KvBatch& b, int heads, int window, in
       p.few_waves = 8;
     }
   }
-  // Ranges while the work-groups do not fill the chip.
+  // Ranges where they are worth writing and joining their parts: by the time, in us, of a
+  // work-group's tiles of 64 positions (1.8 with one work-group a CU and head_dim 128, 1.6
+  // times that with two) and of the parts' way through memory.
   p.ts = {1, 0x7FFFFFFF};
   if (p.few != 0x7FFFFFFF) {
     const int64_t seen =
         window ? std::min<int64_t>(kv, (int64_t)window + up(p.tile_rows, G)) : kv;
-    const int64_t groups = std::max<int64_t>(1, rows / p.tile_rows) * c.kv_heads;
-    const int64_t want = std::max<int64_t>(1, 2 * num_cus / groups);
-    const int64_t chunk = std::max<int64_t>(256, (up(seen, want) + 63) / 64 * 64);
-    p.ts.splits = up(seen, chunk);
-    p.ts.chunk = (int)std::min<int64_t>(chunk, 0x7FFFFFFF);
+    const double groups = std::max(1.0, (double)rows / p.tile_rows) * c.kv_heads;
+    const double part_us = (double)b.tokens * heads * c.head_dim * 8 / 3.5e6;
+    const int dim = c.head_dim <= 64 ? 64 : c.head_dim <= 96 ? 96 : 128;
+    const double tile_us = ((c.head_dim > 128 ? 2 : 1) * 0.8 + dim / 128.0) *
+                           (c.dtype == kKvInt8 ? 1.2 : 1.0);
+    double best = 1e30;
+    for (int n = 1; n <= 64; n++) {
+      const int64_t chunk = (up(seen, n) + 63) / 64 * 64;
+      const int splits = up(seen, chunk);
+      const double each = groups * splits <= num_cus ? tile_us : 1.6 * tile_us;
+      const double us = std::ceil(groups * splits / (2 * num_cus)) * (4.0 + chunk / 64 * each) +
+                        (splits > 1 ? 5.0 + part_us * splits : 0.0);
+      if (us < best * 0.98) {
+        best = us;
+        p.ts.splits = splits;
+        p.ts.chunk = (int)std::min<int64_t>(chunk, 0x7FFFFFFF);
+      }
+    }
   }
   const int most = std::max(p.fs.splits, p.ts.splits);
   p.ml_bytes = most > 1 ? ((size_t)most * b.tokens * heads * 8 + 255) / 256 * 256 : 0;
