@@ -24,29 +24,39 @@ HypnoHipError.
 """
 from __future__ import annotations
 
+import ctypes
 import math
+import os
 import struct
 
-from ._lib import check, load
+from ._lib import HERE, check, load
 
 __all__ = ["append_kv", "paged_attention"]
 
 _STYLES = {"halves": 0, "pairs": 1}  # HYPNO_HIP_ROPE_*
 
-# The structs of include/hypno_hip.h (as _lib.KvCache and _lib.KvBatch, packed at once:
-# a call of one token takes the GPU 5 us, and its checks should not take longer).
+# The structs of include/hypno_hip.h (_lib.KvCache and _lib.KvBatch), packed at once.
 _CACHE = struct.Struct("=I4x12Q")
 _BATCH = struct.Struct("=6Q")
 
 torch = None
+_args = None  # csrc/attention_args.cpp: the same checks and packing, where all is right
 
 
 def _torch():
     """(imported by the first call: the rest of the package works without it)"""
-    global torch
-    if torch is None:
-        import torch
-    return torch
+    global torch, _args
+    import torch
+    lib = load()
+    if not os.path.exists(os.path.join(HERE, "_attention_args.so")):
+        raise ImportError("hypno_amd/_attention_args.so is missing: build it with "
+                          "`python -m hypno_amd.build`")
+    from . import _attention_args
+    _attention_args.bind(
+        *(ctypes.cast(f, ctypes.c_void_p).value
+          for f in (lib.hypno_hip_append_kv_dev, lib.hypno_hip_paged_attention_dev)),
+        torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream)
+    _args = _attention_args
 
 
 def _rows(t, what: str):
@@ -150,6 +160,12 @@ def _call(fn, where: str, dev: int, *args) -> None:
         check(status, where)
 
 
+def _done(result, where: str):
+    if type(result) is int:
+        check(result, where)
+    return result
+
+
 def append_kv(q, k, v, k_cache, v_cache, page_table, kv_lens, cu_q, inv_freq=None,
               style: str = "halves", k_scale=None, v_scale=None, out=None):
     """Rotates the new tokens' q and k to their positions, writes k and v to their
@@ -158,9 +174,14 @@ def append_kv(q, k, v, k_cache, v_cache, page_table, kv_lens, cu_q, inv_freq=Non
     None: no rotation.  style "halves": pair j is elements j and j + rot_dim / 2;
     "pairs": 2j and 2j + 1.  q may be None (k and v only).  int8 caches: see
     include/hypno_hip.h for the codes."""
-    _torch()
+    if _args is None:
+        _torch()
     if style not in _STYLES:
         raise ValueError(f"style must be 'halves' or 'pairs', got {style!r}")
+    done = _args.append_kv(q, k, v, k_cache, v_cache, page_table, kv_lens, cu_q, inv_freq,
+                           _STYLES[style], k_scale, v_scale, out)
+    if done is not NotImplemented:
+        return _done(done, "append_kv")
     tokens, kv_heads, dim, k_stride, dev = _rows(k, "k")
     n, vh, vd, v_stride, vdev = _rows(v, "v")
     if n != tokens or vh != kv_heads or vd != dim or vdev != dev:
@@ -207,7 +228,12 @@ def paged_attention(q, k_cache, v_cache, page_table, kv_lens, cu_q, scale=None, 
     scores, by default head_dim ** -0.5.  max_kv_len: an upper bound of kv_lens, if the
     host knows one (default: what page_table has room for); it decides how many
     work-groups share a sequence."""
-    _torch()
+    if _args is None:
+        _torch()
+    done = _args.paged_attention(q, k_cache, v_cache, page_table, kv_lens, cu_q, scale, window,
+                                 k_scale, v_scale, max_kv_len, out)
+    if done is not NotImplemented:
+        return _done(done, "paged_attention")
     tokens, heads, dim, q_stride, dev = _rows(q, "q")
     cache, kv_heads, cd = _cache(k_cache, v_cache, k_scale, v_scale, dev)
     if cd != dim or not kv_heads or heads % kv_heads:

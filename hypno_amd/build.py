@@ -1,4 +1,5 @@
-"""Builds libhypno_hip.so (gfx950) in-tree with hipcc.
+"""Builds libhypno_hip.so (gfx950) in-tree with hipcc, and _attention_args.so (host
+code over torch's headers) with g++.
 
     python -m hypno_amd.build        # or hypno_amd.build.build()
 
@@ -13,6 +14,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -78,11 +80,33 @@ def _compile(src: str) -> str:
     return obj
 
 
+def _build_args() -> None:
+    """Host code that reads torch's tensors (a Python module beside the library)."""
+    try:
+        import torch
+        from torch.utils.cpp_extension import include_paths
+    except ImportError:
+        return  # (its callers need torch too)
+    out = os.path.join(HERE, "_attention_args.so")
+    libs = os.path.join(os.path.dirname(torch.__file__), "lib")
+    cmd = ["g++", "-O2", "-fPIC", "-shared", "-std=c++17", "-w",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}"]
+    cmd += [f"-I{p}" for p in [*include_paths(), sysconfig.get_paths()["include"]]]
+    cmd += [os.path.join(CSRC, "attention_args.cpp"), "-o", out + ".tmp", f"-L{libs}", "-lc10",
+            "-ltorch_cpu", "-ltorch_python"]
+    p = subprocess.run(cmd, capture_output=True, text=True)
+    if p.returncode != 0:
+        raise RuntimeError(f"g++ failed for attention_args.cpp:\n{p.stderr}")
+    os.replace(out + ".tmp", out)
+
+
 def build(verbose: bool = False) -> str:
     """Compile every source for gfx950 and link LIB_PATH.  Always rebuilds."""
     os.makedirs(OBJ_DIR, exist_ok=True)
     with concurrent.futures.ThreadPoolExecutor(max_workers=min(8, len(SOURCES))) as ex:
+        args = ex.submit(_build_args)
         objs = list(ex.map(_compile, SOURCES))
+        args.result()
     tmp = LIB_PATH + ".tmp"
     cmd = [hipcc(), f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", tmp] + objs
     p = subprocess.run(cmd, capture_output=True, text=True)
