@@ -49,6 +49,38 @@ template <int kType>
 __global__ void __launch_bounds__(kAppendThreads) append_kv_kernel(AppendArgs a) {
   __shared__ double cs[kMaxHeadDim / 2], sn[kMaxHeadDim / 2];
   const int t = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+  const int D = a.c.head_dim, KV = a.c.kv_heads, half = a.rot / 2;
+  const int per_wave = 64 >> a.lane_shift;
+  const int unit = lane & ((1 << a.lane_shift) - 1), e0 = 8 * unit;
+  const int waves = kAppendThreads / 64 * gridDim.y, all = a.heads + 2 * KV;
+  int r0 = (blockIdx.y * (kAppendThreads / 64) + tid / 64) * per_wave;
+  float x[8], w[8], xn[8], wn[8];  // a lane's elements, the other ones of their pairs
+  auto load = [&](float (&x)[8], float (&w)[8], int r0) __attribute__((always_inline)) {
+    const int row = r0 + (lane >> a.lane_shift);
+#pragma unroll
+    for (int i = 0; i < 8; i++) x[i] = w[i] = 0.0f;
+    if (row >= all || e0 >= D) return;
+    const bool is_q = row < a.heads, is_k = !is_q && row < a.heads + KV;
+    const float* src = is_q   ? a.q + (size_t)t * a.q_stride + (size_t)row * D
+                       : is_k ? a.k + (size_t)t * a.k_stride + (size_t)(row - a.heads) * D
+                              : a.v + (size_t)t * a.v_stride + (size_t)(row - a.heads - KV) * D;
+    load8(x, src + e0, a.vec);
+    if ((is_q || is_k) && !a.pairs) {
+      // Read before anything is written, as a row belongs to one wave (q_out may be q).
+      if (half % 8 == 0) {
+        if (e0 < a.rot) load8(w, src + (e0 < half ? e0 + half : e0 - half), a.vec);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          const int e = e0 + i;
+          if (e < a.rot) w[i] = load_global<float>(src + (e < half ? e + half : e - half));
+        }
+      }
+    }
+  };
+  // The first rows and the frequencies come in while the token's place is looked up.
+  load(xn, wn, r0);
+  const float freq = tid < half ? load_global<float>(a.inv_freq + tid) : 0.0f;
   const int b = find_seq(a.b, t, 0, 0);
   if (b < 0 || b >= a.b.batch) return;  // a token of no sequence
   const int first = cu_at(a.b, b), n = cu_at(a.b, b + 1) - first;
@@ -57,41 +89,18 @@ __global__ void __launch_bounds__(kAppendThreads) append_kv_kernel(AppendArgs a)
   int page = -1;
   if (pos >= 0 && at < a.b.width)
     page = load_global<int>(a.b.page_table + (size_t)b * a.b.width + at);
-  const bool stored = page >= 0 && page < a.c.pages;
-  for (int j = tid; j < a.rot / 2; j += kAppendThreads) {
-    double s, c;
-    sincos((double)pos * (double)load_global<float>(a.inv_freq + j), &s, &c);
-    cs[j] = c;
-    sn[j] = s;
-  }
+  if (tid < half) sincos((double)pos * (double)freq, &sn[tid], &cs[tid]);
   __syncthreads();
-  const int D = a.c.head_dim, KV = a.c.kv_heads, half = a.rot / 2;
-  const int per_wave = 64 >> a.lane_shift;
-  const int unit = lane & ((1 << a.lane_shift) - 1), e0 = 8 * unit;
-  const int waves = kAppendThreads / 64 * gridDim.y;
+  const bool stored = page >= 0 && page < a.c.pages;
   const int slot = (int)(pos & ((1 << a.c.page_shift) - 1));
-  for (int r0 = (blockIdx.y * (kAppendThreads / 64) + tid / 64) * per_wave;
-       r0 < a.heads + 2 * KV; r0 += waves * per_wave) {
+  for (; r0 < all; r0 += waves * per_wave) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) x[i] = xn[i], w[i] = wn[i];
+    load(xn, wn, r0 + waves * per_wave);
     const int row = r0 + (lane >> a.lane_shift);
     const bool is_q = row < a.heads, is_k = !is_q && row < a.heads + KV;
     const int h = is_q ? row : is_k ? row - a.heads : row - a.heads - KV;
-    const bool live = row < a.heads + 2 * KV && e0 < D && (is_q || stored);
-    float x[8] = {}, w[8] = {};
-    if (live) {
-      const float* src = (is_q ? a.q + (size_t)t * a.q_stride
-                               : is_k ? a.k + (size_t)t * a.k_stride
-                                      : a.v + (size_t)t * a.v_stride) + (size_t)h * D;
-      load8(x, src + e0, a.vec);
-      if ((is_q || is_k) && !a.pairs) {
-        // The other element of each pair; read before anything is written, as a
-        // row belongs to one wave (q_out may be q).
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-          const int e = e0 + i;
-          if (e < a.rot) w[i] = load_global<float>(src + (e < half ? e + half : e - half));
-        }
-      }
-    }
+    const bool live = row < all && e0 < D && (is_q || stored);
     if (live && (is_q || is_k)) {
       if (a.pairs) {
 #pragma unroll
