@@ -153,23 +153,34 @@ __global__ void __launch_bounds__(256, 2) attn_tile_kernel(AttnArgs a) {
     if (lane < 2 * kMine) scales[(buf * 2 + !sk) * BK + srow] = sr;
   };
 
+  // fp16: tile i + 1 is copied into LDS while tile i is worked on.  8-bit: tile i + 1 is
+  // stored there (its codes came in during tile i - 1) and the loads of i + 2 begin.
+  constexpr int kAhead = kType == kKvFp16 ? 1 : 2;
   const int tiles = (hi - lo + BK - 1) / BK;
   if (tiles > 0) {
     look_up(lo);
     issue(lo, 0);
-    if (kType == kKvInt8) store(0);
-    look_up(lo + BK);
+    if (kType == kKvInt8) {
+      store(0);
+      look_up(lo + BK);
+      if (tiles > 1) issue(lo + BK, 1);
+    }
+    look_up(lo + kAhead * BK);
   }
   R x;
   x.init(live ? a.q + (size_t)t * a.q_stride + (size_t)h * D : nullptr, D, a.scale);
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  if (kType == kKvFp16)
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  else
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
   // Tiles that all of the wave's rows see whole need no mask; each wave goes through
   // its own runs of the two kinds, tile by tile with the others.
   auto step = [&](auto masked, int i) __attribute__((always_inline)) {
     const int p0 = lo + i * BK, buf = i & 1;
-    if (i + 1 < tiles) {
-      issue(p0 + BK, buf ^ 1);
-      look_up(p0 + 2 * BK);
+    if (kType == kKvInt8 && i + 1 < tiles) store(buf ^ 1);
+    if (i + kAhead < tiles) {
+      issue(p0 + kAhead * BK, buf ^ 1);
+      look_up(p0 + (kAhead + 1) * BK);
     }
     if (!masked || (p0 <= any_hi && p0 + BK > any_lo)) {
       const uint8_t* kt = kbuf + buf * T::kBytes;
@@ -182,8 +193,10 @@ __global__ void __launch_bounds__(256, 2) attn_tile_kernel(AttnArgs a) {
       x.template maximum<masked>(s, seen_lo - p0, seen_hi - p0, ks);
       x.values(s, vbuf + buf * T::kBytes, ks + BK);
     }
-    if (kType == kKvInt8 && i + 1 < tiles) store(buf ^ 1);
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (kType == kKvFp16)
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    else
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
   };
   const int full0 = some ? min(max(all_lo - lo + BK - 1, 0) / BK, tiles) : tiles;
   const int full1 = some ? max(full0, min((all_hi + 1 - lo) / BK, tiles)) : tiles;
