@@ -411,7 +411,7 @@ struct Rows {
     const int row0 = 4 * grp + l16 / 4;
     const int col = (NQ == 32 ? (lane >> 4 & 1) * 2 : 0) + (l16 & 3) / 2;
     const float off = kTop - (m == -__builtin_inff() ? 0.0f : m);
-    float neg = -1.0f;
+    float neg = -1.0f, sum = 0.0f;  // (the tile's sum apart: fewer additions to the long one)
     asm("" : "+s"(neg));
     u32x4 w[2][3];  // the weights' parts of this step and the next, two a register
     auto pair = [&](int p, int i) __attribute__((always_inline)) {
@@ -420,7 +420,7 @@ struct Rows {
 #pragma unroll
       for (int j = 0; j < 2; j++)
         x[j] = __builtin_amdgcn_exp2f(fmaf(s[u / kPer][u % kPer * 4 + r + j], c, off));
-      l += x[0] + x[1];
+      sum += x[0] + x[1];
       uint32_t a, b, d = 0;
       if (kType == kKvFp16) {
         split_f16(x[0], x[1], neg, a, b);
@@ -480,6 +480,7 @@ struct Rows {
           if (p + 1 < kPv && i * kGroups / 4 == g) pair(p + 1, i);
         __builtin_amdgcn_sched_barrier(0);
       }
+    l += sum;
   }
 
   // Ends the pass: this lane's row sum, NaN where the tiles held pages that are none.
