@@ -169,14 +169,21 @@ struct KvTile {
 
 // Lane i's 16 bytes at base + off to lds + 16 i, asynchronously; counted by vmcnt, which
 // the caller waits for.  (Not the builtin: the compiler then has every transposing read
-// of LDS wait for all such copies, the next tile's too.)
+// of LDS wait for all such copies, the next tile's too.)  kNt: read once, not kept.
+template <bool kNt = false>
 __device__ __forceinline__ void dma16(const void* base, uint32_t off, uint8_t* lds) {
 #if defined(__HIP_DEVICE_COMPILE__)
   const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)lds;
-  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-               :
-               : "{m0}"(at), "v"(off), "s"(base)
-               : "memory");
+  if (kNt)
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt"
+                 :
+                 : "{m0}"(at), "v"(off), "s"(base)
+                 : "memory");
+  else
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                 :
+                 : "{m0}"(at), "v"(off), "s"(base)
+                 : "memory");
 #endif
 }
 __device__ __forceinline__ void dma16(const void* src, uint8_t* lds) {
