@@ -1,6 +1,20 @@
 // Attention for sequences with few rows (single tokens, drafts): a work-group takes
-// one kv head of a sequence and a range of its positions; its four waves run through
+// one kv head of a sequence and a range of its positions; its waves run through
 // tiles of keys on their own, 16 rows at a time, and add up at the end.
+//
+// Bound: HBM.  One token over 131072 positions (32/8 heads of 128, 537 MB): 77 us, 7.0
+// TB/s; 64 sequences of up to 8192 (1.24 GB) 208 us, 5.9; with 8-bit values (0.64 GB) 163
+// us, 3.9: there it is the way through the wave (codes to fp16 and bf16, 310 vector
+// operations a tile, 40% of the cycles) at two waves a SIMD, which is what the registers
+// allow (three with 42 of them spilt: 357 us; tiles of 64 keys, 15 spilt: 206).
+//  * K goes from memory into the MFMA operands' registers, V into LDS, from where it is
+//    read transposed; a wave has its own LDS and meets the others only at the end.
+//  * Nothing but the next tile is in flight: 16 KB a wave, 128 KB a CU, several times
+//    what the memory's latency takes at this rate.
+//  * A context of up to 1024 positions is one work-group of eight waves a kv head: 8.0 us
+//    for one token over 700 (32/4 heads of 64), most of it latency: the sequence's
+//    place, its pages, three tiles one after the other, the waves' sum.
+
 #include "attention.hpp"
 
 namespace hypno {

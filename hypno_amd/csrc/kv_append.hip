@@ -11,6 +11,13 @@
 //   s = max|x| / 127 over the head's row, code = round_half_away(x / s)
 // with both quotients in fp32 (s = 0 and codes 0 where that underflows; s = NaN
 // and codes 0 for a row that holds an infinity or NaN).
+//
+// Bound: HBM for prompts (2048 tokens, 32/8 heads of 128, 92 MB: 20.6 us, 4.5 TB/s, a
+// large copy's 4.9), latency for few tokens (one: 4.4 us, of which an empty kernel is
+// about two): the batch's arrays and the page are two dependent reads, and the sines in 64
+// bits some hundred operations of one wave.  One work-group a token, so that these are
+// computed once for all its heads (a work-group for each 16 of its rows: the prompt takes
+// 27 us); the rows are split over several only while the chip is not full.
 #include "kv_cache.hpp"
 
 namespace hypno {

@@ -474,11 +474,13 @@ int hypno_hip_append_kv_dev(const hypno_hip_kv_cache* cache, const hypno_hip_kv_
 /* out[t][h] = sum_p w_p v_p / sum_p w_p, w_p = exp(scale * q[t][h] . k_p), over the
  * positions p <= the token's own (and, with window > 0, > its own - window) of kv head
  * h / (heads / kv_heads).  Zeros where that leaves none, or no w_p but 0.  The cache's
- * values are used exactly, sums and softmax statistics are fp32, and q and w are held
- * to at least 22 bits: out is as near as an fp32 computation's.  out [tokens][heads]
- * [head_dim], all of it fp32; it may not share memory with an input.  max_kv_len: an
- * upper bound of kv_lens that the host knows (0: table_width * page_size); it sets how
- * many work-groups share a sequence, never the result's range. */
+ * values are used exactly; sums and softmax statistics are fp32; q is held to 22 bits of
+ * its row's largest element and more, w to 22 bits down to 2^-36 of the row's largest
+ * (FP16) or to all 24 (INT8).  out [tokens][heads][head_dim], fp32; it may not share
+ * memory with an input.  max_kv_len: an upper bound of kv_lens that the host knows (0:
+ * table_width * page_size); it sets how many work-groups share a sequence, never the
+ * result's range.  Calls whose positions are split use the stream's workspace; under
+ * capture, without one that is large enough, they are not split. */
 int hypno_hip_paged_attention_dev(float* out, const float* q, size_t q_stride, size_t heads,
                                   const hypno_hip_kv_cache* cache,
                                   const hypno_hip_kv_batch* batch, float scale, size_t window,
