@@ -311,14 +311,22 @@ struct Rows {
   float m, l;   // reference (log2 units); this lane's part of the sum
   float c;      // scores to log2 units
 
-  // `src`: the row's q, or NULL.  Rows are scaled by a power of two to at most 2^15.
-  __device__ __forceinline__ void init(const float* src, int D, float scale) {
+  // First of the eight elements that a lane holds for step s of a score's sum.  kPairs:
+  // two steps' elements side by side, so that 8-bit keys are read sixteen at a time.
+  template <bool kPairs>
+  __device__ static __forceinline__ int element(int s) {
     const int grp = (threadIdx.x & 63) / NQ;
+    return kPairs && s < kSteps / 2 * 2 ? 8 * (NG * (s & ~1) + 2 * grp + (s & 1))
+                                        : 8 * (NG * s + grp);
+  }
+
+  // `src`: the row's q, or NULL.  Rows are scaled by a power of two to at most 2^15.
+  __device__ __forceinline__ void init(const float* src, int D, float scale, bool pairs = false) {
     float x[kSteps][8];
     uint32_t mb = 0;
 #pragma unroll
     for (int s = 0; s < kSteps; s++) {
-      const int d = 8 * (NG * s + grp);
+      const int d = pairs ? element<true>(s) : element<false>(s);
 #pragma unroll
       for (int j = 0; j < 8; j++) x[s][j] = 0.0f;
       if (src && d < D) {

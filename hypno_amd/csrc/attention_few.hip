@@ -3,8 +3,8 @@
 // tiles of keys on their own, 16 rows at a time, and add up at the end.
 //
 // Bound: HBM.  One token over 131072 positions (32/8 heads of 128, 537 MB): 77 us, 7.0
-// TB/s; 64 sequences of up to 8192 (1.24 GB) 208 us, 5.9; with 8-bit values (0.64 GB) 163
-// us, 3.9: there it is the way through the wave (codes to fp16 and bf16, 310 vector
+// TB/s; 64 sequences of up to 8192 (1.24 GB) 208 us, 5.9; with 8-bit values (0.64 GB) 150
+// us, 4.3: there it is the way through the wave (codes to fp16 and bf16, 310 vector
 // operations a tile, 40% of the cycles) at two waves a SIMD, which is what the registers
 // allow (three with 42 of them spilt: 357 us; tiles of 64 keys, 15 spilt: 206).
 //  * K goes from memory into the MFMA operands' registers, V into LDS, from where it is
@@ -22,6 +22,7 @@ namespace hypno {
 namespace {
 
 constexpr int kQ = 16;
+typedef uint32_t u32x4a8 __attribute__((ext_vector_type(4), aligned(8)));
 
 template <int kType, int DP>
 struct Few {
@@ -57,7 +58,7 @@ __global__ void __launch_bounds__(64 * kWaves, (kWaves == 8 ? 1 : Few<kType, DP>
   const int rows = sq.n * G, b = sq.b;
   if (rows > a.few) return;
   const bool past = too_long(a, sq);
-  const int grp = lane / kQ, col = lane % kQ;
+  const int col = lane % kQ;
   uint8_t* const vbuf = smem + wave * T::kWave;
   float* const ks = reinterpret_cast<float*>(vbuf + T::kBufs * T::kBytes);
   float* const vs = ks + kKeys;
@@ -65,11 +66,16 @@ __global__ void __launch_bounds__(64 * kWaves, (kWaves == 8 ? 1 : Few<kType, DP>
   const int mask = (1 << a.c.page_shift) - 1, item = kType == kKvFp16 ? 2 : 1;
   const uint8_t* const kg = (const uint8_t*)a.c.k + ((size_t)g << a.c.page_shift) * D * item;
   const uint8_t* const vg = (const uint8_t*)a.c.v + ((size_t)g << a.c.page_shift) * D * item;
+  // 8-bit keys of head_dim % 16 = 0 are read 16 codes at a time.
+  const bool pairs = kType == kKvInt8 && D % 16 == 0;
   // A lane's columns of a K row, and its rows and columns of 16 V rows (those past D: the
   // row's first, whose products are with zeros or not used).
   int kcol[R::kSteps], vrow[kVs], vcol[kVs];
 #pragma unroll
-  for (int s = 0; s < R::kSteps; s++) kcol[s] = 32 * s + 8 * grp < D ? 32 * s + 8 * grp : 0;
+  for (int s = 0; s < R::kSteps; s++) {
+    const int d = pairs ? R::template element<true>(s) : R::template element<false>(s);
+    kcol[s] = d < D ? d : 0;
+  }
 #pragma unroll
   for (int i = 0; i < kVs; i++) {
     vrow[i] = (i * 64 + lane) / L::kCh;
@@ -127,11 +133,24 @@ __global__ void __launch_bounds__(64 * kWaves, (kWaves == 8 ? 1 : Few<kType, DP>
                            item;
             off = __umul24(min(p0 + kQ * i + col, hi - 1) & mask, D) * item;
           }
+          if (kType == kKvFp16) {
 #pragma unroll
-          for (int s = 0; s < R::kSteps; s++) {
-            if (kType == kKvFp16)
+            for (int s = 0; s < R::kSteps; s++)
               kf[i][s] = load_global<half8>(src + (off + kcol[s] * 2));
-            else
+          } else if (pairs) {
+#pragma unroll
+            for (int s = 0; s < R::kSteps; s += 2) {
+              if (s + 1 < R::kSteps) {
+                const u32x4a8 c = load_global<u32x4a8>(src + (off + kcol[s]));
+                kc[i][s] = make_uint2(c[0], c[1]);
+                kc[i][s + 1] = make_uint2(c[2], c[3]);
+              } else {
+                kc[i][s] = load_global<uint2>(src + (off + kcol[s]));
+              }
+            }
+          } else {
+#pragma unroll
+            for (int s = 0; s < R::kSteps; s++)
               kc[i][s] = load_global<uint2>(src + (off + kcol[s]));
           }
         }
@@ -175,7 +194,7 @@ __global__ void __launch_bounds__(64 * kWaves, (kWaves == 8 ? 1 : Few<kType, DP>
       look_up(lo + wave * kKeys + step);
     }
     R x;
-    x.init(r0 + col < rows ? a.q + (size_t)t * a.q_stride + (size_t)h * D : nullptr, D, a.scale);
+    x.init(r0 + col < rows ? a.q + (size_t)t * a.q_stride + (size_t)h * D : nullptr, D, a.scale, pairs);
     int buf = 0;
     for (int p0 = lo + wave * kKeys; p0 < hi; p0 += step, buf ^= T::kBufs - 1) {
       typename R::acc s[kRuns];
