@@ -140,7 +140,8 @@ AttnPlan attn_plan(const KvCache& c, const KvBatch& b, int heads, int window, in
       const double each = (double)pairs * seen / slots;
       const double best = b.batch > 1 ? std::sqrt(128.0 * each) : each;
       const int64_t least = std::min<int64_t>(std::max<int64_t>(8 * pairs, 128), 512);
-      const int64_t chunk = std::max(least, ((int64_t)best + 127) / 128 * 128);
+      // (whole steps of four waves: a run of positions must not lie across two ranges)
+      const int64_t chunk = (std::max(least, (int64_t)best) + 127) / 128 * 128;
       p.fs.splits = up(seen, chunk);
       p.fs.chunk = (int)std::min<int64_t>(chunk, 0x7FFFFFFF);
     } else if (pairs <= num_cus && seen > 128) {
