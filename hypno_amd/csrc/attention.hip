@@ -60,7 +60,9 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a) {
     o *= f;
     constexpr int kFly = 8;
     const int cnt = min(64, n - i0), step = 64 / lanes;
-    for (int i = sub; i < cnt; i += kFly * step) {
+    // (all lanes go through every step: a range's weight is read from the lane that has it)
+    for (int at = 0; at < cnt; at += kFly * step) {
+      const int i = at + sub;
       f32x4 v[kFly];
 #pragma unroll
       for (int j = 0; j < kFly; j++)

@@ -82,3 +82,55 @@ def test_odd_batches_times_heads(batch, heads, kv_heads, kv, page, kind):
     assert plan(batch, batch, heads, kv_heads, 64, kv, kind, page).fs.splits > 1
     q = queries(bt.tokens, heads, 64, 60)
     check(run_attend(bt, q), *attend(q, bt))
+
+
+# --- the parts' sum ------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [40, 64, 128, 256])
+@pytest.mark.parametrize("ranges", [9, 10, 32, 33, 34, 35, 48, 49, 50, 64, 65, 66, 129, 131, 134,
+                                    138, 196, 200, 258, 262])
+def test_join_by_four_waves(ranges, dim):
+    """Ranges in all numbers that leave some of a wave's lanes without one, split over
+    four waves."""
+    kv = 128 * ranges - 50
+    bt = Batch([(1, kv)], 16, 61, kv_heads=1, dim=dim)
+    p = plan(1, 1, 2, 1, dim, kv)
+    assert (p.fs.splits, p.fs.chunk) == (ranges, 128)
+    q = queries(1, 2, dim, 61)
+    check(run_attend(bt, q), *attend(q, bt))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [40, 64, 128, 256])
+@pytest.mark.parametrize("ranges", [9, 17, 31, 32, 33, 34, 35, 48, 49, 50, 63, 64, 65, 98])
+def test_join_by_one_wave(ranges, dim):
+    """The same with a wave a row: 1024 rows and more."""
+    kv = 128 * ranges - 50
+    bt = Batch([(1, kv)], 16, 62, kv_heads=1, dim=dim)
+    p = plan(1, 1, 1024, 1, dim, kv)
+    assert (p.fs.splits, p.fs.chunk) == (ranges, 128)
+    q = queries(1, 1024, dim, 62)
+    ref, tol = attend(q[:, ::73], bt)  # (all read one kv head)
+    check(run_attend(bt, q)[:, ::73], ref, tol)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["fp16", "int8"])
+@pytest.mark.parametrize("ranges", [33, 34, 49])
+@pytest.mark.parametrize("tokens,heads,dim", [(20, 4, 64), (20, 4, 128), (70, 16, 64)])
+def test_join_of_tiles(tokens, heads, dim, ranges, kind):
+    """Tiles' ranges, of a sequence shorter than max_kv_len says."""
+    p = plan(1, tokens, heads, 1, dim, 60000, kind)
+    assert p.few == 0 and p.ts.splits >= ranges
+    kv = p.ts.chunk * ranges - 40
+    bt = Batch([(tokens, kv)], 16, 63, kv_heads=1, dim=dim, kind=kind)
+    bt.table = np.concatenate([bt.table, np.full((1, 60000 // 16 - bt.table.shape[1]), -1,
+                                                 np.int32)], 1)
+    q = queries(tokens, heads, dim, 63)
+    got = run_attend(bt, q, max_kv_len=60000)
+    # (the last tokens' rows are in the tile that sees all ranges)
+    last = Batch([(3, kv)], 16, 63, kv_heads=1, dim=dim, kind=kind)
+    last.table, last.k, last.v, last.ks, last.vs = bt.table, bt.k, bt.v, bt.ks, bt.vs
+    ref, tol = attend(q[-3:, ::5], last)
+    check(got[-3:, ::5], ref, tol)
