@@ -13,7 +13,8 @@ sequence b are rows cu_q[b] to cu_q[b + 1].  kv_lens[b] counts what it holds wit
 them, so its i-th new token of n has position kv_lens[b] - n + i.  Position p is in
 slot p % page_size of page page_table[b, p // page_size].  cu_q, kv_lens and
 page_table are int32 and are read on the GPU: a page id that is none of the cache's
-(-1 for a freed one, say) is not written, and what reads it is NaN.
+(-1 for a freed one, say) is not written, and what reads it is NaN.  A table has room
+for less than 2^31 positions a sequence, for attention 2^31 - 4096 at most.
 
 The caches are [pages, kv_heads, page_size, head_dim], float16, or int8 with
 float32 k_scale and v_scale [pages, kv_heads, page_size]: one scale a token and kv

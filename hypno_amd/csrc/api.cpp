@@ -1436,6 +1436,9 @@ int hypno_hip_paged_attention_dev(float* out, const float* q, size_t q_stride, s
                 heads, cache->kv_heads);
   if (T * heads > kMaxInt)
     return fail(HYPNO_HIP_EINVAL, "paged_attention: tokens * heads out of range");
+  // (the kernels add up to some hundred to a sequence's last position before they clamp)
+  if (batch->table_width * cache->page_size > kMaxInt - 4095)
+    return fail(HYPNO_HIP_EINVAL, "paged_attention: table_width * page_size is above 2^31 - 4096");
   size_t qb = 0, ob = 0;
   if ((st = rows_bytes("paged_attention", T, heads * D, q_stride, &qb))) return st;
   if ((st = rows_bytes("paged_attention", T, heads * D, heads * D, &ob))) return st;

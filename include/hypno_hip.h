@@ -429,7 +429,8 @@ typedef struct hypno_hip_kv_batch {
   const int32_t* cu_q;        /* [batch + 1], ascending from 0 */
   const int32_t* kv_lens;     /* [batch] */
   const int32_t* page_table;  /* [batch][table_width] */
-  size_t batch, table_width;
+  size_t batch, table_width;  /* table_width * page_size: below 2^31 (attention: at most
+                               * 2^31 - 4096) */
   size_t tokens;              /* rows of q, k, v: cu_q[batch] */
 } hypno_hip_kv_batch;
 

@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 
 from hypno_amd import _lib
-from test_paged_attention import Batch, attend, check, queries, run_attend
+from test_paged_attention import O, Q, Batch, _kv, attend, check, queries, run_attend
 
 RUN = 16  # positions that attn_few_kernel takes to lie in one page (pages of as many or more)
 
@@ -134,3 +134,36 @@ def test_join_of_tiles(tokens, heads, dim, ranges, kind):
     last.table, last.k, last.v, last.ks, last.vs = bt.table, bt.k, bt.v, bt.ks, bt.vs
     ref, tol = attend(q[-3:, ::5], last)
     check(got[-3:, ::5], ref, tol)
+
+
+# --- the last positions ----------------------------------------------------------------------
+
+@pytest.mark.parametrize("page,width", [(128, (1 << 24) - 1), (1, (1 << 31) - 1), (4096, 1 << 19),
+                                        (1, (1 << 31) - 4095), (16, (1 << 27) - 255)])
+def test_refuses_positions_that_the_kernels_cannot_count(page, width):
+    """The kernels add some tiles to a position in 32 bits before they clamp it."""
+    lib = _lib.load()
+    for tokens in (0, 3):
+        c, b = (ctypes.byref(x) for x in _kv(page_size=page, table_width=width, tokens=tokens))
+        assert lib.hypno_hip_paged_attention_dev(O, Q, 256, 4, c, b, 0.1, 1, 0, None) == 22
+        assert b"paged_attention" in lib.hypno_hip_last_error()
+    # One page less is taken.
+    c, b = (ctypes.byref(x) for x in _kv(page_size=page, tokens=0,
+                                         table_width=((1 << 31) - 4096) // page))
+    assert lib.hypno_hip_paged_attention_dev(O, Q, 256, 4, c, b, 0.1, 1, 0, None) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["fp16", "int8"])
+@pytest.mark.parametrize("window,page", [(1, 64), (70, 8), (70, 4096), (700, 64), (700, 4096)])
+@pytest.mark.parametrize("n", [1, 40])
+def test_last_positions(n, window, page, kind):
+    """A sequence that ends where the longest table does (earlier pages are not there)."""
+    kv = (1 << 31) - 4096
+    bt = Batch([(n, 6 * 4096)], page, 64, kind=kind)
+    held = bt.table[0]
+    bt.table = np.full((1, kv // page), -1, np.int32)
+    bt.table[0, -len(held):] = held
+    bt.seqs, bt.lens = [(n, kv)], np.array([kv], np.int32)
+    q = queries(n, 4, 64, 64)
+    check(run_attend(bt, q, window=window), *attend(q, bt, window=window))
