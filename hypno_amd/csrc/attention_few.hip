@@ -181,7 +181,7 @@ __global__ void __launch_bounds__(64 * kWaves, (kWaves == 8 ? 1 : Few<kType, DP>
 #pragma unroll
           for (int i = 1; i < kRuns; i++) page = lane % kKeys / kRun == i ? pg[i] : page;
         }
-        const int tok = (g << a.c.page_shift) + (min(p0 + lane % kKeys, hi - 1) & mask);
+        const size_t tok = ((size_t)g << a.c.page_shift) + (min(p0 + lane % kKeys, hi - 1) & mask);
         kss = load_global<float>(a.c.k_scale + (size_t)page * a.c.ks_page + tok);
         vss = load_global<float>(a.c.v_scale + (size_t)page * a.c.vs_page + tok);
       }

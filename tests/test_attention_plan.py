@@ -167,3 +167,35 @@ def test_last_positions(n, window, page, kind):
     bt.seqs, bt.lens = [(n, kv)], np.array([kv], np.int32)
     q = queries(n, 4, 64, 64)
     check(run_attend(bt, q, window=window), *attend(q, bt, window=window))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 20])
+def test_pages_of_more_than_2e31_places(n):
+    """One page of 65536 tokens and 32769 kv heads: its last head's scales are 2^31 of them
+    from its first (52 GB)."""
+    import torch
+
+    import hypno_amd as hk
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("needs 60 GB of device memory")
+    kv_heads, page, kv = 32769, 65536, 150
+    at = torch.tensor([0, 1, 77, 32766, 32767, 32768], device="cuda")
+    bt = Batch([(n, kv)], 256, 65, extra=0, kv_heads=len(at), dim=8, kind="int8")
+    q = queries(n, len(at), 8, 65)
+    ref, tol = attend(q, bt)
+    big = {}
+    for name, x in (("k_cache", bt.k), ("v_cache", bt.v), ("k_scale", bt.ks), ("v_scale", bt.vs)):
+        x = torch.from_numpy(x[0, :, :kv]).cuda()
+        t = big[name] = torch.empty((1, kv_heads, page, *x.shape[2:]), dtype=x.dtype,
+                                    device="cuda")
+        t[:, :, :kv] = 1
+        t[0, at, :kv] = x
+    x = torch.ones(n, kv_heads, 8, device="cuda")
+    x[:, at] = torch.from_numpy(q).cuda()
+    i = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    got = hk.paged_attention(x, page_table=i(0)[None], kv_lens=i(kv), cu_q=i(0, n), **big)
+    got = got[:, at].cpu().numpy()
+    del big, t, x
+    torch.cuda.empty_cache()
+    check(got, ref, tol)
