@@ -38,13 +38,15 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a) {
   const bool few = rows <= a.few;
   const AttnSplit sp = few ? a.fs : a.ts;
   if (sp.splits <= 1) return;  // written already
-  const int per = few ? 16 : a.tile_rows, r0 = r / per * per;
+  const int per = few ? kFewRows : a.tile_rows, r0 = r / per * per;
   const bool past = too_long(a, sq);
   const int all = past ? 0 : split_count(sp, span_of(a, sq, r0, min(r0 + per, rows)));
   const int first = all * part / kWaves, n = all * (part + 1) / kWaves - first;
-  const float2* ml = a.part_ml + row * a.row_parts + first;
+  const AttnParts parts = few ? a.fp : a.tp;
+  const size_t at0 = (few ? few_part(a, sq, h / G, r) : row) * sp.splits + first;
+  const float2* ml = parts.ml + at0;
   const int lanes = D <= 64 ? 16 : D <= 128 ? 32 : 64, sub = lane / lanes, d = lane % lanes * 4;
-  const float* po = a.part_o + (row * a.row_parts + first) * D + d;
+  const float* po = parts.o + at0 * D + d;
   float m = -__builtin_inff(), l = 0.0f;
   f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
   for (int i0 = 0; i0 < n; i0 += 64) {
@@ -106,6 +108,10 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a) {
 // From here on a wave a row, not four.
 constexpr unsigned kJoinRows = 1024;
 
+// Bytes of one kernel's ranges at most: a million of them at head_dim 128, where 64
+// sequences of 32 heads take 16 to 32 a row and a chunk of 512 tokens four.
+constexpr size_t kMaxParts = (size_t)512 << 20;
+
 int up(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
 }  // namespace
@@ -122,7 +128,7 @@ AttnPlan attn_plan(const KvCache& c, const KvBatch& b, int heads, int window, in
   // beside the others, which costs less than a second kernel after them).
   const bool only_few = b.tokens <= b.batch || (b.batch == 1 && rows <= 16);
   const bool only_tile = !only_few && (b.batch <= 8 || G > 16);
-  p.few = only_few ? 0x7FFFFFFF : only_tile ? 0 : 16;
+  p.few = only_few ? 0x7FFFFFFF : only_tile ? 0 : kFewRows;
   const int64_t room = (int64_t)b.width << c.page_shift;
   const int64_t kv = std::max<int64_t>(1, max_kv ? std::min(max_kv, room) : room);
   // Up to 1024 positions (2048 where sequences and heads alone fill the chip) a
@@ -135,6 +141,13 @@ AttnPlan attn_plan(const KvCache& c, const KvBatch& b, int heads, int window, in
   // - / 67 / 58 / 53.)
   p.fs = {1, 0x7FFFFFFF};
   p.few_waves = 4;
+  const size_t token_rows = (size_t)b.tokens * heads, place = (size_t)c.head_dim * 4 + 8;
+  const size_t seq_rows = (size_t)b.batch * c.kv_heads * kFewRows;
+  p.by_seq = p.few == kFewRows && seq_rows < token_rows;
+  const size_t few_rows = p.by_seq ? seq_rows : token_rows;
+  const auto most = [&](size_t rows) {  // ranges that kMaxParts has room for
+    return std::max<int64_t>(1, (int64_t)std::min<size_t>(kMaxParts / place / rows, 1 << 30));
+  };
   if (p.few) {
     const int64_t seen = window ? std::min<int64_t>(kv, (int64_t)window + 16) : kv;
     const int64_t pairs = (int64_t)b.batch * c.kv_heads, slots = 2 * num_cus;
@@ -143,7 +156,8 @@ AttnPlan attn_plan(const KvCache& c, const KvBatch& b, int heads, int window, in
       const double best = b.batch > 1 ? std::sqrt(128.0 * each) : each;
       const int64_t least = std::min<int64_t>(std::max<int64_t>(8 * pairs, 128), 512);
       // (whole steps of four waves: a run of positions must not lie across two ranges)
-      const int64_t chunk = (std::max(least, (int64_t)best) + 127) / 128 * 128;
+      const int64_t fit = (seen + most(few_rows) - 1) / most(few_rows);
+      const int64_t chunk = (std::max({least, (int64_t)best, fit}) + 127) / 128 * 128;
       p.fs.splits = up(seen, chunk);
       p.fs.chunk = (int)std::min<int64_t>(chunk, 0x7FFFFFFF);
     } else if (pairs <= num_cus && seen > 128) {
@@ -166,6 +180,7 @@ AttnPlan attn_plan(const KvCache& c, const KvBatch& b, int heads, int window, in
     for (int n = 1; n <= 64; n++) {
       const int64_t chunk = (up(seen, n) + 63) / 64 * 64;
       const int splits = up(seen, chunk);
+      if (splits > most(token_rows)) break;
       const double each = groups * splits <= num_cus ? tile_us : 1.6 * tile_us;
       const double us = std::ceil(groups * splits / (2 * num_cus)) * (4.0 + chunk / 64 * each) +
                         (splits > 1 ? 5.0 + part_us * splits : 0.0);
@@ -176,9 +191,10 @@ AttnPlan attn_plan(const KvCache& c, const KvBatch& b, int heads, int window, in
       }
     }
   }
-  const int most = std::max(p.fs.splits, p.ts.splits);
-  p.ml_bytes = most > 1 ? ((size_t)most * b.tokens * heads * 8 + 255) / 256 * 256 : 0;
-  p.bytes = most > 1 ? p.ml_bytes + (size_t)most * b.tokens * heads * c.head_dim * 4 : 0;
+  p.few_places = p.fs.splits > 1 ? few_rows * p.fs.splits : 0;
+  p.tile_places = p.ts.splits > 1 ? token_rows * p.ts.splits : 0;
+  p.ml_bytes = ((p.few_places + p.tile_places) * 8 + 255) / 256 * 256;
+  p.bytes = p.ml_bytes + (p.few_places + p.tile_places) * c.head_dim * 4;
   return p;
 }
 
@@ -186,11 +202,12 @@ hipError_t launch_paged_attention(const AttnPlan& p, float* out, const float* q,
                                   int heads, const KvCache& c, const KvBatch& b, float scale,
                                   int window, void* ws, hipStream_t s) {
   AttnArgs a = {c, b, out, q, q_stride, heads, heads / c.kv_heads, window, scale,
-                p.few, p.few_waves, p.tile_rows, p.fs, p.ts, p.cus, std::max(p.fs.splits, p.ts.splits),
-                nullptr, nullptr};
+                p.few, p.few_waves, p.tile_rows, p.fs, p.ts, p.cus, p.by_seq, {}, {}};
   if (!ws) a.fs = a.ts = {1, 0x7FFFFFFF};
-  a.part_ml = reinterpret_cast<float2*>(ws);
-  a.part_o = reinterpret_cast<float*>((uint8_t*)ws + p.ml_bytes);
+  a.fp.ml = reinterpret_cast<float2*>(ws);
+  a.tp.ml = a.fp.ml + p.few_places;
+  a.fp.o = reinterpret_cast<float*>((uint8_t*)ws + p.ml_bytes);
+  a.tp.o = a.fp.o + p.few_places * c.head_dim;
   const unsigned rows = (unsigned)b.tokens * (unsigned)heads;
   if (c.pages == 0) {
     attn_rows_kernel<<<rows, 64, 0, s>>>(a);

@@ -28,6 +28,15 @@ typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
 typedef uint32_t uint2_t __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4), aligned(4)));  // (rows at any float)
 
+// What the ranges of rows gave: [row][range], of o [head_dim] each.
+struct AttnParts {
+  float2* ml;  // maximum (log2), sum
+  float* o;
+};
+
+// Rows of a sequence that attn_few_kernel takes beside attn_tile_kernel.
+constexpr int kFewRows = 16;
+
 struct AttnArgs {
   KvCache c;
   KvBatch b;
@@ -41,9 +50,8 @@ struct AttnArgs {
   int tile_rows;          // rows of a work-group of the other
   AttnSplit fs, ts;       // of attn_few_kernel and attn_tile_kernel
   int cus;
-  int row_parts;          // the larger of both splits
-  float* part_o;          // [token][head][row_parts][head_dim], if that is above 1
-  float2* part_ml;        // [token][head][row_parts]: maximum (log2), sum
+  int by_seq;             // fp's rows: see few_part
+  AttnParts fp, tp;       // of the two kernels, where they take ranges
 };
 
 // The new tokens of a sequence and what it holds (both at least 0).
@@ -87,6 +95,14 @@ __device__ __forceinline__ Span span_of(const AttnArgs& a, const Seq& s, int r0,
 // Ranges that a span is split into (0: nothing is seen).
 __device__ __forceinline__ int split_count(const AttnSplit& sp, const Span& x) {
   return x.hi <= x.lo ? 0 : min(sp.splits, (x.hi - x.lo - 1) / sp.chunk + 1);
+}
+
+// Row r (of kv head g) of a sequence among the rows of fp: by sequence kFewRows for each kv
+// head, where both kernels run and that is less than a row for each (token, head), which
+// it is otherwise (as in tp).
+__device__ __forceinline__ size_t few_part(const AttnArgs& a, const Seq& s, int g, int r) {
+  return a.by_seq ? ((size_t)s.b * a.c.kv_heads + g) * kFewRows + r
+                  : (size_t)(s.first + r / a.group) * a.heads + g * a.group + r % a.group;
 }
 
 // One row by a wave, plainly, sums in 64 bits.

@@ -21,7 +21,7 @@ namespace hypno {
 
 namespace {
 
-constexpr int kQ = 16;
+constexpr int kQ = kFewRows;
 typedef uint32_t u32x4a8 __attribute__((ext_vector_type(4), aligned(8)));
 
 template <int kType, int DP>
@@ -263,10 +263,10 @@ __global__ void __launch_bounds__(64 * kWaves, (kWaves == 8 ? 1 : Few<kType, DP>
     const bool live = r0 + or_ < rows;
     const int rr = min(r0 + or_, rows - 1);
     const size_t orow = (size_t)(sq.first + rr / G) * a.heads + g * G + rr % G;
-    const size_t prow = orow * a.row_parts + split;
+    const size_t prow = few_part(a, sq, g, rr) * a.fs.splits + split;
     const bool parts = a.fs.splits > 1;
     const float inv = parts ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
-    float* const dst = parts ? a.part_o + prow * D : a.out + orow * D;
+    float* const dst = parts ? a.fp.o + prow * D : a.out + orow * D;
     float z = l * 0.0f;
     if (live) {
       for (int d = 4 * piece; d < D; d += 16 * kWaves) {
@@ -279,7 +279,7 @@ __global__ void __launch_bounds__(64 * kWaves, (kWaves == 8 ? 1 : Few<kType, DP>
         for (int j = 0; j < 4; j++) z += v[j] * 0.0f;
         *reinterpret_cast<f32x4*>(dst + d) = v;
       }
-      if (parts && piece == 0) a.part_ml[prow] = make_float2(m, l);
+      if (parts && piece == 0) a.fp.ml[prow] = make_float2(m, l);
       if (!parts && (!(z == 0.0f) || past)) atomicOr(&again, 1u << or_);
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");

@@ -228,8 +228,8 @@ __global__ void __launch_bounds__(256, 2) attn_tile_kernel(AttnArgs a) {
   const size_t orow = (size_t)t * a.heads + h;
   if (a.ts.splits > 1) {
     if (!live) return;
-    const size_t part = orow * a.row_parts + split;
-    float* po = a.part_o + part * D;
+    const size_t part = orow * a.ts.splits + split;
+    float* po = a.tp.o + part * D;
 #pragma unroll
     for (int k = 0; k < R::kDt; k++)
 #pragma unroll
@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(256, 2) attn_tile_kernel(AttnArgs a) {
           *reinterpret_cast<f32x4*>(po + d) =
               f32x4{x.o[k][i], x.o[k][i + 1], x.o[k][i + 2], x.o[k][i + 3]};
       }
-    if (lane < NQ) a.part_ml[part] = make_float2(x.m, x.l);
+    if (lane < NQ) a.tp.ml[part] = make_float2(x.m, x.l);
     return;
   }
   const float inv = x.l == 0.0f ? 0.0f : 1.0f / x.l;

@@ -71,7 +71,8 @@ struct AttnSplit {
   int splits, chunk;
 };
 
-// How a call's rows and positions are split, and the workspace that takes.
+// How a call's rows and positions are split, and the workspace that takes: a place for
+// each range of each row that a kernel may have (none where it takes no ranges).
 struct AttnPlan {
   int few;        // sequences of at most so many rows go to attn_few_kernel
   int few_waves;  // of its work-groups
@@ -79,6 +80,8 @@ struct AttnPlan {
   int cus;
   AttnSplit fs, ts;
   size_t bytes, ml_bytes;
+  size_t few_places, tile_places;
+  bool by_seq;    // attn_few_kernel's rows are counted by sequence, not by token
 };
 AttnPlan attn_plan(const KvCache& c, const KvBatch& b, int heads, int window, int64_t max_kv,
                    int num_cus);

@@ -480,8 +480,8 @@ int hypno_hip_append_kv_dev(const hypno_hip_kv_cache* cache, const hypno_hip_kv_
  * (FP16) or to all 24 (INT8).  out [tokens][heads][head_dim], fp32; it may not share
  * memory with an input.  max_kv_len: an upper bound of kv_lens that the host knows (0:
  * table_width * page_size); it sets how many work-groups share a sequence, never the
- * result's range.  Calls whose positions are split use the stream's workspace; under
- * capture, without one that is large enough, they are not split. */
+ * result's range.  Calls whose positions are split use the stream's workspace (1 GB at
+ * most); under capture, without one that is large enough, they are not split. */
 int hypno_hip_paged_attention_dev(float* out, const float* q, size_t q_stride, size_t heads,
                                   const hypno_hip_kv_cache* cache,
                                   const hypno_hip_kv_batch* batch, float scale, size_t window,

@@ -33,7 +33,8 @@ class Split(ctypes.Structure):
 class Plan(ctypes.Structure):
     """The first members of AttnPlan, and room for the rest."""
     _fields_ = [("few", ctypes.c_int), ("few_waves", ctypes.c_int), ("tile_rows", ctypes.c_int),
-                ("cus", ctypes.c_int), ("fs", Split), ("ts", Split), ("rest", ctypes.c_byte * 256)]
+                ("cus", ctypes.c_int), ("fs", Split), ("ts", Split), ("bytes", ctypes.c_size_t),
+                ("rest", ctypes.c_byte * 256)]
 
 
 def plan(batch, tokens, heads, kv_heads, dim, kv, kind="fp16", page=16, window=0, max_kv=0,
@@ -66,6 +67,50 @@ def test_ranges_are_whole_runs():
                                 assert s.chunk % RUN == 0, (batch, kv_heads, kv, tokens, s.chunk)
                                 seen.add(s.chunk)
     assert len(seen) > 10
+
+
+def places(p, dim):
+    return p.bytes // (4 * dim + 8)
+
+
+def test_workspace_goes_by_the_rows_that_take_ranges():
+    """Ranges of a long context beside a prompt take room for the few rows that have them,
+    and no call more than 512 MB a kernel."""
+    # One sequence of 8192 new tokens and eight of one, 131072 positions at most.
+    p = plan(9, 8200, 32, 8, 128, 131072)
+    assert p.few == 16 and p.fs.splits > 50 and 1 < p.ts.splits < 5
+    assert places(p, 128) == p.fs.splits * 9 * 8 * 16 + p.ts.splits * 8200 * 32
+    p = plan(16, 2063, 32, 8, 128, 131072)
+    assert p.fs.splits > 30 and p.bytes < 512 << 20
+    for batch in (1, 2, 8, 9, 17, 64, 256, 1000):
+        for new in (1, 2, 7, 40, 300, 2400, 10000):
+            for heads, kv_heads, dim in ((32, 8, 128), (12, 12, 64), (64, 1, 256), (7, 7, 40)):
+                for kv in (1500, 9000, 131072, 1 << 24):
+                    tokens = batch - 1 + new
+                    if tokens * heads > 2 ** 31 or batch * kv > 2 ** 31:
+                        continue
+                    p = plan(batch, tokens, heads, kv_heads, dim, kv)
+                    assert p.bytes <= (512 << 20) * (2 if p.few == 16 else 1) + 256
+                    if batch == 1 and new * heads // kv_heads <= 16 and kv > 1500:
+                        assert p.fs.splits > 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["fp16", "int8"])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(4, 2, 64), (8, 8, 40), (16, 1, 128)])
+@pytest.mark.parametrize("tokens", [20, 300])
+def test_ranges_of_both_kernels(tokens, heads, kv_heads, dim, kind):
+    """Chunks and single tokens in one call, both in ranges; rows counted by token and by
+    sequence."""
+    seqs = [(1, 3100), (tokens, 2600), (1, 2), (2, 1500), (0, 900), (1, 2100), (30, 3000), (1, 1111),
+            (16 * kv_heads // heads, 1900), (1, 3090)]
+    bt = Batch(seqs, 16, 66, kv_heads=kv_heads, dim=dim, kind=kind)
+    p = plan(len(seqs), bt.tokens, heads, kv_heads, dim, 3100, kind)
+    assert p.few == 16 and p.fs.splits > 1 and p.ts.splits > 1
+    q = queries(bt.tokens, heads, dim, 66)
+    rows = np.r_[0:bt.cu[1] + 2, bt.cu[2] - 2:bt.cu[6] + 2, bt.cu[7] - 2:bt.tokens]
+    ref, tol = attend(q, bt)
+    check(run_attend(bt, q)[rows], ref[rows], tol[rows])
 
 
 # Batches times kv heads whose ranges' least length (8 positions for each) is no multiple
