@@ -27,10 +27,9 @@ from __future__ import annotations
 
 import ctypes
 import math
-import os
 import struct
 
-from ._lib import HERE, check, load
+from ._lib import check, load
 
 __all__ = ["append_kv", "paged_attention"]
 
@@ -44,15 +43,26 @@ torch = None
 _args = None  # csrc/attention_args.cpp: the same checks and packing, where all is right
 
 
+class _NoArgs:
+    """Stands for it where it was not built."""
+
+    @staticmethod
+    def append_kv(*_):
+        return NotImplemented
+
+    paged_attention = append_kv
+
+
 def _torch():
     """(imported by the first call: the rest of the package works without it)"""
     global torch, _args
     import torch
     lib = load()
-    if not os.path.exists(os.path.join(HERE, "_attention_args.so")):
-        raise ImportError("hypno_amd/_attention_args.so is missing: build it with "
-                          "`python -m hypno_amd.build`")
-    from . import _attention_args
+    try:
+        from . import _attention_args
+    except ImportError:
+        _args = _NoArgs
+        return
     _attention_args.bind(
         *(ctypes.cast(f, ctypes.c_void_p).value
           for f in (lib.hypno_hip_append_kv_dev, lib.hypno_hip_paged_attention_dev)),

@@ -81,13 +81,21 @@ def _compile(src: str) -> str:
 
 
 def _build_args() -> None:
-    """Host code that reads torch's tensors (a Python module beside the library)."""
-    try:
-        import torch
-        from torch.utils.cpp_extension import include_paths
-    except ImportError:
-        return  # (its callers need torch too)
+    """Host code that reads torch's tensors (a Python module beside the library).  Where it
+    does not build (no g++, no headers of Python or torch), attention.py does without it,
+    some microseconds a call slower."""
     out = os.path.join(HERE, "_attention_args.so")
+    try:
+        _compile_args(out)
+    except (ImportError, OSError, RuntimeError) as e:
+        sys.stderr.write(f"_attention_args.so (optional) was not built: {e}\n")
+        if os.path.exists(out):
+            os.remove(out)  # (of other sources)
+
+
+def _compile_args(out: str) -> None:
+    import torch
+    from torch.utils.cpp_extension import include_paths
     libs = os.path.join(os.path.dirname(torch.__file__), "lib")
     cmd = ["g++", "-O2", "-fPIC", "-shared", "-std=c++17", "-w",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}"]
