@@ -11,9 +11,13 @@
 //
 // Arithmetic: the cache's values are fp16 or 8-bit codes, both exact as MFMA operands.
 // q (scaled by a power of two per row) goes in as two fp16, 22 bits, every product
-// twice.  The weights go in as two fp16 beside fp16 values (22 bits, or 2^-37 of the
-// row's largest), and times the values' scale as three bf16, all of an fp32, beside
-// 8-bit ones: a code of 0 beside the largest weight leaves an element to the smallest.
+// twice.  The weights times the values' scale go in as three bf16, all of an fp32, beside
+// 8-bit values: a code of 0 beside the largest weight leaves an element to the smallest.
+// Beside fp16 values they go in as two fp16: 22 bits down to 2^-15 of the row's largest, and
+// steps of 2^-36 of that largest below.  That adds at most 2^-37 of the sum of the |values|
+// seen to an element, far less than the heaviest keys' own values round off, but all that
+// there is where those are 0 and the rest weighs e^-26.  (fp16 values are no bf16: three
+// parts of the weights would take two of the values and three times the products.)
 // Sums are fp32.  What this cannot hold (infinities and NaN anywhere in a tile, masked
 // places among them, pages that are none) ends in a sum that is no finite number, and
 // such a row is computed again by attn_row.

@@ -476,8 +476,12 @@ int hypno_hip_append_kv_dev(const hypno_hip_kv_cache* cache, const hypno_hip_kv_
  * positions p <= the token's own (and, with window > 0, > its own - window) of kv head
  * h / (heads / kv_heads).  Zeros where that leaves none, or no w_p but 0.  The cache's
  * values are used exactly; sums and softmax statistics are fp32; q is held to 22 bits of
- * its row's largest element and more, w to 22 bits down to 2^-36 of the row's largest
- * (FP16) or to all 24 (INT8).  out [tokens][heads][head_dim], fp32; it may not share
+ * its row's largest element and more.  Beside an INT8 cache w is held to all 24 bits;
+ * beside an FP16 one to 22, but to no less than 2^-37 of the row's largest w: from 2^-15 of
+ * that largest on a w has fewer bits, from 2^-37 on none.  That is below fp32's rounding of
+ * the heaviest keys' values unless these are 0 or nearly so: an element of out that then
+ * comes from w of e^-20 of the largest may be off by 0.4%, one from w of e^-26 is 0.
+ * out [tokens][heads][head_dim], fp32; it may not share
  * memory with an input.  max_kv_len: an upper bound of kv_lens that the host knows (0:
  * table_width * page_size); it sets how many work-groups share a sequence, never the
  * result's range.  Calls whose positions are split use the stream's workspace (1 GB at

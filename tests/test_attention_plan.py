@@ -244,3 +244,32 @@ def test_pages_of_more_than_2e31_places(n):
     del big, t, x
     torch.cuda.empty_cache()
     check(got, ref, tol)
+
+
+# --- small weights ----------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["fp16", "int8"])
+@pytest.mark.parametrize("n", [1, 40])
+@pytest.mark.parametrize("score", [9, 12, 15, 18, 20, 22, 24, 26, 30, 60])
+def test_small_weights(score, n, kind):
+    """A first key whose value is 0 beside 3000 of weight e^-score: fp32's bits beside 8-bit
+    codes; beside fp16 values each weight is off by 2^-37 of the largest at most."""
+    kv = 3000
+    bt = Batch([(n, kv)], 64, 67, kv_heads=1, kind=kind)
+    pg, sl = bt.place(0, np.arange(kv))
+    q = np.zeros((n, 2, 64), np.float32)
+    q[:, :, 0] = 8.0
+    bt.k[pg, 0, sl, 0] = 0
+    bt.v[pg, 0, sl] = np.abs(bt.v[pg, 0, sl].astype(np.float32)).astype(bt.v.dtype)
+    bt.v[pg[0], 0, sl[0]] = 0
+    if kind == "fp16":
+        bt.k[pg[0], 0, sl[0], 0] = score
+    else:
+        bt.k[pg[0], 0, sl[0], 0] = 120
+        bt.ks[:] = score / 120
+    ref, tol = attend(q, bt)
+    if kind == "fp16":
+        v = np.abs(bt.v[pg, 0, sl].astype(np.float64))
+        tol += 2.0 ** -37 * v.sum(0)
+    check(run_attend(bt, q), ref, tol)
