@@ -25,7 +25,7 @@ template <int kWaves>
 __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a) {
   __shared__ f32x4 so[4][64];
   __shared__ float2 sml[4];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int part = wave % kWaves;
   const size_t row = (size_t)blockIdx.x * (4 / kWaves) + wave / kWaves;
   const int t = (int)(row / a.heads), h = (int)(row % a.heads);
@@ -43,7 +43,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a) {
   const int all = past ? 0 : split_count(sp, span_of(a, sq, r0, min(r0 + per, rows)));
   const int first = all * part / kWaves, n = all * (part + 1) / kWaves - first;
   const AttnParts parts = few ? a.fp : a.tp;
-  const size_t at0 = (few ? few_part(a, sq, h / G, r) : row) * sp.splits + first;
+  const size_t at0 = (few ? few_part(a, sq, h / G, r, row) : row) * sp.splits + first;
   const float2* ml = parts.ml + at0;
   const int lanes = D <= 64 ? 16 : D <= 128 ? 32 : 64, sub = lane / lanes, d = lane % lanes * 4;
   const float* po = parts.o + at0 * D + d;
@@ -72,7 +72,9 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a) {
           v[j] = load_global<f32x4>(po + (size_t)(i0 + i + j * step) * D);
 #pragma unroll
       for (int j = 0; j < kFly; j++) {
-        const float wj = __shfl(w, min(i + j * step, 63), 64);
+        // (the lane's number goes modulo 64)
+        const float wj = __int_as_float(
+            __builtin_amdgcn_ds_bpermute((i + j * step) << 2, __float_as_int(w)));
         if (i + j * step < cnt && d < D) o += v[j] * wj;
       }
     }

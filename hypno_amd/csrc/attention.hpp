@@ -101,12 +101,12 @@ __device__ __forceinline__ int split_count(const AttnSplit& sp, const Span& x) {
   return x.hi <= x.lo ? 0 : min(sp.splits, (x.hi - x.lo - 1) / sp.chunk + 1);
 }
 
-// Row r (of kv head g) of a sequence among the rows of fp: by sequence kFewRows for each kv
-// head, where both kernels run and that is less than a row for each (token, head), which
-// it is otherwise (as in tp).
-__device__ __forceinline__ size_t few_part(const AttnArgs& a, const Seq& s, int g, int r) {
-  return a.by_seq ? ((size_t)s.b * a.c.kv_heads + g) * kFewRows + r
-                  : (size_t)(s.first + r / a.group) * a.heads + g * a.group + r % a.group;
+// Row r (of kv head g) of a sequence, `row` of all (token, head), among the rows of fp: by
+// sequence kFewRows for each kv head, where both kernels run and that is less than a row
+// for each (token, head), which it is otherwise (as in tp).
+__device__ __forceinline__ size_t few_part(const AttnArgs& a, const Seq& s, int g, int r,
+                                           size_t row) {
+  return a.by_seq ? ((size_t)s.b * a.c.kv_heads + g) * kFewRows + r : row;
 }
 
 // One row by a wave, plainly, sums in 64 bits.

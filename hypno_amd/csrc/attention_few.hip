@@ -263,7 +263,7 @@ __global__ void __launch_bounds__(64 * kWaves, (kWaves == 8 ? 1 : Few<kType, DP>
     const bool live = r0 + or_ < rows;
     const int rr = min(r0 + or_, rows - 1);
     const size_t orow = (size_t)(sq.first + rr / G) * a.heads + g * G + rr % G;
-    const size_t prow = few_part(a, sq, g, rr) * a.fs.splits + split;
+    const size_t prow = few_part(a, sq, g, rr, orow) * a.fs.splits + split;
     const bool parts = a.fs.splits > 1;
     const float inv = parts ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
     float* const dst = parts ? a.fp.o + prow * D : a.out + orow * D;
