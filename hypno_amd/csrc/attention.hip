@@ -1,5 +1,5 @@
 // Attention of each sequence's new tokens over its pages of the cache: which kernels
-// a call takes, and the sum of what a row's ranges of positions gave (5 us for 64 ranges
+// a call takes, and the sum of what a row's ranges of positions gave (5.6 us for 64 ranges
 // of 32 rows, 15 for four of 16384, 42 MB: 2.8 TB/s).
 #include <cmath>
 
@@ -126,8 +126,14 @@ AttnPlan attn_plan(const KvCache& c, const KvBatch& b, int heads, int window, in
   const int64_t rows = (int64_t)b.tokens * G;
   p.tile_rows = c.head_dim <= 128 ? 128 : 64;
   // Single tokens, or one sequence of few rows: attn_few_kernel alone.  Few sequences, or
-  // groups of more than 16: attn_tile_kernel alone (single tokens among them then run
-  // beside the others, which costs less than a second kernel after them).
+  // groups of more than 16: attn_tile_kernel alone, where single tokens run beside the
+  // others and not in a second kernel after them.  (us at 32/8 heads of 128, one kernel /
+  // both: 333 tokens over 700 / 2000 / 5000 / 16000 beside seven single ones 28 / 39, 50 / 62,
+  // 88 / 113, 273 / 305; with 8-bit values 43 / 51, 69 / 76, 134 / 148, 401 / 416; 40 tokens
+  // over 2000 beside three 24 / 28 and 30 / 34; a group of 32, 16 sequences, 46 / 48 to 75 /
+  // 76.  It costs where no chunk fills the tiles: five tokens beside seven over 16000 116 /
+  // 101, with 8-bit values over 2000 and 16000 45 / 29 and 169 / 101; 40 tokens over 16000
+  // beside three, 8-bit, 113 / 102.)
   const bool only_few = b.tokens <= b.batch || (b.batch == 1 && rows <= 16);
   const bool only_tile = !only_few && (b.batch <= 8 || G > 16);
   p.few = only_few ? 0x7FFFFFFF : only_tile ? 0 : kFewRows;

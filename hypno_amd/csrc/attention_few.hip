@@ -2,9 +2,9 @@
 // one kv head of a sequence and a range of its positions; its waves run through
 // tiles of keys on their own, 16 rows at a time, and add up at the end.
 //
-// Bound: HBM.  One token over 131072 positions (32/8 heads of 128, 537 MB): 77 us, 7.0
-// TB/s; 64 sequences of up to 8192 (1.24 GB) 208 us, 5.9; with 8-bit values (0.64 GB) 150
-// us, 4.3: there it is the way through the wave (codes to fp16 and bf16, 310 vector
+// Bound: HBM.  One token over 131072 positions (32/8 heads of 128, 537 MB): 78 us, 6.9
+// TB/s; 64 sequences of up to 8192 (1.24 GB) 211 us with the sum of their ranges, 5.9; with
+// 8-bit values (0.64 GB) 151 us, 4.3: there it is the way through the wave (codes to fp16 and bf16, 310 vector
 // operations a tile, 40% of the cycles) at two waves a SIMD, which is what the registers
 // allow (three with 42 of them spilt: 357 us; tiles of 64 keys, 15 spilt: 206).
 //  * K goes from memory into the MFMA operands' registers, V into LDS, from where it is
@@ -168,8 +168,9 @@ __global__ void __launch_bounds__(64 * kWaves, (kWaves == 8 ? 1 : Few<kType, DP>
           if (kType == kKvInt8)
             vc[i * kVs + j] = load_global<uint2>(vp + off);
           else if (kOne)
-            // (non-temporal; K is not, as each line of it is read by several loads: one
-            // token over 131072 positions takes 98 us with neither, 91 with both, 83 so)
+            // (non-temporal; K is not, as each line of it is read by several loads: the 64
+            // sequences take 230 us with neither, 217 with both, 211 so; one token over
+            // 131072 positions 98, 88 and 88)
             dma16<true>(vp, off, dst + j * 1024);
           else
             dma16(vp + off, dst + j * 1024);

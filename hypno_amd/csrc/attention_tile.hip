@@ -4,9 +4,9 @@
 //
 // Bound: the matrix cores, at the clock that power leaves them.  Each product goes in
 // twice (the two parts of q and of the weights), so that 8192 tokens of 32/8 heads of 128
-// (0.55 PFLOP) issue 1.1 PFLOP: 0.93 ms, 1.19 PFLOP/s, where nothing but these MFMAs on
+// (0.55 PFLOP) issue 1.1 PFLOP: 0.94 ms, 1.17 PFLOP/s, where nothing but these MFMAs on
 // random data reaches 1.6 (2.46 on zeros: the clock falls) and a large fp16 product of
-// the library 1.3.  MFMAs are busy 68% of the cycles, at 1.62 GHz.
+// the library 1.3.  MFMAs are busy 67% of the cycles, at 1.6 GHz.
 //  * 32 rows a wave (32x32x16 MFMA): each piece of K or V that it reads from LDS feeds
 //    two MFMAs, and without these reads the whole takes 5% less; 64 rows would need 512
 //    registers.  With head_dim above 128, 16 rows: 32 need the registers of two waves for
@@ -16,8 +16,9 @@
 //  * Rows of one kv head from all of its query heads: K and V are read once for the group,
 //    and a causal tile ends after 128 / group tokens.
 //  * Work-groups of one kv head share an XCD's L2 (see the order in the kernel).
-// A prompt of 2048: 78 us; its longest work-group's 32 tiles one after the other are 60
-// of it.  512 tokens over 16384: 239 us, 15 more to join four ranges.
+// A prompt of 2048: 80 us; its longest work-group's 32 tiles one after the other are 60
+// of it, the last of them alone on a CU whose short work-group has ended.  512 tokens over
+// 16384: 258 us, 15 of them to join four ranges.
 
 #include <type_traits>
 
