@@ -1,4 +1,4 @@
-"""Builds libhypno_hip.so (gfx950) in-tree with hipcc, and _attention_args.so (host
+"""Builds libhypno_hip.so (gfx950) in-tree with hipcc, and _attention_args.so (optional host
 code over torch's headers) with g++.
 
     python -m hypno_amd.build        # or hypno_amd.build.build()
