@@ -14,7 +14,9 @@ them, so its i-th new token of n has position kv_lens[b] - n + i.  Position p is
 slot p % page_size of page page_table[b, p // page_size].  cu_q, kv_lens and
 page_table are int32 and are read on the GPU: a page id that is none of the cache's
 (-1 for a freed one, say) is not written, and what reads it is NaN.  A table has room
-for less than 2^31 positions a sequence, for attention 2^31 - 4096 at most.
+for less than 2^31 positions a sequence, for attention 2^31 - 4096 at most.  Rows of q,
+k and v of no sequence (past cu_q's last, for padding) are left alone: so are the outputs'
+rows in `out`, which in a new tensor hold anything.
 
 The caches are [pages, kv_heads, page_size, head_dim], float16, or int8 with
 float32 k_scale and v_scale [pages, kv_heads, page_size]: one scale a token and kv
