@@ -497,7 +497,7 @@ def run(state):
         return _plain_selected(s)
     if c["op"] == "bounds":
         if own:
-            hk.page_bounds(s["kc"], s["bc"], s["bs"], **batch, k_scale=s["ks"])
+            hk.key_bounds(s["kc"], s["bc"], s["bs"], **batch, k_scale=s["ks"])
         else:
             _plain_bounds(s)
         # (the values that the codes stand for)
