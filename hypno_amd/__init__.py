@@ -38,7 +38,13 @@ from .kernels import (  # noqa: F401
     unregister_weight,
 )
 
-from .attention import append_kv, paged_attention  # noqa: F401
+from .attention import (  # noqa: F401
+    append_kv,
+    key_bounds,
+    paged_attention,
+    select_pages,
+    selected_attention,
+)
 from .model import FormatError, HypnoModel  # noqa: F401
 
 __version__ = "0.1.0"

@@ -56,6 +56,10 @@ SIGNATURES = {
                                      _sz, _u32, _vp]),
     "hypno_hip_paged_attention_dev": (_i, [_vp, _vp, _sz, _sz, _vp, _vp, ctypes.c_float, _sz, _sz,
                                            _vp]),
+    "hypno_hip_key_bounds_dev": (_i, [_vp, _vp, _vp, _vp]),
+    "hypno_hip_select_pages_dev": (_i, [_vp, _sz, _sz, _sz, _vp, _sz, _sz, _vp, _vp, _sz, _vp]),
+    "hypno_hip_selected_attention_dev": (_i, [_vp, _vp, _sz, _sz, _vp, _vp, ctypes.c_float, _vp,
+                                              _sz, _vp]),
     "hypno_hip_model_open": (_i, [ctypes.c_char_p, _u32, ctypes.POINTER(_vp)]),
     "hypno_hip_model_close": (_i, [_vp]),
     "hypno_hip_model_header": (_i, [_vp, ctypes.POINTER(_u32), ctypes.POINTER(_u32),
@@ -92,6 +96,14 @@ class KvCache(ctypes.Structure):
                 ("k_page_stride", ctypes.c_size_t), ("v_page_stride", ctypes.c_size_t),
                 ("k_scale_page_stride", ctypes.c_size_t),
                 ("v_scale_page_stride", ctypes.c_size_t)]
+
+
+class KeyBounds(ctypes.Structure):
+    """struct hypno_hip_key_bounds of include/hypno_hip.h."""
+    _fields_ = [("codes", ctypes.c_void_p), ("scale", ctypes.c_void_p),
+                ("pages", ctypes.c_size_t), ("kv_heads", ctypes.c_size_t),
+                ("page_size", ctypes.c_size_t), ("head_dim", ctypes.c_size_t),
+                ("page_stride", ctypes.c_size_t), ("scale_page_stride", ctypes.c_size_t)]
 
 
 class KvBatch(ctypes.Structure):

@@ -20,7 +20,20 @@ rows in `out`, which in a new tensor hold anything.
 
 The caches are [pages, kv_heads, page_size, head_dim], float16, or int8 with
 float32 k_scale and v_scale [pages, kv_heads, page_size]: one scale a token and kv
-head.  Pages may be strided (a pool of [pages, layers, ...]); the rest is contiguous.
+head.  In 4 bits they are uint8 [pages, kv_heads, page_size, head_dim / 2] with
+float16 k_scale and v_scale [pages, kv_heads, head_dim / 32, page_size]: one scale
+for 32 elements (head_dim: a multiple of 32, page_size: 16 or more).  Pages may be
+strided (a pool of [pages, layers, ...]); the rest is contiguous.
+
+Of a long context a token may read some pages only, chosen by a cheap score of each:
+
+    key_bounds(k_cache, bounds, bounds_scale, page_table, kv_lens, cu_q)
+    pages = select_pages(q, bounds, bounds_scale, page_size, page_table, kv_lens, cu_q, count)
+    o = selected_attention(q, k_cache, v_cache, pages, page_table, kv_lens, cu_q)
+
+after append_kv and in place of paged_attention.  The bounds (int8 [pages, kv_heads, 2,
+head_dim] and float32 [pages, kv_heads], kept beside the cache, any type of it) hold
+each page's smallest and largest key in every channel.
 
 Arguments that cannot be right raise ValueError; a library failure raises
 HypnoHipError.
@@ -33,13 +46,16 @@ import struct
 
 from ._lib import check, load
 
-__all__ = ["append_kv", "paged_attention"]
+__all__ = ["append_kv", "paged_attention", "key_bounds", "select_pages", "selected_attention"]
 
 _STYLES = {"halves": 0, "pairs": 1}  # HYPNO_HIP_ROPE_*
 
-# The structs of include/hypno_hip.h (_lib.KvCache and _lib.KvBatch), packed at once.
+# The structs of include/hypno_hip.h (_lib.KvCache, KvBatch and KeyBounds), packed at once.
 _CACHE = struct.Struct("=I4x12Q")
 _BATCH = struct.Struct("=6Q")
+_BOUNDS = struct.Struct("=8Q")
+
+_ANY = 0x7FFFFFFF  # tokens of a batch whose rows are in no tensor of the call
 
 torch = None
 _args = None  # csrc/attention_args.cpp: the same checks and packing, where all is right
@@ -52,7 +68,7 @@ class _NoArgs:
     def append_kv(*_):
         return NotImplemented
 
-    paged_attention = append_kv
+    paged_attention = key_bounds = select_pages = selected_attention = append_kv
 
 
 def _torch():
@@ -67,7 +83,9 @@ def _torch():
         return
     _attention_args.bind(
         *(ctypes.cast(f, ctypes.c_void_p).value
-          for f in (lib.hypno_hip_append_kv_dev, lib.hypno_hip_paged_attention_dev)),
+          for f in (lib.hypno_hip_append_kv_dev, lib.hypno_hip_paged_attention_dev,
+                    lib.hypno_hip_key_bounds_dev, lib.hypno_hip_select_pages_dev,
+                    lib.hypno_hip_selected_attention_dev)),
         torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream)
     _args = _attention_args
 
@@ -121,15 +139,25 @@ def _cache(k_cache, v_cache, k_scale, v_scale, dev: int):
             k_cache.get_device() != dev or v_cache.get_device() != dev:
         raise ValueError(f"k_cache and v_cache must be tensors on GPU {dev}")
     dtype, shape = k_cache.dtype, k_cache.shape
-    int8 = dtype is torch.int8
-    if not int8 and dtype is not torch.float16:
-        raise ValueError(f"k_cache must be float16 or int8, got {dtype}")
+    int8, fp4 = dtype is torch.int8, dtype is torch.uint8
+    if not int8 and not fp4 and dtype is not torch.float16:
+        raise ValueError(f"k_cache must be float16, int8 or uint8 (two 4-bit codes), got {dtype}")
     if len(shape) != 4 or v_cache.shape != shape or v_cache.dtype is not dtype:
         raise ValueError("k_cache and v_cache must be [pages, kv_heads, page_size, head_dim] of "
                          "one type")
     pages, heads, size, dim = shape
     ks = vs = kss = vss = 0
-    if int8:
+    if fp4:
+        dim *= 2
+        want = (pages, heads, dim // 32, size)
+        for t, what in ((k_scale, "k_scale"), (v_scale, "v_scale")):
+            if not isinstance(t, torch.Tensor) or t.get_device() != dev or \
+                    t.dtype is not torch.float16 or t.shape != want:
+                raise ValueError(f"{what} must be float16 [pages, kv_heads, head_dim / 32, "
+                                 f"page_size] on GPU {dev} beside a 4-bit cache")
+        ks, kss = k_scale.data_ptr(), _page_stride(k_scale, "k_scale")
+        vs, vss = v_scale.data_ptr(), _page_stride(v_scale, "v_scale")
+    elif int8:
         for t, what in ((k_scale, "k_scale"), (v_scale, "v_scale")):
             if not isinstance(t, torch.Tensor) or t.get_device() != dev or \
                     t.dtype is not torch.float32 or t.shape != shape[:3]:
@@ -139,7 +167,7 @@ def _cache(k_cache, v_cache, k_scale, v_scale, dev: int):
         vs, vss = v_scale.data_ptr(), _page_stride(v_scale, "v_scale")
     elif k_scale is not None or v_scale is not None:
         raise ValueError("a float16 cache has no scales")
-    return _CACHE.pack(int8, k_cache.data_ptr(), v_cache.data_ptr(), ks, vs, pages, heads,
+    return _CACHE.pack(2 if fp4 else int8, k_cache.data_ptr(), v_cache.data_ptr(), ks, vs, pages, heads,
                        size, dim,
                        0 if k_cache.is_contiguous() else _page_stride(k_cache, "k_cache"),
                        0 if v_cache.is_contiguous() else _page_stride(v_cache, "v_cache"),
@@ -161,6 +189,26 @@ def _batch(page_table, kv_lens, cu_q, tokens: int, dev: int):
         pass
     raise ValueError("page_table [sequences, width], kv_lens [sequences] and cu_q [sequences + 1] "
                      f"must be contiguous int32 tensors on GPU {dev}")
+
+
+def _bounds(bounds, scale, page_size: int, dev: int):
+    """The packed bounds, their kv heads and head_dim."""
+    if not isinstance(bounds, torch.Tensor) or bounds.get_device() != dev or \
+            bounds.dtype is not torch.int8 or bounds.dim() != 4 or bounds.shape[2] != 2:
+        raise ValueError(f"bounds must be int8 [pages, kv_heads, 2, head_dim] on GPU {dev}")
+    if not isinstance(scale, torch.Tensor) or scale.get_device() != dev or \
+            scale.dtype is not torch.float32 or scale.shape != bounds.shape[:2]:
+        raise ValueError(f"bounds_scale must be float32 [pages, kv_heads] on GPU {dev}")
+    pages, heads, _, dim = bounds.shape
+    return _BOUNDS.pack(bounds.data_ptr(), scale.data_ptr(), pages, heads, page_size, dim,
+                        _page_stride(bounds, "bounds"),
+                        _page_stride(scale, "bounds_scale")), heads, dim
+
+
+def _whole(x, what: str, least: int) -> int:
+    if not isinstance(x, int) or x < least:
+        raise ValueError(f"{what} must be a whole number from {least} on, got {x!r}")
+    return min(x, 1 << 62)
 
 
 def _call(fn, where: str, dev: int, *args) -> None:
@@ -267,4 +315,99 @@ def paged_attention(q, k_cache, v_cache, page_table, kv_lens, cu_q, scale=None, 
     _call(load().hypno_hip_paged_attention_dev, "paged_attention", dev, out.data_ptr(),
           q.data_ptr(), q_stride, heads, cache, _batch(page_table, kv_lens, cu_q, tokens, dev),
           scale, window, max_kv_len)
+    return out
+
+
+def key_bounds(k_cache, bounds, bounds_scale, page_table, kv_lens, cu_q, k_scale=None):
+    """Computes the bounds (see above) of every page that holds a new token of the batch,
+    from all of the page's tokens below kv_lens; other pages' are left alone.  Called
+    after append_kv; with cu_q counting all tokens of a sequence, for all of its pages.
+    include/hypno_hip.h has the codes."""
+    if _args is None:
+        _torch()
+    done = _args.key_bounds(k_cache, bounds, bounds_scale, page_table, kv_lens, cu_q, k_scale)
+    if done is not NotImplemented:
+        return _done(done, "key_bounds")
+    if not isinstance(k_cache, torch.Tensor) or not k_cache.is_cuda:
+        raise ValueError("k_cache must be a GPU tensor")
+    dev = k_cache.get_device()
+    cache, heads, dim = _cache(k_cache, k_cache, k_scale, k_scale, dev)
+    packed, bh, bd = _bounds(bounds, bounds_scale, k_cache.shape[2], dev)
+    if bh != heads or bd != dim or bounds.shape[0] != k_cache.shape[0]:
+        raise ValueError(f"bounds of {list(bounds.shape)} for a cache of {k_cache.shape[0]} pages, "
+                         f"{heads} kv heads of {dim}")
+    _call(load().hypno_hip_key_bounds_dev, "key_bounds", dev, packed, cache,
+          _batch(page_table, kv_lens, cu_q, _ANY, dev))
+
+
+def select_pages(q, bounds, bounds_scale, page_size: int, page_table, kv_lens, cu_q, count: int,
+                 first: int = 1, last: int = 1, max_kv_len=None, out=None):
+    """The pages that each token is to read for each kv head: int32 [tokens, kv_heads,
+    count] (a new tensor, or the contiguous `out`), numbers of the sequence's pages,
+    ascending, -1 behind them.  The sequence's first `first` pages and the last `last` up to
+    the token's own are always among them, then those with the largest score: the most
+    that q . k can be for a key within the page's bounds, in 8-bit codes, the largest over
+    the kv head's query heads; the lower page first among equal ones.  max_kv_len: an upper
+    bound of kv_lens, if the host knows one (default: what page_table has room for, which
+    may be 32768 pages at most); pages past it have no score."""
+    if _args is None:
+        _torch()
+    done = _args.select_pages(q, bounds, bounds_scale, page_size, page_table, kv_lens, cu_q, count,
+                              first, last, max_kv_len, out)
+    if done is not NotImplemented:
+        return _done(done, "select_pages")
+    tokens, heads, dim, q_stride, dev = _rows(q, "q")
+    packed, kv_heads, bd = _bounds(bounds, bounds_scale, _whole(page_size, "page_size", 1), dev)
+    if bd != dim or not kv_heads or heads % kv_heads:
+        raise ValueError(f"q is {list(q.shape)} for bounds of {kv_heads} kv heads of {bd}")
+    count, first, last = _whole(count, "count", 1), _whole(first, "first", 0), \
+        _whole(last, "last", 1)
+    if first + last > count or count > 1024:
+        raise ValueError(f"count {count} is above 1024, or below first {first} and last {last}")
+    most = 0 if max_kv_len is None else _whole(max_kv_len, "max_kv_len", 0)
+    shape = (tokens, kv_heads, count)
+    if out is None:
+        out = torch.empty(shape, dtype=torch.int32, device=q.device)
+    elif not isinstance(out, torch.Tensor) or out.get_device() != dev or \
+            out.dtype is not torch.int32 or out.shape != shape or not out.is_contiguous():
+        raise ValueError(f"out must be a contiguous int32 {list(shape)} on GPU {dev}")
+    _call(load().hypno_hip_select_pages_dev, "select_pages", dev, out.data_ptr(), count, first,
+          last, q.data_ptr(), q_stride, heads, packed,
+          _batch(page_table, kv_lens, cu_q, tokens, dev), most)
+    return out
+
+
+def selected_attention(q, k_cache, v_cache, selected, page_table, kv_lens, cu_q, scale=None,
+                       k_scale=None, v_scale=None, out=None):
+    """paged_attention over the positions up to a token's own that are in its selected
+    pages: `selected` is what select_pages gives, or any contiguous int32 [tokens, kv_heads,
+    count].  Numbers below 0 or past the token's own page are passed over, a page that is
+    named twice counts twice; a token without any gets zeros.  Pages of 16 tokens at
+    least."""
+    if _args is None:
+        _torch()
+    done = _args.selected_attention(q, k_cache, v_cache, selected, page_table, kv_lens, cu_q,
+                                    scale, k_scale, v_scale, out)
+    if done is not NotImplemented:
+        return _done(done, "selected_attention")
+    tokens, heads, dim, q_stride, dev = _rows(q, "q")
+    cache, kv_heads, cd = _cache(k_cache, v_cache, k_scale, v_scale, dev)
+    if cd != dim or not kv_heads or heads % kv_heads:
+        raise ValueError(f"q is {list(q.shape)} for a cache of {kv_heads} kv heads of {cd}")
+    if not isinstance(selected, torch.Tensor) or selected.get_device() != dev or \
+            selected.dtype is not torch.int32 or selected.dim() != 3 or \
+            selected.shape[:2] != (tokens, kv_heads) or not selected.is_contiguous() or \
+            not 0 < selected.shape[2] <= 1024:
+        raise ValueError(f"selected must be a contiguous int32 [{tokens}, {kv_heads}, 1 to 1024] on "
+                         f"GPU {dev}")
+    if scale is None:
+        scale = 1.0 / math.sqrt(dim)
+    if out is None:
+        out = _empty(q)
+    elif not isinstance(out, torch.Tensor) or out.get_device() != dev or \
+            out.dtype is not torch.float32 or out.shape != q.shape or not out.is_contiguous():
+        raise ValueError(f"out must be a contiguous float32 {list(q.shape)} on GPU {dev}")
+    _call(load().hypno_hip_selected_attention_dev, "selected_attention", dev, out.data_ptr(),
+          q.data_ptr(), q_stride, heads, cache, _batch(page_table, kv_lens, cu_q, tokens, dev),
+          scale, selected.data_ptr(), selected.shape[2])
     return out

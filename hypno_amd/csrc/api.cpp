@@ -758,11 +758,24 @@ int scratch_of_current_device(FixedScratch* out) {
 
 constexpr size_t kMaxInt = 0x7FFFFFFF;
 
+// Elements (4-bit: bytes) of a page of k or v.
+size_t kv_page_elems(const hypno_hip_kv_cache& c) {
+  return c.kv_heads * c.page_size * (c.dtype == HYPNO_HIP_KV_FP4 ? c.head_dim / 2 : c.head_dim);
+}
+
 // Checks a cache and a batch and turns them into the kernels' form.
+// (`keys`: only k and k_scale are used.)
 int kv_args(const char* what, const hypno_hip_kv_cache* c, const hypno_hip_kv_batch* b,
-            KvCache* kc, KvBatch* kb) {
+            KvCache* kc, KvBatch* kb, bool keys = false) {
+  hypno_hip_kv_cache only;
+  if (c && keys) {
+    only = *c;
+    only.v = c->k, only.v_scale = c->k_scale;
+    only.v_page_stride = c->k_page_stride, only.v_scale_page_stride = c->k_scale_page_stride;
+    c = &only;
+  }
   if (!c || !b) return fail(HYPNO_HIP_EINVAL, "%s: NULL cache or batch", what);
-  if (c->dtype != HYPNO_HIP_KV_FP16 && c->dtype != HYPNO_HIP_KV_INT8)
+  if (c->dtype > HYPNO_HIP_KV_FP4)
     return fail(HYPNO_HIP_EINVAL, "%s: unknown cache dtype %u", what, c->dtype);
   if (c->head_dim == 0 || c->head_dim % 8 || c->head_dim > 256)
     return fail(HYPNO_HIP_EINVAL, "%s: head_dim %zu is no multiple of 8 up to 256", what,
@@ -770,27 +783,38 @@ int kv_args(const char* what, const hypno_hip_kv_cache* c, const hypno_hip_kv_ba
   if (c->page_size == 0 || (c->page_size & (c->page_size - 1)) || c->page_size > 65536)
     return fail(HYPNO_HIP_EINVAL, "%s: page_size %zu is no power of two up to 65536", what,
                 c->page_size);
+  const bool i8 = c->dtype == HYPNO_HIP_KV_INT8, fp4 = c->dtype == HYPNO_HIP_KV_FP4;
+  if (fp4 && (c->head_dim % kFp4Group || c->page_size < 16))
+    return fail(HYPNO_HIP_EINVAL, "%s: a 4-bit cache has a head_dim of whole groups of 32 and "
+                "pages of 16 tokens at least", what);
   if (c->kv_heads == 0 || c->kv_heads > 65535 || c->pages > kMaxInt)
     return fail(HYPNO_HIP_EINVAL, "%s: kv_heads or pages out of range", what);
   if (b->batch > kMaxInt / 2 || b->tokens > kMaxInt || b->table_width > kMaxInt ||
       mul_overflows(b->batch, b->table_width) || b->table_width * c->page_size > kMaxInt)
     return fail(HYPNO_HIP_EINVAL, "%s: batch, tokens or table_width out of range", what);
-  const bool i8 = c->dtype == HYPNO_HIP_KV_INT8;
   if (b->tokens && b->batch &&
       (!b->cu_q || !b->kv_lens || (b->table_width && !b->page_table) ||
-       (c->pages && (!c->k || !c->v || (i8 && (!c->k_scale || !c->v_scale))))))
+       (c->pages && (!c->k || !c->v || ((i8 || fp4) && (!c->k_scale || !c->v_scale))))))
     return fail(HYPNO_HIP_EINVAL, "%s: NULL pointer", what);
   if (((uintptr_t)c->k | (uintptr_t)c->v) & 15)
     return fail(HYPNO_HIP_EINVAL, "%s: k and v of the cache must be 16-byte aligned", what);
-  const size_t page = c->kv_heads * c->page_size * c->head_dim, sp = c->kv_heads * c->page_size;
-  *kc = KvCache{(int)c->dtype, c->k, c->v, c->k_scale, c->v_scale,
+  if (fp4 && (((uintptr_t)c->k_scale | (uintptr_t)c->v_scale) & 15))
+    return fail(HYPNO_HIP_EINVAL, "%s: a 4-bit cache's scales must be 16-byte aligned", what);
+  const size_t tokens = c->kv_heads * c->page_size, page = kv_page_elems(*c),
+               sp = fp4 ? tokens * (c->head_dim / kFp4Group) : tokens;
+  *kc = KvCache{(int)c->dtype, c->k, c->v, (float*)c->k_scale, (float*)c->v_scale,
                 c->k_page_stride ? c->k_page_stride : page,
                 c->v_page_stride ? c->v_page_stride : page,
                 c->k_scale_page_stride ? c->k_scale_page_stride : sp,
                 c->v_scale_page_stride ? c->v_scale_page_stride : sp,
                 (int)c->pages, (int)c->kv_heads, __builtin_ctzll(c->page_size), (int)c->head_dim};
-  if (kc->k_page < page || kc->v_page < page || (i8 && (kc->ks_page < sp || kc->vs_page < sp)))
+  if (kc->k_page < page || kc->v_page < page ||
+      ((i8 || fp4) && (kc->ks_page < sp || kc->vs_page < sp)))
     return fail(HYPNO_HIP_EINVAL, "%s: a page stride is smaller than a page", what);
+  if (fp4 && (c->k_page_stride % 16 || c->v_page_stride % 16 || c->k_scale_page_stride % 8 ||
+              c->v_scale_page_stride % 8))
+    return fail(HYPNO_HIP_EINVAL, "%s: page strides of a 4-bit cache must be multiples of 16, "
+                "of its scales of 8", what);
   if (c->k_page_stride % 8 || c->v_page_stride % 8)
     return fail(HYPNO_HIP_EINVAL, "%s: page strides of k and v must be multiples of 8", what);
   if (mul_overflows(c->pages, 4 * std::max(std::max(kc->k_page, kc->v_page),
@@ -803,17 +827,49 @@ int kv_args(const char* what, const hypno_hip_kv_cache* c, const hypno_hip_kv_ba
 
 // [p, p + bytes) shares memory with the cache or the batch's arrays.
 bool overlaps_kv(const void* p, size_t bytes, const KvCache& c, const KvBatch& b) {
-  const size_t item = c.dtype == kKvFp16 ? 2 : 1, sp = (size_t)c.kv_heads << c.page_shift;
+  const bool fp4 = c.dtype == kKvFp4;
+  const size_t item = c.dtype == kKvFp16 ? 2 : 1, tokens = (size_t)c.kv_heads << c.page_shift;
+  const size_t sp = fp4 ? tokens * (c.head_dim / kFp4Group) : tokens, si = fp4 ? 2 : 4;
   auto span = [&](size_t stride, size_t page, size_t size) {
     return c.pages ? ((c.pages - 1) * stride + page) * size : 0;
   };
-  const size_t page = sp * c.head_dim, n = b.batch;
+  const size_t page = tokens * (fp4 ? c.head_dim / 2 : c.head_dim), n = b.batch;
   return overlaps(p, bytes, c.k, span(c.k_page, page, item)) ||
          overlaps(p, bytes, c.v, span(c.v_page, page, item)) ||
-         overlaps(p, bytes, c.k_scale, span(c.ks_page, sp, 4)) ||
-         overlaps(p, bytes, c.v_scale, span(c.vs_page, sp, 4)) ||
+         overlaps(p, bytes, c.k_scale, span(c.ks_page, sp, si)) ||
+         overlaps(p, bytes, c.v_scale, span(c.vs_page, sp, si)) ||
          overlaps(p, bytes, b.cu_q, (n + 1) * 4) || overlaps(p, bytes, b.kv_lens, n * 4) ||
          overlaps(p, bytes, b.page_table, n * b.width * 4);
+}
+
+// Checks bounds beside a batch (see kv_args) and turns them into the kernels' form.
+int bounds_args(const char* what, const hypno_hip_key_bounds* o, const hypno_hip_kv_batch* b,
+                KeyBounds* ko, KvBatch* kb) {
+  if (!o) return fail(HYPNO_HIP_EINVAL, "%s: NULL bounds", what);
+  // (a cache of 8-bit keys, two a token, has the same sizes and strides)
+  hypno_hip_kv_cache c = {HYPNO_HIP_KV_INT8, o->codes, o->codes, o->scale, o->scale, o->pages,
+                          o->kv_heads, o->page_size, o->head_dim, 0, 0, 0, 0};
+  KvCache kc;
+  const int st = kv_args(what, &c, b, &kc, kb);
+  if (st) return st;
+  const size_t page = o->kv_heads * 2 * o->head_dim;
+  *ko = KeyBounds{o->codes, o->scale, o->page_stride ? o->page_stride : page,
+                  o->scale_page_stride ? o->scale_page_stride : o->kv_heads, (int)o->pages,
+                  (int)o->kv_heads, kc.page_shift, (int)o->head_dim};
+  if (ko->page < page || ko->s_page < o->kv_heads || o->page_stride % 16)
+    return fail(HYPNO_HIP_EINVAL, "%s: a page stride of the bounds is smaller than a page or no "
+                "multiple of 16", what);
+  if (mul_overflows(o->pages, 4 * std::max(ko->page, ko->s_page)))
+    return fail(HYPNO_HIP_EINVAL, "%s: size of the bounds overflows", what);
+  return HYPNO_HIP_OK;
+}
+
+// [p, p + bytes) shares memory with the bounds.
+bool overlaps_bounds(const void* p, size_t bytes, const KeyBounds& o) {
+  const size_t n = o.pages ? o.pages - 1 : 0, any = o.pages != 0;
+  return overlaps(p, bytes, o.codes,
+                  any * (n * o.page + (size_t)o.kv_heads * 2 * o.head_dim)) ||
+         overlaps(p, bytes, o.scale, any * (n * o.s_page + o.kv_heads) * 4);
 }
 
 // Rows of wa floats from a and of wb from b share memory; parts of one fused
@@ -1460,6 +1516,108 @@ int hypno_hip_paged_attention_dev(float* out, const float* q, size_t q_stride, s
   hipError_t e = launch_paged_attention(p, out, q, q_stride, (int)heads, c, b, scale, win, ws.p,
                                         (hipStream_t)stream);
   return e == hipSuccess ? HYPNO_HIP_OK : hip_fail(e, "paged_attention launch");
+}
+
+int hypno_hip_key_bounds_dev(const hypno_hip_key_bounds* bounds, const hypno_hip_kv_cache* cache,
+                             const hypno_hip_kv_batch* batch, void* stream) {
+  KvCache c;
+  KvBatch b;
+  KeyBounds o;
+  int st = kv_args("key_bounds", cache, batch, &c, &b, true);
+  if (st) return st;
+  if ((st = bounds_args("key_bounds", bounds, batch, &o, &b))) return st;
+  if (o.pages != c.pages || o.kv_heads != c.kv_heads || o.page_shift != c.page_shift ||
+      o.head_dim != c.head_dim)
+    return fail(HYPNO_HIP_EINVAL, "key_bounds: the bounds are of another cache's size");
+  if (batch->tokens == 0 || batch->batch == 0 || cache->pages == 0) return HYPNO_HIP_OK;
+  const size_t codes = ((size_t)(o.pages - 1) * o.page + (size_t)o.kv_heads * 2 * o.head_dim);
+  const size_t scales = ((size_t)(o.pages - 1) * o.s_page + o.kv_heads) * 4;
+  if (overlaps_kv(o.codes, codes, c, b) || overlaps_kv(o.scale, scales, c, b) ||
+      overlaps(o.codes, codes, o.scale, scales))
+    return fail(HYPNO_HIP_EINVAL, "key_bounds: the bounds overlap another buffer");
+  DeviceState* ds = nullptr;
+  {
+    std::lock_guard<std::mutex> g(g_mu);
+    st = device_state(&ds);
+    if (st) return st;
+  }
+  hipError_t e = launch_key_bounds(o, c, b, ds->cus, (hipStream_t)stream);
+  return e == hipSuccess ? HYPNO_HIP_OK : hip_fail(e, "key_bounds launch");
+}
+
+int hypno_hip_select_pages_dev(int32_t* selected, size_t count, size_t first, size_t last,
+                               const float* q, size_t q_stride, size_t heads,
+                               const hypno_hip_key_bounds* bounds,
+                               const hypno_hip_kv_batch* batch, size_t max_kv_len, void* stream) {
+  KvBatch b;
+  KeyBounds o;
+  int st = bounds_args("select_pages", bounds, batch, &o, &b);
+  if (st) return st;
+  const size_t T = batch->tokens, D = bounds->head_dim, KV = bounds->kv_heads;
+  if (heads == 0 || heads % KV || heads > 65535)
+    return fail(HYPNO_HIP_EINVAL, "select_pages: %zu heads are no multiple of %zu kv heads", heads,
+                KV);
+  if (T * heads > kMaxInt)
+    return fail(HYPNO_HIP_EINVAL, "select_pages: tokens * heads out of range");
+  if (count == 0 || count > kMaxSelected || last == 0 || first > count || last > count - first)
+    return fail(HYPNO_HIP_EINVAL, "select_pages: count %zu is not in 1 to %d, or below first %zu "
+                "and last %zu (at least 1)", count, kMaxSelected, first, last);
+  const size_t room = batch->table_width * bounds->page_size;
+  const size_t kv = max_kv_len ? std::min(max_kv_len, room) : room;
+  const size_t pages = (kv + bounds->page_size - 1) / bounds->page_size;
+  if (pages > kMaxScored)
+    return fail(HYPNO_HIP_EINVAL, "select_pages: sequences of up to %zu pages, above %d", pages,
+                kMaxScored);
+  size_t qb = 0;
+  if ((st = rows_bytes("select_pages", T, heads * D, q_stride, &qb))) return st;
+  if (T == 0 || batch->batch == 0) return HYPNO_HIP_OK;
+  if (!selected || !q) return fail(HYPNO_HIP_EINVAL, "select_pages: NULL pointer");
+  const size_t ob = T * KV * count * 4, n = batch->batch;
+  if (overlaps(selected, ob, q, qb) || overlaps_bounds(selected, ob, o) ||
+      overlaps(selected, ob, b.cu_q, (n + 1) * 4) || overlaps(selected, ob, b.kv_lens, n * 4) ||
+      overlaps(selected, ob, b.page_table, n * batch->table_width * 4))
+    return fail(HYPNO_HIP_EINVAL, "select_pages: selected overlaps an input");
+  DeviceState* ds = nullptr;
+  {
+    std::lock_guard<std::mutex> g(g_mu);
+    st = device_state(&ds);
+    if (st) return st;
+  }
+  hipError_t e = launch_select_pages(selected, (int)count, (int)first, (int)last, q, q_stride,
+                                     (int)heads, o, b, (int)pages, ds->cus, (hipStream_t)stream);
+  return e == hipSuccess ? HYPNO_HIP_OK : hip_fail(e, "select_pages launch");
+}
+
+int hypno_hip_selected_attention_dev(float* out, const float* q, size_t q_stride, size_t heads,
+                                     const hypno_hip_kv_cache* cache,
+                                     const hypno_hip_kv_batch* batch, float scale,
+                                     const int32_t* selected, size_t count, void* stream) {
+  KvCache c;
+  KvBatch b;
+  int st = kv_args("selected_attention", cache, batch, &c, &b);
+  if (st) return st;
+  const size_t T = batch->tokens, D = cache->head_dim, KV = cache->kv_heads;
+  if (heads == 0 || heads % KV || heads > 65535)
+    return fail(HYPNO_HIP_EINVAL, "selected_attention: %zu heads are no multiple of %zu kv heads",
+                heads, KV);
+  if (T * heads > kMaxInt)
+    return fail(HYPNO_HIP_EINVAL, "selected_attention: tokens * heads out of range");
+  if (cache->page_size < 16)
+    return fail(HYPNO_HIP_EINVAL, "selected_attention: pages of fewer than 16 tokens");
+  if (count == 0 || count > kMaxSelected)
+    return fail(HYPNO_HIP_EINVAL, "selected_attention: count %zu is not in 1 to %d", count,
+                kMaxSelected);
+  size_t qb = 0, ob = 0;
+  if ((st = rows_bytes("selected_attention", T, heads * D, q_stride, &qb))) return st;
+  if ((st = rows_bytes("selected_attention", T, heads * D, heads * D, &ob))) return st;
+  if (T == 0 || batch->batch == 0) return HYPNO_HIP_OK;
+  if (!out || !q || !selected) return fail(HYPNO_HIP_EINVAL, "selected_attention: NULL pointer");
+  if (overlaps(out, ob, q, qb) || overlaps(out, ob, selected, T * KV * count * 4) ||
+      overlaps_kv(out, ob, c, b))
+    return fail(HYPNO_HIP_EINVAL, "selected_attention: out overlaps an input");
+  hipError_t e = launch_selected_attention(out, q, q_stride, (int)heads, c, b, scale, selected,
+                                           (int)count, (hipStream_t)stream);
+  return e == hipSuccess ? HYPNO_HIP_OK : hip_fail(e, "selected_attention launch");
 }
 
 int hypno_hip_stream_synchronize(void* stream) {

@@ -136,7 +136,7 @@ AttnPlan attn_plan(const KvCache& c, const KvBatch& b, int heads, int window, in
   // beside three, 8-bit, 113 / 102.)
   const bool only_few = b.tokens <= b.batch || (b.batch == 1 && rows <= 16);
   const bool only_tile = !only_few && (b.batch <= 8 || G > 16);
-  p.few = only_few ? 0x7FFFFFFF : only_tile ? 0 : kFewRows;
+  p.few = c.dtype == kKvFp4 ? 0 : only_few ? 0x7FFFFFFF : only_tile ? 0 : kFewRows;
   const int64_t room = (int64_t)b.width << c.page_shift;
   const int64_t kv = std::max<int64_t>(1, max_kv ? std::min(max_kv, room) : room);
   // Up to 1024 positions (2048 where sequences and heads alone fill the chip) a

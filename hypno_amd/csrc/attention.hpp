@@ -109,8 +109,10 @@ __device__ __forceinline__ size_t few_part(const AttnArgs& a, const Seq& s, int 
   return a.by_seq ? ((size_t)s.b * a.c.kv_heads + g) * kFewRows + r : row;
 }
 
-// One row by a wave, plainly, sums in 64 bits.
-__device__ __forceinline__ void attn_row(const AttnArgs& a, const Seq& sq, int i, int h) {
+// One row by a wave, plainly, sums in 64 bits: over all positions that it sees, or those
+// in its `count` pages of `list`.
+__device__ __forceinline__ void attn_row(const AttnArgs& a, const Seq& sq, int i, int h,
+                                         const int* list = nullptr, int count = 0) {
   const int lane = threadIdx.x & 63, t = sq.first + i;
   const int D = a.c.head_dim, g = h / a.group;
   const int pos = sq.kv - sq.n + i;
@@ -121,11 +123,12 @@ __device__ __forceinline__ void attn_row(const AttnArgs& a, const Seq& sq, int i
     const int e = lane + 64 * j;
     q[j] = e < D ? a.q[(size_t)t * a.q_stride + (size_t)h * D + e] * a.scale : 0.0f;
   }
-  for (int p = first_seen(a, sq, i); p <= pos && !past; p++) {
+  auto add = [&](int p) __attribute__((always_inline)) {
     const int page = a.b.page_table[(size_t)sq.b * a.b.width + (p >> a.c.page_shift)];
     const bool there = page >= 0 && page < a.c.pages;
     const size_t tok = ((size_t)g << a.c.page_shift) + (p & ((1 << a.c.page_shift) - 1));
-    const size_t ki = (size_t)page * a.c.k_page + tok * D, vi = (size_t)page * a.c.v_page + tok * D;
+    const size_t td = a.c.dtype == kKvFp4 ? tok * D / 2 : tok * D;
+    const size_t ki = (size_t)page * a.c.k_page + td, vi = (size_t)page * a.c.v_page + td;
     float s = 0.0f, v[4] = {};
     if (there) {
       for (int j = 0; j < 4; j++) {
@@ -134,6 +137,15 @@ __device__ __forceinline__ void attn_row(const AttnArgs& a, const Seq& sq, int i
         if (a.c.dtype == kKvFp16) {
           s = fmaf(q[j], (float)((const _Float16*)a.c.k)[ki + e], s);
           v[j] = (float)((const _Float16*)a.c.v)[vi + e];
+        } else if (a.c.dtype == kKvFp4) {
+          const size_t at = ((size_t)(g * (D / kFp4Group) + e / kFp4Group) << a.c.page_shift) +
+                            (p & ((1 << a.c.page_shift) - 1));
+          const uint32_t kc = ((const uint8_t*)a.c.k)[ki + e / 2] >> e % 2 * 4;
+          const uint32_t vc = ((const uint8_t*)a.c.v)[vi + e / 2] >> e % 2 * 4;
+          const _Float16 ks = ((const _Float16*)a.c.k_scale)[(size_t)page * a.c.ks_page + at];
+          const _Float16 vs = ((const _Float16*)a.c.v_scale)[(size_t)page * a.c.vs_page + at];
+          s = fmaf(q[j], (float)(_Float16)(fp4_value(kc) * ks), s);
+          v[j] = (float)(_Float16)(fp4_value(vc) * vs);
         } else {
           s = fmaf(q[j], (float)((const int8_t*)a.c.k)[ki + e], s);
           v[j] = (float)((const int8_t*)a.c.v)[vi + e] *
@@ -151,6 +163,17 @@ __device__ __forceinline__ void attn_row(const AttnArgs& a, const Seq& sq, int i
     m = mn;
     l = l * r + w;
     for (int j = 0; j < 4; j++) o[j] = o[j] * r + (double)w * v[j];
+  };
+  if (list) {
+    for (int e = 0; e < count && !past; e++) {
+      const int at = list[e];
+      if (at < 0 || at > pos >> a.c.page_shift) continue;
+      const int64_t p0 = (int64_t)at << a.c.page_shift;
+      const int end = (int)min((int64_t)pos + 1, p0 + (1 << a.c.page_shift));
+      for (int p = (int)p0; p < end; p++) add(p);
+    }
+  } else {
+    for (int p = first_seen(a, sq, i); p <= pos && !past; p++) add(p);
   }
   for (int j = 0; j < 4; j++) {
     const int e = lane + 64 * j;
@@ -528,6 +551,20 @@ struct Rows {
     return NQ * t + 4 * NG * (i / 4) + 4 * ((threadIdx.x & 63) / NQ) + i % 4;
   }
 };
+
+// Eight 4-bit codes times their scale (twice in a register) -> eight fp16, each rounded
+// once.
+__device__ __forceinline__ u32x4 fp4_to_f16(uint32_t x, half2v scale) {
+  u32x4 r;
+  const half2v v[4] = {
+      __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(x, 1.0f, 0),
+      __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(x, 1.0f, 1),
+      __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(x, 1.0f, 2),
+      __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(x, 1.0f, 3)};
+#pragma unroll
+  for (int i = 0; i < 4; i++) r[i] = __builtin_bit_cast(uint32_t, (half2v)(v[i] * scale));
+  return r;
+}
 
 // Launchers of the kernels' files.
 hipError_t launch_attn_tile(const AttnArgs& a, hipStream_t s);

@@ -1,5 +1,5 @@
-// The tensors of append_kv and paged_attention (attention.py) to the structs and
-// arguments of include/hypno_hip.h.  What the Python functions check one attribute at a
+// The tensors of append_kv, paged_attention, key_bounds, select_pages and
+// selected_attention (attention.py) to the structs and arguments of include/hypno_hip.h.  What the Python functions check one attribute at a
 // time (5 to 7 us a call, more than a token's kernel takes) is read from the tensors
 // here, 1 to 2 us.  Only calls that are right are made: for any other the answer is
 // NotImplemented, and the Python functions say what is wrong with it.
@@ -14,6 +14,9 @@ namespace {
 
 decltype(&hypno_hip_append_kv_dev) g_append = nullptr;
 decltype(&hypno_hip_paged_attention_dev) g_attend = nullptr;
+decltype(&hypno_hip_key_bounds_dev) g_bounds = nullptr;
+decltype(&hypno_hip_select_pages_dev) g_select = nullptr;
+decltype(&hypno_hip_selected_attention_dev) g_selected = nullptr;
 PyObject* g_device = nullptr;  // current device, and the raw stream of one
 PyObject* g_stream = nullptr;
 
@@ -60,21 +63,29 @@ int64_t page_stride(const at::Tensor& t) {
 bool cache(PyObject* k, PyObject* v, PyObject* ks, PyObject* vs, int dev, hypno_hip_kv_cache& c) {
   if (!THPVariable_Check(k)) return false;
   const auto type = THPVariable_Unpack(k).scalar_type();
-  if (type != at::kHalf && type != at::kChar) return false;
+  const bool fp4 = type == at::kByte;
+  if (type != at::kHalf && type != at::kChar && !fp4) return false;
   const at::Tensor *kt = tensor(k, dev, type, 4), *vt = tensor(v, dev, type, 4);
   if (!kt || !vt || kt->sizes() != vt->sizes()) return false;
   const int64_t kp = page_stride(*kt), vp = page_stride(*vt);
   if (kp < 0 || vp < 0) return false;
   const auto s = kt->sizes();
-  c = hypno_hip_kv_cache{type == at::kChar ? HYPNO_HIP_KV_INT8 : HYPNO_HIP_KV_FP16,
+  const int64_t dim = fp4 ? 2 * s[3] : s[3];
+  c = hypno_hip_kv_cache{fp4                 ? HYPNO_HIP_KV_FP4
+                         : type == at::kChar ? HYPNO_HIP_KV_INT8
+                                             : HYPNO_HIP_KV_FP16,
                          kt->data_ptr(), vt->data_ptr(), nullptr, nullptr, (size_t)s[0],
-                         (size_t)s[1], (size_t)s[2], (size_t)s[3], (size_t)kp, (size_t)vp, 0, 0};
+                         (size_t)s[1], (size_t)s[2], (size_t)dim, (size_t)kp, (size_t)vp, 0, 0};
   if (type == at::kHalf) return ks == Py_None && vs == Py_None;
-  const at::Tensor *kst = tensor(ks, dev, at::kFloat, 3), *vst = tensor(vs, dev, at::kFloat, 3);
-  if (!kst || !vst || kst->sizes() != s.slice(0, 3) || vst->sizes() != s.slice(0, 3)) return false;
+  const at::ScalarType scales = fp4 ? at::kHalf : at::kFloat;
+  const at::Tensor *kst = tensor(ks, dev, scales, fp4 ? 4 : 3),
+                   *vst = tensor(vs, dev, scales, fp4 ? 4 : 3);
+  const int64_t groups[] = {s[0], s[1], dim / 32, s[2]};
+  const at::IntArrayRef want = fp4 ? at::IntArrayRef(groups, 4) : s.slice(0, 3);
+  if (!kst || !vst || kst->sizes() != want || vst->sizes() != want) return false;
   const int64_t ksp = page_stride(*kst), vsp = page_stride(*vst);
   if (ksp < 0 || vsp < 0) return false;
-  c.k_scale = (float*)kst->data_ptr(), c.v_scale = (float*)vst->data_ptr();
+  c.k_scale = kst->data_ptr(), c.v_scale = vst->data_ptr();
   c.k_scale_page_stride = (size_t)ksp, c.v_scale_page_stride = (size_t)vsp;
   return true;
 }
@@ -91,6 +102,34 @@ bool batch(PyObject* table, PyObject* lens, PyObject* cu, int64_t tokens, int de
                          (const int32_t*)t->data_ptr(), (size_t)n, (size_t)t->size(1),
                          (size_t)tokens};
   return true;
+}
+
+// (page_size and the cache's other sizes: the bounds' own)
+bool key_bounds_of(PyObject* codes, PyObject* scale, int64_t page_size, int dev,
+                   hypno_hip_key_bounds& o) {
+  const at::Tensor *c = tensor(codes, dev, at::kChar, 4), *s = tensor(scale, dev, at::kFloat, 2);
+  if (!c || !s || c->size(2) != 2 || s->sizes() != c->sizes().slice(0, 2)) return false;
+  const int64_t cp = page_stride(*c), sp = page_stride(*s);
+  if (cp < 0 || sp < 0) return false;
+  o = hypno_hip_key_bounds{(int8_t*)c->data_ptr(), (float*)s->data_ptr(), (size_t)c->size(0),
+                           (size_t)c->size(1), (size_t)page_size, (size_t)c->size(3), (size_t)cp,
+                           (size_t)sp};
+  return true;
+}
+
+// A Python int (or `none` for None) of `least` or more.
+bool whole(PyObject* x, long long least, long long& v, long long none = -1) {
+  if (x == Py_None && none >= 0) {
+    v = none;
+    return true;
+  }
+  if (!PyLong_Check(x)) return false;
+  v = PyLong_AsLongLong(x);
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    return false;
+  }
+  return v >= least;
 }
 
 // The stream that torch queues on, if `dev` is the current device.
@@ -222,24 +261,146 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   }
 }
 
-// bind(address of hypno_hip_append_kv_dev, of hypno_hip_paged_attention_dev, function of
-// the current device, function of a device's stream)
+// (k_cache, bounds, bounds_scale, page_table, kv_lens, cu_q, k_scale)
+PyObject* key_bounds(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 7 || !g_bounds) return other();
+  try {
+    if (!THPVariable_Check(a[0]) || !THPVariable_Unpack(a[0]).is_cuda()) return other();
+    const int dev = (int)THPVariable_Unpack(a[0]).get_device();
+    hypno_hip_kv_cache c;
+    hypno_hip_kv_batch b;
+    hypno_hip_key_bounds o;
+    if (!cache(a[0], a[0], a[6], a[6], dev, c) ||
+        !key_bounds_of(a[1], a[2], (int64_t)c.page_size, dev, o) || o.pages != c.pages ||
+        o.kv_heads != c.kv_heads || o.head_dim != c.head_dim ||
+        !batch(a[3], a[4], a[5], 0x7FFFFFFF, dev, b))
+      return other();
+    void* s = nullptr;
+    if (!stream_of(dev, &s)) return other();
+    int status;
+    Py_BEGIN_ALLOW_THREADS
+    status = g_bounds(&o, &c, &b, s);
+    Py_END_ALLOW_THREADS
+    if (status) return PyLong_FromLong(status);
+    Py_RETURN_NONE;
+  } catch (...) {
+    return other();
+  }
+}
+
+// (q, bounds, bounds_scale, page_size, page_table, kv_lens, cu_q, count, first, last,
+// max_kv_len, out)
+PyObject* select_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 12 || !g_select) return other();
+  try {
+    Rows q;
+    if (!rows(a[0], -1, q)) return other();
+    const int dev = (int)q.t->get_device();
+    long long size, count, first, last, most;
+    hypno_hip_kv_batch b;
+    hypno_hip_key_bounds o;
+    if (!whole(a[3], 1, size) || !whole(a[7], 1, count) || !whole(a[8], 0, first) ||
+        !whole(a[9], 1, last) || !whole(a[10], 0, most, 0) || count > 1024 || first > count ||
+        last > count - first || !key_bounds_of(a[1], a[2], size, dev, o) ||
+        !batch(a[4], a[5], a[6], q.n, dev, b) || (int64_t)o.head_dim != q.d || o.kv_heads == 0 ||
+        q.h % (int64_t)o.kv_heads)
+      return other();
+    const int64_t shape[] = {q.n, (int64_t)o.kv_heads, count};
+    at::Tensor made;
+    int32_t* op = nullptr;
+    if (a[11] == Py_None) {
+      made = at::empty(shape, q.t->options().dtype(at::kInt));
+      op = (int32_t*)made.data_ptr();
+    } else {
+      const at::Tensor* t = tensor(a[11], dev, at::kInt, 3);
+      if (!t || t->sizes() != at::IntArrayRef(shape, 3) || !t->is_contiguous()) return other();
+      op = (int32_t*)t->data_ptr();
+    }
+    void* s = nullptr;
+    if (!stream_of(dev, &s)) return other();
+    const float* qp = (const float*)q.t->data_ptr();
+    int status;
+    Py_BEGIN_ALLOW_THREADS
+    status = g_select(op, (size_t)count, (size_t)first, (size_t)last, qp, (size_t)q.stride,
+                      (size_t)q.h, &o, &b, (size_t)most, s);
+    Py_END_ALLOW_THREADS
+    return result(status, a[11], made);
+  } catch (...) {
+    return other();
+  }
+}
+
+// (q, k_cache, v_cache, selected, page_table, kv_lens, cu_q, scale, k_scale, v_scale, out)
+PyObject* selected_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 11 || !g_selected) return other();
+  try {
+    Rows q;
+    if (!rows(a[0], -1, q)) return other();
+    const int dev = (int)q.t->get_device();
+    hypno_hip_kv_cache c;
+    hypno_hip_kv_batch b;
+    if (!cache(a[1], a[2], a[8], a[9], dev, c) || !batch(a[4], a[5], a[6], q.n, dev, b) ||
+        (int64_t)c.head_dim != q.d || c.kv_heads == 0 || q.h % (int64_t)c.kv_heads)
+      return other();
+    const at::Tensor* sel = tensor(a[3], dev, at::kInt, 3);
+    if (!sel || !sel->is_contiguous() || sel->size(0) != q.n ||
+        sel->size(1) != (int64_t)c.kv_heads || sel->size(2) < 1 || sel->size(2) > 1024)
+      return other();
+    if (a[7] != Py_None && !PyFloat_Check(a[7])) return other();
+    const double scale = a[7] == Py_None ? 1.0 / std::sqrt((double)q.d) : PyFloat_AsDouble(a[7]);
+    at::Tensor made;
+    float* op = nullptr;
+    if (a[10] == Py_None) {
+      made = at::empty(q.t->sizes(), q.t->options());
+      op = (float*)made.data_ptr();
+    } else {
+      const at::Tensor* o = tensor(a[10], dev, at::kFloat, 3);
+      if (!o || o->sizes() != q.t->sizes() || !o->is_contiguous()) return other();
+      op = (float*)o->data_ptr();
+    }
+    void* s = nullptr;
+    if (!stream_of(dev, &s)) return other();
+    const float* qp = (const float*)q.t->data_ptr();
+    const int32_t* sp = (const int32_t*)sel->data_ptr();
+    int status;
+    Py_BEGIN_ALLOW_THREADS
+    status = g_selected(op, qp, (size_t)q.stride, (size_t)q.h, &c, &b, (float)scale, sp,
+                        (size_t)sel->size(2), s);
+    Py_END_ALLOW_THREADS
+    return result(status, a[10], made);
+  } catch (...) {
+    return other();
+  }
+}
+
+// bind(addresses of hypno_hip_append_kv_dev, _paged_attention_dev, _key_bounds_dev,
+// _select_pages_dev and _selected_attention_dev, function of the current device, function
+// of a device's stream)
 PyObject* bind(PyObject*, PyObject* args) {
-  unsigned long long append = 0, attend = 0;
+  unsigned long long append = 0, attend = 0, bounds = 0, select = 0, selected = 0;
   PyObject *device = nullptr, *stream = nullptr;
-  if (!PyArg_ParseTuple(args, "KKOO", &append, &attend, &device, &stream)) return nullptr;
+  if (!PyArg_ParseTuple(args, "KKKKKOO", &append, &attend, &bounds, &select, &selected, &device,
+                        &stream))
+    return nullptr;
   Py_INCREF(device);
   Py_INCREF(stream);
   Py_XSETREF(g_device, device);
   Py_XSETREF(g_stream, stream);
   g_append = reinterpret_cast<decltype(g_append)>((uintptr_t)append);
   g_attend = reinterpret_cast<decltype(g_attend)>((uintptr_t)attend);
+  g_bounds = reinterpret_cast<decltype(g_bounds)>((uintptr_t)bounds);
+  g_select = reinterpret_cast<decltype(g_select)>((uintptr_t)select);
+  g_selected = reinterpret_cast<decltype(g_selected)>((uintptr_t)selected);
   Py_RETURN_NONE;
 }
 
 PyMethodDef methods[] = {
     {"append_kv", (PyCFunction)(void (*)(void))append_kv, METH_FASTCALL, nullptr},
     {"paged_attention", (PyCFunction)(void (*)(void))paged_attention, METH_FASTCALL, nullptr},
+    {"key_bounds", (PyCFunction)(void (*)(void))key_bounds, METH_FASTCALL, nullptr},
+    {"select_pages", (PyCFunction)(void (*)(void))select_pages, METH_FASTCALL, nullptr},
+    {"selected_attention", (PyCFunction)(void (*)(void))selected_attention, METH_FASTCALL,
+     nullptr},
     {"bind", bind, METH_VARARGS, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 

@@ -33,6 +33,8 @@ struct Tile {
   static constexpr int kRows = 4 * NQ;
   static constexpr int kBytes = BK * DP * 2;          // K or V of one tile
   static constexpr int kN = BK * DP / 8 / 256;        // 16-byte pieces of it a thread
+  // 4-bit: groups of 32 codes, 16 bytes, of a wave's BK / 4 rows, and of them a lane.
+  static constexpr int kG = BK / 4 * DP / kFp4Group, kNg = (kG + 63) / 64;
   // K and V twice; 8-bit: their scales twice.
   static constexpr int kLds = 4 * kBytes + (kType == kKvInt8 ? 4 * BK * 4 : 0);
 };
@@ -70,7 +72,7 @@ __global__ void __launch_bounds__(256, 2) attn_tile_kernel(AttnArgs a) {
   }
 
   // This wave's rows: lane % NQ of it, and the positions that it sees.
-  typedef Rows<kType, NQ, DP, BK> R;
+  typedef Rows<kType == kKvInt8 ? kKvInt8 : kKvFp16, NQ, DP, BK> R;
   const int w0 = r0 + wave * NQ, row = w0 + lane % NQ;
   const bool live = row < rows;
   const int ti = min(row, rows - 1) / G, h = g * G + min(row, rows - 1) % G;
@@ -92,8 +94,11 @@ __global__ void __launch_bounds__(256, 2) attn_tile_kernel(AttnArgs a) {
   // (Rows past the end: the last row again, whose weights are 0.)
   constexpr int kMine = BK / 4;
   const int mask = (1 << a.c.page_shift) - 1, item = kType == kKvFp16 ? 2 : 1;
+  static_assert(kType != kKvFp4 || kOne, "4-bit pages have kRun positions or more");
   int id = 0, ids[T::kN];  // (with `ids`, id: of the lane's scale)
   uint2 kr[T::kN], vr[T::kN];   // 8-bit codes on their way
+  u32x4 kr4[T::kNg], vr4[T::kNg];  // 4-bit: codes and scales on their way
+  _Float16 ks4[T::kNg], vs4[T::kNg];
   float sr = 0.0f;
   const int srow = wave * kMine + lane % kMine;
   const bool sk = lane < kMine;
@@ -120,6 +125,30 @@ __global__ void __launch_bounds__(256, 2) attn_tile_kernel(AttnArgs a) {
   const float* const ksg = a.c.k_scale + ((size_t)g << a.c.page_shift);
   const float* const vsg = a.c.v_scale + ((size_t)g << a.c.page_shift);
   auto issue = [&](int p0, int buf) __attribute__((always_inline)) {
+    if constexpr (kType == kKvFp4) {
+      const int pg = __builtin_amdgcn_readfirstlane(page_of(a, id, bad)), B = D / kFp4Group;
+      const uint8_t* const kp =
+          (const uint8_t*)a.c.k + (size_t)pg * a.c.k_page + (((size_t)g << a.c.page_shift) * D >> 1);
+      const uint8_t* const vp =
+          (const uint8_t*)a.c.v + (size_t)pg * a.c.v_page + (((size_t)g << a.c.page_shift) * D >> 1);
+      const _Float16* const ksp = (const _Float16*)a.c.k_scale + (size_t)pg * a.c.ks_page +
+                                  ((size_t)(g * B) << a.c.page_shift);
+      const _Float16* const vsp = (const _Float16*)a.c.v_scale + (size_t)pg * a.c.vs_page +
+                                  ((size_t)(g * B) << a.c.page_shift);
+#pragma unroll
+      for (int i = 0; i < T::kNg; i++) {
+        // (lanes past the groups, and groups past D: the row's first)
+        const int j = min(i * 64 + lane, T::kG - 1), blk = j % (DP / kFp4Group);
+        const int tok = min(p0 + wave * kMine + j / (DP / kFp4Group), hi - 1) & mask;
+        const int at = blk < B ? blk : 0;
+        const uint32_t off = __umul24(tok, D / 2) + at * 16, so = (at << a.c.page_shift) + tok;
+        kr4[i] = load_global<u32x4>(kp + off);
+        vr4[i] = load_global<u32x4>(vp + off);
+        ks4[i] = load_global<_Float16>(ksp + so);
+        vs4[i] = load_global<_Float16>(vsp + so);
+      }
+      return;
+    }
     const int page = kType == kKvInt8 || kOne ? page_of(a, id, bad) : 0;
     uint32_t off[T::kN];
 #pragma unroll
@@ -162,7 +191,23 @@ __global__ void __launch_bounds__(256, 2) attn_tile_kernel(AttnArgs a) {
                                   : vsg + (size_t)page * a.c.vs_page) + tok);
     }
   };
-  auto store = [&](int buf) __attribute__((always_inline)) {  // 8-bit: what `issue` loaded
+  auto store = [&](int buf) __attribute__((always_inline)) {  // codes: what `issue` loaded
+    if constexpr (kType == kKvFp4) {
+#pragma unroll
+      for (int i = 0; i < T::kNg; i++) {
+        const int j = i * 64 + lane, blk = j % (DP / kFp4Group);
+        if (T::kG % 64 && j >= T::kG) continue;
+        const int r = wave * kMine + j / (DP / kFp4Group);
+        const half2v ks = {ks4[i], ks4[i]}, vs = {vs4[i], vs4[i]};
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+          const int at = L::at(r, 4 * blk + c) + buf * T::kBytes;
+          *reinterpret_cast<u32x4*>(kbuf + at) = fp4_to_f16(kr4[i][c], ks);
+          *reinterpret_cast<u32x4*>(vbuf + at) = fp4_to_f16(vr4[i][c], vs);
+        }
+      }
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < T::kN; i++) {
       const int at = ((wave * T::kN + i) * 64 + lane) * 16 + buf * T::kBytes;
@@ -172,14 +217,14 @@ __global__ void __launch_bounds__(256, 2) attn_tile_kernel(AttnArgs a) {
     if (lane < 2 * kMine) scales[(buf * 2 + !sk) * BK + srow] = sr;
   };
 
-  // fp16: tile i + 1 is copied into LDS while tile i is worked on.  8-bit: tile i + 1 is
+  // fp16: tile i + 1 is copied into LDS while tile i is worked on.  Codes: tile i + 1 is
   // stored there (its codes came in during tile i - 1) and the loads of i + 2 begin.
   constexpr int kAhead = kType == kKvFp16 ? 1 : 2;
   const int tiles = (hi - lo + BK - 1) / BK;
   if (tiles > 0) {
     look_up(lo);
     issue(lo, 0);
-    if (kType == kKvInt8) {
+    if (kType != kKvFp16) {
       store(0);
       look_up(lo + BK);
       if (tiles > 1) issue(lo + BK, 1);
@@ -196,7 +241,7 @@ __global__ void __launch_bounds__(256, 2) attn_tile_kernel(AttnArgs a) {
   // its own runs of the two kinds, tile by tile with the others.
   auto step = [&](auto masked, int i) __attribute__((always_inline)) {
     const int p0 = lo + i * BK, buf = i & 1;
-    if (kType == kKvInt8 && i + 1 < tiles) store(buf ^ 1);
+    if (kType != kKvFp16 && i + 1 < tiles) store(buf ^ 1);
     if (i + kAhead < tiles) {
       issue(p0 + kAhead * BK, buf ^ 1);
       look_up(p0 + (kAhead + 1) * BK);
@@ -288,6 +333,11 @@ hipError_t run(const AttnArgs& a, hipStream_t s) {
 
 hipError_t launch_attn_tile(const AttnArgs& a, hipStream_t s) {
   const int D = a.c.head_dim;
+  if (a.c.dtype == kKvFp4)
+    return D <= 64    ? launch<kKvFp4, 32, 64, 64, true>(a, s)
+           : D <= 96  ? launch<kKvFp4, 32, 96, 64, true>(a, s)
+           : D <= 128 ? launch<kKvFp4, 32, 128, 64, true>(a, s)
+                      : launch<kKvFp4, 16, 256, 32, true>(a, s);
   if (a.c.dtype == kKvFp16)
     return D <= 64    ? run<kKvFp16, 32, 64, 64>(a, s)
            : D <= 96  ? run<kKvFp16, 32, 96, 64>(a, s)

@@ -10,7 +10,9 @@
 // then to the cache's type: fp16 to nearest, or int8 codes
 //   s = max|x| / 127 over the head's row, code = round_half_away(x / s)
 // with both quotients in fp32 (s = 0 and codes 0 where that underflows; s = NaN
-// and codes 0 for a row that holds an infinity or NaN).
+// and codes 0 for a row that holds an infinity or NaN), or 4-bit codes, the same for each
+// group of 32 elements: s = max|x| / 6 rounded to fp16, code the nearest of the grid to
+// x / s in fp32.
 //
 // Bound: HBM for prompts (2048 tokens, 32/8 heads of 128, 92 MB: 20.6 us, 4.5 TB/s, a
 // large copy's 4.9; 999 tokens into an 8-bit cache 9.8, 1.2 TB/s), latency for few tokens (one: 4.2 us, of which an empty kernel is
@@ -145,6 +147,31 @@ __global__ void __launch_bounds__(kAppendThreads) append_kv_kernel(AppendArgs a)
                  ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)x[2 * i + 1]) << 16);
         *reinterpret_cast<u32x4*>(dst) = p;
       }
+    } else if (kType == kKvFp4) {
+      // A group of 32 elements is four lanes.
+      uint32_t mb = 0;
+#pragma unroll
+      for (int i = 0; i < 8; i++) mb = max(mb, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+      mb = max(mb, (uint32_t)__shfl_xor((int)mb, 1, 64));
+      mb = max(mb, (uint32_t)__shfl_xor((int)mb, 2, 64));
+      if (live && !is_q) {
+        _Float16 s = (_Float16)(__uint_as_float(mb) / 6.0f);
+        if (!((float)s <= 65504.0f)) s = (_Float16)__builtin_nanf("");
+        const float sf = (float)s;
+        uint32_t p = 0;
+        if (sf > 0.0f) {
+#pragma unroll
+          for (int i = 0; i < 8; i++) p |= fp4_code(x[i] / sf) << 4 * i;
+        }
+        uint8_t* dst = (is_k ? (uint8_t*)a.c.k + (size_t)page * a.c.k_page
+                             : (uint8_t*)a.c.v + (size_t)page * a.c.v_page) + (tok * D + e0) / 2;
+        *reinterpret_cast<uint32_t*>(dst) = p;
+        if (unit % 4 == 0) {
+          const size_t at = ((size_t)(h * (D / kFp4Group) + unit / 4) << a.c.page_shift) + slot;
+          (is_k ? (_Float16*)a.c.k_scale + (size_t)page * a.c.ks_page
+                : (_Float16*)a.c.v_scale + (size_t)page * a.c.vs_page)[at] = s;
+        }
+      }
     } else {
       // By bit pattern infinities and NaN are above every finite value.
       uint32_t mb = 0;
@@ -193,6 +220,8 @@ hipError_t launch_append_kv(const KvCache& c, const KvBatch& b, float* q_out, si
   const dim3 grid(b.tokens, split);
   if (c.dtype == kKvFp16)
     append_kv_kernel<kKvFp16><<<grid, kAppendThreads, 0, s>>>(a);
+  else if (c.dtype == kKvFp4)
+    append_kv_kernel<kKvFp4><<<grid, kAppendThreads, 0, s>>>(a);
   else
     append_kv_kernel<kKvInt8><<<grid, kAppendThreads, 0, s>>>(a);
   return hipGetLastError();

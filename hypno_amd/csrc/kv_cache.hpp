@@ -10,10 +10,12 @@ namespace hypno {
 
 constexpr int kKvFp16 = 0;  // values of HYPNO_HIP_KV_* in include/hypno_hip.h
 constexpr int kKvInt8 = 1;
+constexpr int kKvFp4 = 2;
 
 // K and V as [pages][kv_heads][page_size][head_dim] (one kv head's tokens of a
 // page are one run of memory), fp16, or int8 codes beside [pages][kv_heads][page_size]
-// fp32 scales.  Page strides are in elements.
+// fp32 scales, or 4-bit codes, two a byte, beside [pages][kv_heads][head_dim / 32][page_size]
+// fp16 scales.  Page strides are in elements, of 4-bit codes in bytes.
 struct KvCache {
   int dtype;
   void* k;
@@ -23,6 +25,24 @@ struct KvCache {
   size_t k_page, v_page, ks_page, vs_page;
   int pages, kv_heads, page_shift, head_dim;  // page_size = 1 << page_shift
 };
+
+// Elements of a group of 4-bit codes with one scale.
+constexpr int kFp4Group = 32;
+
+// A 4-bit code's value, exact in fp16: its sign, exponent and fraction bit in fp16's
+// places have the value times 2^-14 (0.5 of it a subnormal number there too).
+__device__ __forceinline__ _Float16 fp4_value(uint32_t code) {
+  const uint16_t bits = (uint16_t)((code & 8) << 12 | (code & 7) << 9);
+  return __builtin_bit_cast(_Float16, bits) * (_Float16)16384.0f;
+}
+
+// The code of y: the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6, halves to the even code.
+__device__ __forceinline__ uint32_t fp4_code(float y) {
+  const float a = fabsf(y);
+  const uint32_t c = (a > 0.25f) + (a >= 0.75f) + (a > 1.25f) + (a >= 1.75f) + (a > 2.5f) +
+                     (a >= 3.5f) + (a > 5.0f);
+  return c | (__float_as_uint(y) >> 28 & 8);
+}
 
 // Sequence b brings the tokens [cu_q[b], cu_q[b + 1]) of `tokens`, the last ones
 // of the kv_lens[b] that it then holds; its page i is page_table[b * width + i].
@@ -64,6 +84,30 @@ hipError_t launch_append_kv(const KvCache& c, const KvBatch& b, float* q_out, si
                             size_t k_stride, const float* v, size_t v_stride,
                             const float* inv_freq, int rot, bool pairs, int num_cus,
                             hipStream_t s);
+
+// The keys' bounds of each page and kv head, [pages][kv_heads][2][head_dim] codes (the
+// smallest, the largest) beside [pages][kv_heads] fp32 scales.  Page strides are in elements.
+struct KeyBounds {
+  int8_t* codes;
+  float* scale;
+  size_t page, s_page;
+  int pages, kv_heads, page_shift, head_dim;
+};
+
+// Pages of a sequence that scores are kept of at most (in LDS).
+constexpr int kMaxScored = 32768;
+// Pages that a token reads at most.
+constexpr int kMaxSelected = 1024;
+
+hipError_t launch_key_bounds(const KeyBounds& o, const KvCache& c, const KvBatch& b, int num_cus,
+                             hipStream_t s);
+// `pages`: of a sequence, at most kMaxScored.
+hipError_t launch_select_pages(int* out, int count, int first, int last, const float* q,
+                               size_t q_stride, int heads, const KeyBounds& k, const KvBatch& b,
+                               int pages, int num_cus, hipStream_t s);
+hipError_t launch_selected_attention(float* out, const float* q, size_t q_stride, int heads,
+                                     const KvCache& c, const KvBatch& b, float scale,
+                                     const int* selected, int count, hipStream_t s);
 
 // How the positions of a tile of rows are split: into ranges of `chunk`, the last
 // one of `splits` taking what is left.

@@ -1,0 +1,415 @@
+// Pages that a token reads of a long context, by a cheap score of each, and the bounds
+// of the keys that the score is made of.
+//
+// Bounds of a page and kv head: the smallest and largest key in each channel, as codes
+//   s = max|k| / 127 over the page's keys, code = round_half_away(k / s)
+// with both quotients in fp32 (s = 0 and codes 0 where that underflows; s = NaN and
+// codes 0 for a page that holds an infinity or NaN).  For any key of the page
+//   q.k <= q+ . hi + q- . lo = sum_d max(q_d lo_d, q_d hi_d),
+// q+ and q- the positive and negative part of q: but for the codes' rounding the score
+// is the most that any key of the page can give.  With q in 8-bit codes of its own (per
+// head, the same rule) that is a product of whole numbers, exact on the matrix cores
+// in any order, so that the choice depends on no sum's order:
+//   score = bounds' scale * max over the kv head's query heads of q's scale * (whole number)
+// with these two products in fp32.
+#include "kv_cache.hpp"
+
+namespace hypno {
+
+namespace {
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4a8 __attribute__((ext_vector_type(4), aligned(8)));
+typedef float f32x4a4 __attribute__((ext_vector_type(4), aligned(4)));
+
+constexpr int kMaxDim = 256;
+
+// The code of x with scale s > 0.
+__device__ __forceinline__ uint32_t code8(float x, float s) {
+  return (uint32_t)(int)fminf(fmaxf(roundf(x / s), -127.0f), 127.0f) & 0xFFu;
+}
+
+// --- bounds -------------------------------------------------------------------------------
+
+struct BoundsArgs {
+  KvCache c;
+  KvBatch b;
+  KeyBounds o;
+  int lane_shift;  // 1 << lane_shift lanes a key, each with 8 channels
+};
+
+// The sequence whose pages' numbers reach `slot`, where sequence i's start at
+// floor(cu_q[i] / page_size) + 2 i (n tokens are in floor((n - 1) / page_size) + 2 pages at
+// most).
+__device__ __forceinline__ int seq_of_page(const BoundsArgs& a, int slot) {
+  const int lane = threadIdx.x & 63;
+  int count = 0;
+  for (int i0 = 0; i0 <= a.b.batch; i0 += 64) {
+    const int i = i0 + lane;
+    bool in = false;
+    if (i <= a.b.batch) in = (cu_at(a.b, i) >> a.c.page_shift) + 2 * (int64_t)i <= slot;
+    count += __popcll(__ballot(in));
+  }
+  return count - 1;
+}
+
+template <int kType>
+__device__ __forceinline__ void load_keys(float (&x)[8], const BoundsArgs& a, int page, int g,
+                                          int slot, int e0) {
+  const int D = a.c.head_dim;
+  const size_t tok = ((size_t)g << a.c.page_shift) + slot;
+  if (kType == kKvFp16) {
+    const u32x4 v = load_global<u32x4>((const _Float16*)a.c.k + (size_t)page * a.c.k_page +
+                                       tok * D + e0);
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+      x[i] = (float)__builtin_bit_cast(_Float16, (uint16_t)(v[i / 2] >> 16 * (i % 2)));
+  } else if (kType == kKvInt8) {
+    const uint2 v = load_global<uint2>((const int8_t*)a.c.k + (size_t)page * a.c.k_page + tok * D +
+                                       e0);
+    const float s = load_global<float>(a.c.k_scale + (size_t)page * a.c.ks_page + tok);
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+      x[i] = (float)(int8_t)((i < 4 ? v.x : v.y) >> 8 * (i % 4)) * s;
+  } else {
+    const uint32_t v = load_global<uint32_t>((const uint8_t*)a.c.k + (size_t)page * a.c.k_page +
+                                             (tok * D + e0) / 2);
+    const size_t at = ((size_t)(g * (D / kFp4Group) + e0 / kFp4Group) << a.c.page_shift) + slot;
+    const _Float16 s = load_global<_Float16>((const _Float16*)a.c.k_scale +
+                                             (size_t)page * a.c.ks_page + at);
+#pragma unroll
+    for (int i = 0; i < 8; i++) x[i] = (float)(_Float16)(fp4_value(v >> 4 * i) * s);
+  }
+}
+
+// One work-group a (page, kv head) at a time; 8 channels a lane, keys over the rest.
+template <int kType>
+__global__ void __launch_bounds__(256) key_bounds_kernel(BoundsArgs a) {
+  __shared__ float s_lo[4][kMaxDim], s_hi[4][kMaxDim];
+  __shared__ uint32_t s_bits[4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int D = a.c.head_dim, KV = a.c.kv_heads;
+  const int unit = tid & ((1 << a.lane_shift) - 1), row = tid >> a.lane_shift;
+  const int e0 = 8 * unit, rows = 256 >> a.lane_shift;
+  const int64_t slots = (cu_at(a.b, a.b.batch) >> a.c.page_shift) + 2 * (int64_t)a.b.batch;
+  for (int64_t w = blockIdx.x; w < slots * KV; w += gridDim.x) {
+    // (all lanes decide the same)
+    const int slot = (int)(w / KV), g = (int)(w % KV);
+    const int b = seq_of_page(a, slot);
+    if (b < 0 || b >= a.b.batch) continue;
+    const int first = cu_at(a.b, b), n = cu_at(a.b, b + 1) - first;
+    const int kv = load_global<int>(a.b.kv_lens + b);
+    if (n <= 0 || kv <= 0) continue;
+    const int at = (int)(max((int64_t)kv - n, (int64_t)0) >> a.c.page_shift) + slot -
+                   ((first >> a.c.page_shift) + 2 * b);
+    if (at > (kv - 1) >> a.c.page_shift || at >= a.b.width) continue;
+    const int page = load_global<int>(a.b.page_table + (size_t)b * a.b.width + at);
+    if (page < 0 || page >= a.c.pages) continue;
+    const int keys = min(1 << a.c.page_shift, kv - (at << a.c.page_shift));
+    float lo[8], hi[8];
+    uint32_t mb = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) lo[i] = __builtin_inff(), hi[i] = -__builtin_inff();
+    if (e0 < D) {
+#pragma unroll 4
+      for (int r = row; r < keys; r += rows) {
+        float x[8];
+        load_keys<kType>(x, a, page, g, r, e0);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          lo[i] = fminf(lo[i], x[i]);
+          hi[i] = fmaxf(hi[i], x[i]);
+          mb = max(mb, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+        }
+      }
+    }
+    for (int off = 1 << a.lane_shift; off < 64; off <<= 1)
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        lo[i] = fminf(lo[i], __shfl_xor(lo[i], off, 64));
+        hi[i] = fmaxf(hi[i], __shfl_xor(hi[i], off, 64));
+      }
+    for (int off = 32; off > 0; off >>= 1) mb = max(mb, (uint32_t)__shfl_xor((int)mb, off, 64));
+    if (lane < 1 << a.lane_shift && e0 < D) {
+#pragma unroll
+      for (int i = 0; i < 8; i++) s_lo[wave][e0 + i] = lo[i], s_hi[wave][e0 + i] = hi[i];
+    }
+    if (lane == 0) s_bits[wave] = mb;
+    __syncthreads();
+    // Two rows of codes, four a lane.
+    const int e = 4 * tid % kMaxDim, half = 4 * tid / kMaxDim;
+    mb = max(max(s_bits[0], s_bits[1]), max(s_bits[2], s_bits[3]));
+    const float s = mb < 0x7F800000u ? __uint_as_float(mb) / 127.0f : __builtin_nanf("");
+    if (half < 2 && e < D) {
+      uint32_t codes = 0;
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const float x =
+            half ? fmaxf(fmaxf(s_hi[0][e + i], s_hi[1][e + i]), fmaxf(s_hi[2][e + i], s_hi[3][e + i]))
+                 : fminf(fminf(s_lo[0][e + i], s_lo[1][e + i]), fminf(s_lo[2][e + i], s_lo[3][e + i]));
+        if (s > 0.0f) codes |= code8(x, s) << 8 * i;
+      }
+      *reinterpret_cast<uint32_t*>(a.o.codes + (size_t)page * a.o.page + (size_t)(2 * g + half) * D +
+                                   e) = codes;
+    }
+    if (tid == 0) a.o.scale[(size_t)page * a.o.s_page + g] = s;
+    __syncthreads();
+  }
+}
+
+// --- selection ------------------------------------------------------------------------------
+
+struct SelectArgs {
+  KeyBounds k;
+  KvBatch b;
+  int* out;
+  const float* q;
+  size_t q_stride;
+  int heads, group, count, first, last;
+  int most;    // pages of a sequence that have a score at most
+  int pitch;   // of a token's keys in LDS
+  int tokens;  // of a work-group
+};
+
+// Scores as whole numbers in their order, from 1 on; 0: no candidate.  (What is no
+// number, and infinities, as the largest finite one: below what is always selected.)
+__device__ __forceinline__ uint32_t key_of(float x) {
+  const float m = 3.4028234663852886e38f;
+  const float y = (x == x ? fminf(fmaxf(x, -m), m) : m) + 0.0f;
+  const uint32_t u = __float_as_uint(y);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+// Orders LDS accesses of a wave's lanes among themselves.
+__device__ __forceinline__ void wave_lds_sync() {
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_wave_barrier();
+#endif
+}
+
+// One work-group a kv head of up to 16 / group tokens of a sequence: scores of their
+// pages into LDS, 16 pages by 16 rows (token, head) a wave at a time, then for each token
+// the largest.  kTeam: all waves search one token's keys, else each wave its own tokens'.
+template <int DP, int kWaves, bool kTeam>
+__global__ void __launch_bounds__(64 * kWaves) select_pages_kernel(SelectArgs a) {
+  constexpr int kSteps = 2 * DP / 64, kPitch = 2 * DP + 16;
+  __shared__ __attribute__((aligned(16))) uint8_t codes[16 * kPitch];
+  __shared__ float row_scale[16], part[kWaves][16][17];
+  __shared__ int counts[2][kWaves];
+  extern __shared__ uint32_t keys[];  // [tokens][pitch]
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int KV = a.k.kv_heads, G = a.group, D = a.k.head_dim, shift = a.k.page_shift;
+  const int g = blockIdx.x % KV, slot = blockIdx.x / KV;
+  const int b = find_seq(a.b, slot, 1, a.tokens);
+  if (b < 0 || b >= a.b.batch) return;
+  const int first = cu_at(a.b, b), n = cu_at(a.b, b + 1) - first;
+  const int i0 = (slot - (first / a.tokens + b)) * a.tokens, nt = min(a.tokens, n - i0);
+  if (i0 < 0 || nt <= 0) return;
+  const int t0 = first + i0;
+  // The page of token i of the tile is (pos0 + i) >> shift: -1 and less if it has no place.
+  const int64_t pos0 = (int64_t)load_global<int>(a.b.kv_lens + b) - n + i0;
+  const int most = min(a.most, a.b.width);
+  const int top = (int)min((int64_t)most, ((pos0 + nt - 1) >> shift) + 1 - a.last);
+  const int* const table = a.b.page_table + (size_t)b * a.b.width;
+
+  for (int h0 = 0; h0 < G && top > a.first; h0 += 16) {
+    // The rows' codes, [negative part][positive part]; 16 lanes a row.
+    if (wave < 4) {
+      const int r = tid / 16, sub = tid % 16;
+      const int tok = G <= 16 ? r / G : 0, h = G <= 16 ? r % G : h0 + r;
+      const bool live = tok < nt && h < G && (G > 16 || r < nt * G);
+      float x[DP / 128 + 1][8];
+      uint32_t mb = 0;
+#pragma unroll
+      for (int j = 0; j < (DP + 127) / 128; j++) {
+        const int e = sub * 8 + 128 * j;
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[j][i] = 0.0f;
+        if (live && e < D) {
+          const float* src = a.q + (size_t)(t0 + tok) * a.q_stride + (size_t)(g * G + h) * D + e;
+          const f32x4a4 u = load_global<f32x4a4>(src), v = load_global<f32x4a4>(src + 4);
+#pragma unroll
+          for (int i = 0; i < 8; i++) x[j][i] = i < 4 ? u[i] : v[i - 4];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) mb = max(mb, __float_as_uint(x[j][i]) & 0x7FFFFFFFu);
+      }
+#pragma unroll
+      for (int off = 8; off > 0; off >>= 1) mb = max(mb, (uint32_t)__shfl_xor((int)mb, off, 64));
+      const float s = mb < 0x7F800000u ? __uint_as_float(mb) / 127.0f : 0.0f;
+#pragma unroll
+      for (int j = 0; j < (DP + 127) / 128; j++) {
+        const int e = sub * 8 + 128 * j;
+        if (e >= DP) continue;
+        uint32_t neg[2] = {0, 0}, pos[2] = {0, 0};
+        if (s > 0.0f) {
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            const uint32_t c = code8(x[j][i], s) << 8 * (i % 4);
+            (x[j][i] < 0.0f ? neg : pos)[i / 4] |= c;
+          }
+        }
+        *reinterpret_cast<uint2*>(codes + r * kPitch + e) = make_uint2(neg[0], neg[1]);
+        *reinterpret_cast<uint2*>(codes + r * kPitch + DP + e) = make_uint2(pos[0], pos[1]);
+      }
+      if (sub == 0) row_scale[r] = s;
+    }
+    __syncthreads();
+    i32x4 q[kSteps];
+#pragma unroll
+    for (int s = 0; s < kSteps; s++)
+      q[s] = *reinterpret_cast<const i32x4*>(codes + lane % 16 * kPitch + 64 * s + lane / 16 * 16);
+    const float qs = row_scale[lane % 16];
+    for (int p0 = a.first + 16 * wave; p0 < top; p0 += 16 * kWaves) {
+      const int p = p0 + lane % 16;
+      int page = p < top ? load_global<int>(table + p) : -1;
+      const bool there = page >= 0 && page < a.k.pages;
+      page = there ? page : 0;
+      i32x4 acc = {0, 0, 0, 0};
+      if (a.k.pages) {  // (none: nothing is read)
+        const int8_t* const src = a.k.codes + (size_t)page * a.k.page + (size_t)2 * g * D;
+        i32x4 k[kSteps];
+#pragma unroll
+        for (int s = 0; s < kSteps; s++) {
+          // Sixteen channels from d on of one bound; those past D meet zeros.
+          const int c = 64 * s + lane / 16 * 16, d = c % DP;
+          const int8_t* const at = src + (c < DP ? 0 : D) + (d < D ? d : 0);
+          if (D % 16 == 0) {
+            k[s] = __builtin_bit_cast(i32x4, load_global<u32x4a8>(at));
+          } else {
+            const uint2 lo = load_global<uint2>(at);
+            const uint2 hi = load_global<uint2>(d + 8 < D ? at + 8 : at);
+            k[s] = i32x4{(int)lo.x, (int)lo.y, (int)hi.x, (int)hi.y};
+          }
+        }
+#pragma unroll
+        for (int s = 0; s < kSteps; s++)
+          acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[s], q[s], acc, 0, 0, 0);
+      }
+      const float ks = there ? load_global<float>(a.k.scale + (size_t)page * a.k.s_page + g) : 0.0f;
+#pragma unroll
+      for (int i = 0; i < 4; i++) part[wave][lane / 16 * 4 + i][lane % 16] = (float)acc[i] * qs;
+      wave_lds_sync();
+      for (int tok = lane / 16; tok < nt; tok += 4) {
+        const float* const rows = part[wave][lane % 16] + (G <= 16 ? tok * G : 0);
+        float m = rows[0];
+        for (int h = 1; h < min(G - h0, 16); h++) m = fmaxf(m, rows[h]);
+        uint32_t key = key_of(m * ks);
+        if (!there || p > ((pos0 + tok) >> shift) - a.last) key = 0;
+        if (p < top) {
+          uint32_t* const to = keys + (size_t)tok * a.pitch + p;
+          *to = h0 ? max(*to, key) : key;
+        }
+      }
+      wave_lds_sync();
+    }
+    __syncthreads();
+  }
+
+  // Each token's largest, in the pages' order.
+  int at = 0;  // of counts
+  for (int tok = kTeam ? 0 : wave; tok < nt; tok += kTeam ? 1 : kWaves) {
+    const int64_t pos = pos0 + tok;
+    const int own = pos < 0 ? -1 : (int)(pos >> shift);
+    const int hi = min(most, own + 1 - a.last), need = a.count - a.first - a.last;
+    const uint32_t* const key = keys + (size_t)tok * a.pitch;
+    auto above = [&](uint32_t least) __attribute__((always_inline)) {
+      int c = 0;
+      for (int p = a.first + (kTeam ? tid : lane); p - (kTeam ? tid : lane) < hi;
+           p += kTeam ? 64 * kWaves : 64)
+        c += __popcll(__ballot(p < hi && key[p] >= least));
+      if (!kTeam) return c;
+      if (lane == 0) counts[at][wave] = c;
+      __syncthreads();
+      c = 0;
+#pragma unroll
+      for (int w = 0; w < kWaves; w++) c += counts[at][w];
+      at ^= 1;
+      return c;
+    };
+    // The key of the last one that is taken: the largest that `need` reach.
+    uint32_t least = 1;
+    int ties = 0x7FFFFFFF;  // of those with this key that are taken
+    if (hi > a.first && above(1) > need) {
+      int c = 0;
+      least = 0;
+      for (uint32_t bit = 0x80000000u; bit && c != need; bit >>= 1) {
+        const int x = above(least | bit);
+        if (x >= need) least |= bit, c = x;
+      }
+      if (c != need) ties = need - (least == 0xFFFFFFFFu ? 0 : above(least + 1));
+    }
+    if (kTeam && wave) continue;
+    int* const out = a.out + ((size_t)(t0 + tok) * KV + g) * a.count;
+    int put = min(a.first, own + 1);
+    if (lane < put) out[lane] = lane;
+    for (int i = lane + 64; i < put; i += 64) out[i] = i;
+    for (int p0 = a.first; p0 < hi && need > 0; p0 += 64) {
+      const int p = p0 + lane;
+      const uint32_t k = p < hi ? key[p] : 0;
+      const uint64_t same = __ballot(k == least), before = (1ull << lane) - 1;
+      const bool take = k > least || (k == least && k && __popcll(same & before) < ties);
+      const uint64_t taken = __ballot(take);
+      if (take) out[put + __popcll(taken & before)] = p;
+      put += __popcll(taken);
+      ties -= min(ties, (int)__popcll(same));
+    }
+    const int tail = max(own + 1 - a.last, min(a.first, own + 1));
+    for (int p = tail + lane; p <= own; p += 64) out[put + p - tail] = p;
+    put += own + 1 - tail;
+    for (int i = put + lane; i < a.count; i += 64) out[i] = -1;
+  }
+}
+
+template <int DP>
+hipError_t run_select(const SelectArgs& a, size_t lds, bool team, hipStream_t s) {
+  const size_t grid = ((size_t)a.b.tokens / a.tokens + a.b.batch) * a.k.kv_heads;
+  if (grid > 0x7FFFFFFF) return hipErrorInvalidValue;
+  const void* fn = team ? (const void*)select_pages_kernel<DP, 16, true>
+                        : (const void*)select_pages_kernel<DP, 4, false>;
+  const hipError_t e = set_lds_limit(fn, (int)lds);
+  if (e != hipSuccess) return e;
+  if (team)
+    select_pages_kernel<DP, 16, true><<<(unsigned)grid, 1024, lds, s>>>(a);
+  else
+    select_pages_kernel<DP, 4, false><<<(unsigned)grid, 256, lds, s>>>(a);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_key_bounds(const KeyBounds& o, const KvCache& c, const KvBatch& b, int num_cus,
+                             hipStream_t s) {
+  BoundsArgs a = {c, b, o, 0};
+  while (8 << a.lane_shift < c.head_dim) a.lane_shift++;
+  // Work-groups for all pages that the batch can have, or as many as the chip holds.
+  const size_t slots = std::min((size_t)(b.tokens >> c.page_shift) + 2 * (size_t)b.batch,
+                                (size_t)b.batch * ((size_t)b.width + 2));
+  const unsigned grid = (unsigned)std::min(slots * c.kv_heads, (size_t)8 * num_cus);
+  if (c.dtype == kKvFp16)
+    key_bounds_kernel<kKvFp16><<<grid, 256, 0, s>>>(a);
+  else if (c.dtype == kKvInt8)
+    key_bounds_kernel<kKvInt8><<<grid, 256, 0, s>>>(a);
+  else
+    key_bounds_kernel<kKvFp4><<<grid, 256, 0, s>>>(a);
+  return hipGetLastError();
+}
+
+hipError_t launch_select_pages(int* out, int count, int first, int last, const float* q,
+                               size_t q_stride, int heads, const KeyBounds& k, const KvBatch& b,
+                               int pages, int num_cus, hipStream_t s) {
+  SelectArgs a = {k, b, out, q, q_stride, heads, heads / k.kv_heads, count, first, last, pages,
+                  (pages + 3) / 4 * 4, 1};
+  a.tokens = std::max(1, 16 / a.group);
+  const size_t room = 128 << 10;
+  a.tokens = (int)std::min<size_t>(a.tokens, std::max<size_t>(1, room / 4 / std::max(a.pitch, 1)));
+  const size_t groups = ((size_t)b.tokens / a.tokens + b.batch) * k.kv_heads;
+  const bool team = pages > 2048 || (pages > 256 && groups <= (size_t)num_cus);
+  const size_t lds = (size_t)a.tokens * a.pitch * 4;
+  return k.head_dim <= 64    ? run_select<64>(a, lds, team, s)
+         : k.head_dim <= 128 ? run_select<128>(a, lds, team, s)
+                             : run_select<256>(a, lds, team, s);
+}
+
+}  // namespace hypno

@@ -437,21 +437,34 @@ typedef struct hypno_hip_kv_batch {
 /* Element types of a cache.  INT8: per (token, kv head) the codes c = round(x / s),
  * halves away from zero, and one fp32 scale s = max|x| / 127 (a row of zeros, or one
  * whose scale underflows: s = 0 and codes 0; one that holds an infinity or NaN: s =
- * NaN and codes 0).  FP16: rounded to nearest (from 65520 on: infinity). */
+ * NaN and codes 0).  FP16: rounded to nearest (from 65520 on: infinity).
+ *
+ * FP4: two codes a byte, that of the even element in its low four bits: a sign above
+ * one of 0, 0.5, 1, 1.5, 2, 3, 4, 6 (two bits of exponent, one of fraction), and one
+ * fp16 scale for each 32 elements of a (token, kv head).  The value is code * scale,
+ * rounded to fp16 (from 65520 on: infinity), so that such a cache stands for an FP16
+ * one.  append: s = max|x| / 6 in fp32, rounded to fp16; code = x / s in fp32, rounded
+ * to the nearest of the grid, halves to the even code (the even fraction bit), and to 6
+ * beyond it (a group whose scale underflows: s = 0 and codes 0; one that holds an
+ * infinity, a NaN or whose scale overflows: s = NaN and codes 0). */
 #define HYPNO_HIP_KV_FP16 0u
 #define HYPNO_HIP_KV_INT8 1u
+#define HYPNO_HIP_KV_FP4 2u
 
 typedef struct hypno_hip_kv_cache {
   uint32_t dtype;             /* HYPNO_HIP_KV_* */
   void* k;                    /* [pages][kv_heads][page_size][head_dim], 16-byte aligned */
-  void* v;
-  float* k_scale;             /* INT8: [pages][kv_heads][page_size]; FP16: NULL */
-  float* v_scale;
+  void* v;                    /* (FP4: the last is head_dim / 2 bytes) */
+  void* k_scale;              /* INT8: float [pages][kv_heads][page_size]; FP16: NULL;
+                               * FP4: fp16 [pages][kv_heads][head_dim / 32][page_size],
+                               * 16-byte aligned */
+  void* v_scale;
   size_t pages, kv_heads;
-  size_t page_size;           /* a power of two, at most 2^16 */
-  size_t head_dim;            /* a multiple of 8, at most 256 */
-  /* Elements from one page to the next, of k, v, k_scale and v_scale (0: no gap
-   * between pages; of k and v multiples of 8). */
+  size_t page_size;           /* a power of two, at most 2^16 (FP4: at least 16) */
+  size_t head_dim;            /* a multiple of 8 (FP4: of 32), at most 256 */
+  /* Elements (of k and v of FP4: bytes) from one page to the next, of k, v, k_scale and
+   * v_scale (0: no gap between pages; of k and v multiples of 8, FP4: of 16, and of the
+   * scales of FP4 multiples of 8). */
   size_t k_page_stride, v_page_stride, k_scale_page_stride, v_scale_page_stride;
 } hypno_hip_kv_cache;
 
@@ -477,7 +490,7 @@ int hypno_hip_append_kv_dev(const hypno_hip_kv_cache* cache, const hypno_hip_kv_
  * h / (heads / kv_heads).  Zeros where that leaves none, or no w_p but 0.  The cache's
  * values are used exactly; sums and softmax statistics are fp32; q is held to 22 bits of
  * its row's largest element and more.  Beside an INT8 cache w is held to all 24 bits;
- * beside an FP16 one to 22, but to no less than 2^-37 of the row's largest w: from 2^-15 of
+ * beside an FP16 or FP4 one to 22, but to no less than 2^-37 of the row's largest w: from 2^-15 of
  * that largest on a w has fewer bits, from 2^-37 on none.  That is below fp32's rounding of
  * the heaviest keys' values unless these are 0 or nearly so: an element of out that then
  * comes from w of e^-20 of the largest may be off by 0.4%, one from w of e^-26 is 0.
@@ -490,6 +503,61 @@ int hypno_hip_paged_attention_dev(float* out, const float* q, size_t q_stride, s
                                   const hypno_hip_kv_cache* cache,
                                   const hypno_hip_kv_batch* batch, float scale, size_t window,
                                   size_t max_kv_len, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Attention over the pages of a long context that a cheap score selects for each new
+ * token and kv head (no counterpart in hypno).  After append_kv: key_bounds brings the
+ * bounds of the pages that the new tokens are in up to date, select_pages ranks a
+ * sequence's pages by them, selected_attention reads the chosen ones.
+ * ------------------------------------------------------------------------- */
+/* The smallest and largest key of each channel over the tokens of a page, per kv head:
+ * with s = max|k| / 127 over both, codes round(k / s), halves away from zero, quotients
+ * in fp32 (s = 0 and codes 0 where s underflows; s = NaN and codes 0 for a page that
+ * holds an infinity or NaN).  The keys are the cache's values (INT8: code * scale in
+ * fp32). */
+typedef struct hypno_hip_key_bounds {
+  int8_t* codes;              /* [pages][kv_heads][2][head_dim]: smallest, largest; 16-byte
+                               * aligned */
+  float* scale;               /* [pages][kv_heads] */
+  size_t pages, kv_heads, page_size, head_dim; /* the cache's */
+  /* Elements from one page to the next (0: no gap; of codes a multiple of 16). */
+  size_t page_stride, scale_page_stride;
+} hypno_hip_key_bounds;
+
+/* Computes the bounds of every page that holds a new token of the batch from all of its
+ * tokens in the cache, the sequence's positions below kv_lens[b]; other pages' bounds are
+ * left alone.  batch->tokens: cu_q[batch] or more.  Of the cache only k and k_scale are
+ * read (v and v_scale may be NULL). */
+int hypno_hip_key_bounds_dev(const hypno_hip_key_bounds* bounds, const hypno_hip_kv_cache* cache,
+                             const hypno_hip_kv_batch* batch, void* stream);
+
+/* selected[t][g] [tokens][kv_heads][count]: the pages (their numbers j in the sequence,
+ * page_table[b][j]) that token t at position p is to read for kv head g, ascending, and
+ * -1 behind them.  Of the pages 0 to p / page_size the first `first` and the last `last`
+ * (at least 1: the token's own) are always among them, and then those with the largest
+ * score, the lower page first among equal ones, until there are `count`:
+ *   score = (max over the heads h of g of (sum_d c_d b_d) * s) * scale
+ * with c and s the codes and scale of q[t][h] by the rule of the bounds (a head that holds
+ * an infinity or NaN: 0), b_d the smallest of the page's bounds where c_d < 0 and else the
+ * largest (so that c_d b_d is the larger product), scale the bounds' (0 or more); the sum is
+ * a whole number, the two products are fp32.  A score that is NaN, or above every fp32 number, counts as
+ * the largest one.  Pages that are none of the cache's, or past the table or max_kv_len,
+ * have no score.  A token at a negative position selects nothing; rows of no sequence are
+ * left alone.  max_kv_len: an upper bound of kv_lens (0: table_width * page_size), at most
+ * 32768 pages.  count: at most 1024; first + last at most count. */
+int hypno_hip_select_pages_dev(int32_t* selected, size_t count, size_t first, size_t last,
+                               const float* q, size_t q_stride, size_t heads,
+                               const hypno_hip_key_bounds* bounds,
+                               const hypno_hip_kv_batch* batch, size_t max_kv_len, void* stream);
+
+/* paged_attention over the positions p <= the token's own that are in one of the pages
+ * selected[t][g][0..count) (of kv head g = h / (heads / kv_heads)): numbers below 0 or
+ * past the token's own page are passed over, and a page that is named twice counts twice.
+ * Arithmetic, zeros and NaN as there; pages of 16 tokens at least. */
+int hypno_hip_selected_attention_dev(float* out, const float* q, size_t q_stride, size_t heads,
+                                     const hypno_hip_kv_cache* cache,
+                                     const hypno_hip_kv_batch* batch, float scale,
+                                     const int32_t* selected, size_t count, void* stream);
 
 /* Block until all work this library queued on `stream` is done. */
 int hypno_hip_stream_synchronize(void* stream);
