@@ -1615,8 +1615,17 @@ int hypno_hip_selected_attention_dev(float* out, const float* q, size_t q_stride
   if (overlaps(out, ob, q, qb) || overlaps(out, ob, selected, T * KV * count * 4) ||
       overlaps_kv(out, ob, c, b))
     return fail(HYPNO_HIP_EINVAL, "selected_attention: out overlaps an input");
-  hipError_t e = launch_selected_attention(out, q, q_stride, (int)heads, c, b, scale, selected,
-                                           (int)count, (hipStream_t)stream);
+  DeviceState* ds = nullptr;
+  {
+    std::lock_guard<std::mutex> g(g_mu);
+    st = device_state(&ds);
+    if (st) return st;
+  }
+  const SelectedPlan p = selected_plan(c, b, (int)heads, (int)count, ds->cus);
+  WsLock ws;
+  if (p.bytes) (void)try_workspace(ds, (hipStream_t)stream, p.bytes, ws);
+  hipError_t e = launch_selected_attention(p, out, q, q_stride, (int)heads, c, b, scale, selected,
+                                           (int)count, ws.p, (hipStream_t)stream);
   return e == hipSuccess ? HYPNO_HIP_OK : hip_fail(e, "selected_attention launch");
 }
 

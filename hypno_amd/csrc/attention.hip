@@ -15,13 +15,16 @@ __global__ void __launch_bounds__(64) attn_rows_kernel(AttnArgs a) {
   const int b = find_seq(a.b, t, 0, 0);
   if (b < 0 || b >= a.b.batch) return;
   const Seq sq = seq_of(a.b, b);
-  attn_row(a, sq, t - sq.first, h);
+  attn_row(a, sq, t - sq.first, h,
+           a.selected ? a.selected + ((size_t)t * a.c.kv_heads + h / a.group) * a.count : nullptr,
+           a.count);
 }
 
 // One (token, head): the maxima, sums and outputs of its ranges, by kWaves waves (one
 // where rows are many), each on a part of the ranges.  A lane holds one range's maximum
 // and sum, then four elements of the output in every (64 / lanes)th range.
-template <int kWaves>
+// kList: every row has all ranges of a.fs.
+template <int kWaves, bool kList>
 __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a) {
   __shared__ f32x4 so[4][64];
   __shared__ float2 sml[4];
@@ -35,15 +38,17 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a) {
   const Seq sq = seq_of(a.b, b);
   const int rows = sq.n * G, r = (t - sq.first) * G + h % G;
   if (r < 0 || r >= rows) return;
-  const bool few = rows <= a.few;
+  const bool few = kList || rows <= a.few;
   const AttnSplit sp = few ? a.fs : a.ts;
   if (sp.splits <= 1) return;  // written already
   const int per = few ? kFewRows : a.tile_rows, r0 = r / per * per;
   const bool past = too_long(a, sq);
-  const int all = past ? 0 : split_count(sp, span_of(a, sq, r0, min(r0 + per, rows)));
+  const int all = past    ? 0
+                  : kList ? sp.splits
+                          : split_count(sp, span_of(a, sq, r0, min(r0 + per, rows)));
   const int first = all * part / kWaves, n = all * (part + 1) / kWaves - first;
   const AttnParts parts = few ? a.fp : a.tp;
-  const size_t at0 = (few ? few_part(a, sq, h / G, r, row) : row) * sp.splits + first;
+  const size_t at0 = (few && !kList ? few_part(a, sq, h / G, r, row) : row) * sp.splits + first;
   const float2* ml = parts.ml + at0;
   const int lanes = D <= 64 ? 16 : D <= 128 ? 32 : 64, sub = lane / lanes, d = lane % lanes * 4;
   const float* po = parts.o + at0 * D + d;
@@ -102,7 +107,8 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a) {
   const float z = ((l + v[0]) + (v[1] + v[2]) + v[3]) * 0.0f;
   const bool again = __any(!(z == 0.0f)) || past;
   if (again)
-    attn_row(a, sq, t - sq.first, h);
+    attn_row(a, sq, t - sq.first, h,
+             kList ? a.selected + ((size_t)t * a.c.kv_heads + h / G) * a.count : nullptr, a.count);
   else if (sub == 0 && d < D)
     *reinterpret_cast<f32x4*>(a.out + row * D + d) = v;
 }
@@ -113,6 +119,15 @@ constexpr unsigned kJoinRows = 1024;
 // Bytes of one kernel's ranges at most: a million of them at head_dim 128, where 64
 // sequences of 32 heads take 16 to 32 a row and a chunk of 512 tokens four.
 constexpr size_t kMaxParts = (size_t)512 << 20;
+
+template <bool kList>
+hipError_t join(const AttnArgs& a, unsigned rows, hipStream_t s) {
+  if (rows < kJoinRows)
+    attn_join_kernel<4, kList><<<rows, 256, 0, s>>>(a);
+  else
+    attn_join_kernel<1, kList><<<(rows + 3) / 4, 256, 0, s>>>(a);
+  return hipGetLastError();
+}
 
 int up(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
@@ -136,7 +151,7 @@ AttnPlan attn_plan(const KvCache& c, const KvBatch& b, int heads, int window, in
   // beside three, 8-bit, 113 / 102.)
   const bool only_few = b.tokens <= b.batch || (b.batch == 1 && rows <= 16);
   const bool only_tile = !only_few && (b.batch <= 8 || G > 16);
-  p.few = c.dtype == kKvFp4 ? 0 : only_few ? 0x7FFFFFFF : only_tile ? 0 : kFewRows;
+  p.few = only_few ? 0x7FFFFFFF : only_tile ? 0 : kFewRows;
   const int64_t room = (int64_t)b.width << c.page_shift;
   const int64_t kv = std::max<int64_t>(1, max_kv ? std::min(max_kv, room) : room);
   // Up to 1024 positions (2048 where sequences and heads alone fill the chip) a
@@ -210,7 +225,7 @@ hipError_t launch_paged_attention(const AttnPlan& p, float* out, const float* q,
                                   int heads, const KvCache& c, const KvBatch& b, float scale,
                                   int window, void* ws, hipStream_t s) {
   AttnArgs a = {c, b, out, q, q_stride, heads, heads / c.kv_heads, window, scale,
-                p.few, p.few_waves, p.tile_rows, p.fs, p.ts, p.cus, p.by_seq, {}, {}};
+                p.few, p.few_waves, p.tile_rows, p.fs, p.ts, p.cus, p.by_seq, {}, {}, nullptr, 0};
   if (!ws) a.fs = a.ts = {1, 0x7FFFFFFF};
   a.fp.ml = reinterpret_cast<float2*>(ws);
   a.tp.ml = a.fp.ml + p.few_places;
@@ -224,13 +239,49 @@ hipError_t launch_paged_attention(const AttnPlan& p, float* out, const float* q,
   hipError_t e = hipSuccess;
   if (a.few != 0x7FFFFFFF) e = launch_attn_tile(a, s);
   if (e == hipSuccess && a.few) e = launch_attn_few(a, s);
-  if (e == hipSuccess && (a.fs.splits > 1 || a.ts.splits > 1)) {
-    if (rows < kJoinRows)
-      attn_join_kernel<4><<<rows, 256, 0, s>>>(a);
-    else
-      attn_join_kernel<1><<<(rows + 3) / 4, 256, 0, s>>>(a);
-    e = hipGetLastError();
+  if (e == hipSuccess && (a.fs.splits > 1 || a.ts.splits > 1)) e = join<false>(a, rows, s);
+  return e;
+}
+
+SelectedPlan selected_plan(const KvCache& c, const KvBatch& b, int heads, int count,
+                           int num_cus) {
+  SelectedPlan p = {4, {1, 0x7FFFFFFF}, 0, 0};
+  const int64_t positions = (int64_t)count << c.page_shift;
+  const int64_t pairs = (int64_t)b.tokens * c.kv_heads, slots = 2 * num_cus;
+  const size_t rows = (size_t)b.tokens * heads, place = (size_t)c.head_dim * 4 + 8;
+  // All work-groups are about equally long, so that they are as many as the chip holds at a
+  // time; ranges of 256 positions at least, as joining them costs 4 us and its launch.
+  if (positions > 1024 && pairs < slots) {
+    const int64_t most = std::max<int64_t>(1, (int64_t)(kMaxParts / place / rows));
+    const int64_t splits = std::min(slots / pairs, most);
+    const int64_t chunk = (std::max<int64_t>(256, up(positions, splits)) + 127) / 128 * 128;
+    p.fs = {up(positions, chunk), (int)chunk};
+  } else if (pairs <= num_cus && positions > 128) {
+    p.waves = 8;
   }
+  p.ml_bytes = p.fs.splits > 1 ? (rows * p.fs.splits * 8 + 255) / 256 * 256 : 0;
+  p.bytes = p.fs.splits > 1 ? p.ml_bytes + rows * p.fs.splits * c.head_dim * 4 : 0;
+  return p;
+}
+
+hipError_t launch_selected_attention(const SelectedPlan& p, float* out, const float* q,
+                                     size_t q_stride, int heads, const KvCache& c,
+                                     const KvBatch& b, float scale, const int* selected, int count,
+                                     void* ws, hipStream_t s) {
+  AttnArgs a = {};
+  a.c = c, a.b = b, a.out = out, a.q = q, a.q_stride = q_stride, a.heads = heads;
+  a.group = heads / c.kv_heads, a.scale = scale, a.selected = selected, a.count = count;
+  a.few_waves = p.waves, a.fs = ws ? p.fs : AttnSplit{1, 0x7FFFFFFF};
+  a.ts = {1, 0x7FFFFFFF};
+  a.fp.ml = reinterpret_cast<float2*>(ws);
+  a.fp.o = reinterpret_cast<float*>((uint8_t*)ws + p.ml_bytes);
+  const unsigned rows = (unsigned)b.tokens * (unsigned)heads;
+  if (c.pages == 0) {
+    attn_rows_kernel<<<rows, 64, 0, s>>>(a);
+    return hipGetLastError();
+  }
+  hipError_t e = launch_attn_few(a, s);
+  if (e == hipSuccess && a.fs.splits > 1) e = join<true>(a, rows, s);
   return e;
 }
 

@@ -56,6 +56,8 @@ struct AttnArgs {
   int cus;
   int by_seq;             // fp's rows: see few_part
   AttnParts fp, tp;       // of the two kernels, where they take ranges
+  const int* selected;    // pages of each token and kv head, `count` numbers; or NULL
+  int count;
 };
 
 // The new tokens of a sequence and what it holds (both at least 0).
@@ -365,11 +367,19 @@ struct Rows {
 
   // `src`: the row's q, or NULL.  Rows are scaled by a power of two to at most 2^15.
   __device__ __forceinline__ void init(const float* src, int D, float scale, bool pairs = false) {
+    init_of(src, D, scale, [&](int s) __attribute__((always_inline)) {
+      return pairs ? element<true>(s) : element<false>(s);
+    });
+  }
+
+  // first(s): of the lane's elements of step s.
+  template <typename F>
+  __device__ __forceinline__ void init_of(const float* src, int D, float scale, F&& first) {
     float x[kSteps][8];
     uint32_t mb = 0;
 #pragma unroll
     for (int s = 0; s < kSteps; s++) {
-      const int d = pairs ? element<true>(s) : element<false>(s);
+      const int d = first(s);
 #pragma unroll
       for (int j = 0; j < 8; j++) x[s][j] = 0.0f;
       if (src && d < D) {
@@ -426,9 +436,10 @@ struct Rows {
   }
 
   // Scores times the keys' scales (8-bit keys: `ks`, the tile's in LDS), -inf where a
-  // key is not seen (kMask: those outside [lo, hi], relative to the tile), and the
-  // running maximum; o and the sum go down where it went up.
-  template <bool kMask>
+  // key is not seen (kMask 1: those outside [lo, hi], relative to the tile; 2: of two
+  // runs of 16 keys those from lo and hi on), and the running maximum; o and the sum go
+  // down where it went up.
+  template <int kMask>
   __device__ __forceinline__ void maximum(acc (&s)[BK / NQ], int lo, int hi, const float* ks) {
     constexpr int kPer = kAcc / 4;  // quads of one accumulator
     const int grp = (threadIdx.x & 63) / NQ;
@@ -443,7 +454,8 @@ struct Rows {
         float x = s[u / kPer][u % kPer * 4 + r];
         if (kType == kKvInt8) x *= k4[r];
         const int key = 4 * NG * u + r;
-        if (kMask) x = key < l0 || key > h0 ? -__builtin_inff() : x;
+        if (kMask == 1) x = key < l0 || key > h0 ? -__builtin_inff() : x;
+        if (kMask == 2) x = r >= (u ? h0 : l0) ? -__builtin_inff() : x;
         s[u / kPer][u % kPer * 4 + r] = x;
         mx = fmaxf(mx, x);
       }
@@ -569,5 +581,6 @@ __device__ __forceinline__ u32x4 fp4_to_f16(uint32_t x, half2v scale) {
 // Launchers of the kernels' files.
 hipError_t launch_attn_tile(const AttnArgs& a, hipStream_t s);
 hipError_t launch_attn_few(const AttnArgs& a, hipStream_t s);
+hipError_t launch_attn_few4(const AttnArgs& a, hipStream_t s);  // (4-bit caches)
 
 }  // namespace hypno

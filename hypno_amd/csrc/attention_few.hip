@@ -15,18 +15,18 @@
 //    for one token over 700 (32/4 heads of 64), most of it latency: the sequence's
 //    place, its pages, three tiles one after the other, the waves' sum.
 
-#include "attention.hpp"
+#include "attention_few.hpp"
 
 namespace hypno {
 
 namespace {
 
-constexpr int kQ = kFewRows;
+constexpr int kQ = kFewQ;
 typedef uint32_t u32x4a8 __attribute__((ext_vector_type(4), aligned(8)));
 
 template <int kType, int DP>
 struct Few {
-  static constexpr int kKeys = 32;
+  static constexpr int kKeys = kFewKeys;
   static constexpr int kGroups = DP > 128 ? 1 : 2;  // a CU
   static constexpr int kRuns = kKeys / kRun;
   static constexpr int kBytes = kKeys * DP * 2;        // V of one tile in LDS
@@ -34,13 +34,14 @@ struct Few {
   static constexpr int kBufs = kType == kKvFp16 ? 2 : 1;
   // Per wave: V, 8-bit: scales of K and V; afterwards o of 16 rows, maxima and sums.
   static constexpr int kStage = kBufs * kBytes + (kType == kKvInt8 ? 2 * kKeys * 4 : 0);
-  static constexpr int kOut = kQ * (DP + 4) * 4 + kQ * 8;
+  static constexpr int kOut = few_part_bytes<DP>();
   static constexpr int kWave = kStage > kOut ? kStage : kOut;
 };
 
 // kOne: pages have kRun positions or more.  kWaves: 4, or 8 where a work-group takes all
-// positions and these are few: half the tiles one after the other.
-template <int kType, int DP, bool kOne, int kWaves>
+// positions and these are few: half the tiles one after the other.  kList: a work-group
+// takes one token and the pages selected for it, whose positions it counts page after page.
+template <int kType, int DP, bool kOne, int kWaves, bool kList>
 __global__ void __launch_bounds__(64 * kWaves, (kWaves == 8 ? 1 : Few<kType, DP>::kGroups))
     attn_few_kernel(AttnArgs a) {
   typedef Few<kType, DP> T;
@@ -49,14 +50,21 @@ __global__ void __launch_bounds__(64 * kWaves, (kWaves == 8 ? 1 : Few<kType, DP>
   typedef Rows<kType, kQ, DP, kKeys> R;
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   __shared__ uint32_t again;
+  __shared__ int counts[kWaves];
+  static_assert(kOne || !kList, "selected pages have kRun positions or more");
+  SeenPage* const list = reinterpret_cast<SeenPage*>(smem + kWaves * T::kWave);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int KV = a.c.kv_heads, G = a.group, D = a.c.head_dim;
   // The kv head goes fastest and the range slowest: the last ranges, which the shorter
   // sequences do not have, come last.
-  const int g = blockIdx.x % KV, split = blockIdx.x / KV / a.b.batch;
-  const Seq sq = seq_of(a.b, blockIdx.x / KV % a.b.batch);
-  const int rows = sq.n * G, b = sq.b;
-  if (rows > a.few) return;
+  const int units = kList ? a.b.tokens : a.b.batch;
+  const int g = blockIdx.x % KV, split = blockIdx.x / KV / units;
+  const int unit = blockIdx.x / KV % units, b = kList ? find_seq(a.b, unit, 0, 0) : unit;
+  if (kList && (b < 0 || b >= a.b.batch)) return;
+  const Seq sq = seq_of(a.b, b);
+  const int ti0 = kList ? unit - sq.first : 0;  // (the token in its sequence)
+  const int rows = kList ? G : sq.n * G;
+  if (!kList && rows > a.few) return;
   const bool past = too_long(a, sq);
   const int col = lane % kQ;
   uint8_t* const vbuf = smem + wave * T::kWave;
@@ -83,18 +91,26 @@ __global__ void __launch_bounds__(64 * kWaves, (kWaves == 8 ? 1 : Few<kType, DP>
     vcol[i] = c < D ? c : 0;
   }
 
+  int seen = 0;  // positions of the pages in `list`
+  if (kList && !past) {
+    const int* const selected = a.selected + ((size_t)unit * KV + g) * a.count;
+    seen = seen_pages(a, b, sq.kv - sq.n + ti0, selected, list, counts) << a.c.page_shift;
+  }
   for (int r0 = 0; r0 < rows; r0 += kQ) {
     const int r1 = min(r0 + kQ, rows);
-    const Span span = span_of(a, sq, r0, r1);
+    const Span span = kList ? Span{0, seen} : span_of(a, sq, r0, r1);
     int lo = past ? 0 : span.lo, hi = past ? 0 : span.hi;
-    if (a.fs.splits > 1) {
+    if (kList) {
+      lo = (int)min((int64_t)split * a.fs.chunk, (int64_t)hi);
+      hi = (int)min((int64_t)hi, (int64_t)lo + a.fs.chunk);
+    } else if (a.fs.splits > 1) {
       const int64_t start = lo + (int64_t)split * a.fs.chunk;
       if (start >= hi && split) continue;
       if (split + 1 < a.fs.splits) hi = (int)min((int64_t)hi, start + a.fs.chunk);
       lo = (int)start;
     }
     const int row = min(r0 + col, rows - 1);
-    const int ti = row / G, h = g * G + row % G;
+    const int ti = kList ? ti0 : row / G, h = g * G + (kList ? row : row % G);
     const int t = sq.first + ti;
     const int seen_lo = first_seen(a, sq, ti), seen_hi = min(sq.kv - sq.n + ti, hi - 1);
     const int all_lo = first_seen(a, sq, (r1 - 1) / G);
@@ -102,11 +118,13 @@ __global__ void __launch_bounds__(64 * kWaves, (kWaves == 8 ? 1 : Few<kType, DP>
     bool bad = false;
     // Pages of the next tile's keys: kOne: of its runs; else the lane's.
     int pid[kRuns] = {};
+    int now[kRuns] = {}, then[kRuns] = {};  // kList: positions of the runs that are seen
     half8 kf[kRuns][R::kSteps];     // K of the next tile: keys 16 i + col, columns kcol
     uint2 kc[kRuns][R::kSteps], vc[T::kN];  // 8-bit: its codes, and V's
     float kss = 0.0f, vss = 0.0f;
     auto look_up = [&](int p0) __attribute__((always_inline)) {
-      if (kOne) {
+      if (kList) {
+      } else if (kOne) {
 #pragma unroll
         for (int i = 0; i < kRuns; i++)
           pid[i] = load_const<int>(a.b.page_table + (size_t)b * a.b.width +
@@ -116,11 +134,16 @@ __global__ void __launch_bounds__(64 * kWaves, (kWaves == 8 ? 1 : Few<kType, DP>
       }
     };
     auto issue = [&](int p0, int buf) __attribute__((always_inline)) {
-      int pg[kRuns] = {};
+      int pg[kRuns] = {}, slot0[kRuns], last0[kRuns];
 #pragma unroll
       for (int i = 0; i < kRuns; i++) {
         // (kOne: a run past the end is the last one again, rows past it the last row)
-        const int start = min(p0 + kRun * i, (hi - 1) & -kRun), last = hi - 1 - start;
+        int start = min(p0 + kRun * i, (hi - 1) & -kRun), last = hi - 1 - start;
+        if (kList) {
+          const SeenRun run = seen_run(a, list, start);
+          pid[i] = run.page, slot0[i] = start = run.slot, last0[i] = last = run.last;
+          then[i] = p0 + kRun * i < hi ? run.seen : 0;
+        }
         if (kOne) pg[i] = __builtin_amdgcn_readfirstlane(page_of(a, pid[i], bad));
         {
           const uint8_t* src;
@@ -182,7 +205,14 @@ __global__ void __launch_bounds__(64 * kWaves, (kWaves == 8 ? 1 : Few<kType, DP>
 #pragma unroll
           for (int i = 1; i < kRuns; i++) page = lane % kKeys / kRun == i ? pg[i] : page;
         }
-        const size_t tok = ((size_t)g << a.c.page_shift) + (min(p0 + lane % kKeys, hi - 1) & mask);
+        int slot = min(p0 + lane % kKeys, hi - 1) & mask;
+        if (kList) {
+          slot = slot0[0] + min(lane % kRun, last0[0]);
+#pragma unroll
+          for (int i = 1; i < kRuns; i++)
+            slot = lane % kKeys / kRun == i ? slot0[i] + min(lane % kRun, last0[i]) : slot;
+        }
+        const size_t tok = ((size_t)g << a.c.page_shift) + slot;
         kss = load_global<float>(a.c.k_scale + (size_t)page * a.c.ks_page + tok);
         vss = load_global<float>(a.c.v_scale + (size_t)page * a.c.vs_page + tok);
       }
@@ -206,6 +236,8 @@ __global__ void __launch_bounds__(64 * kWaves, (kWaves == 8 ? 1 : Few<kType, DP>
         }
       };
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+      for (int i = 0; i < kRuns; i++) now[i] = then[i];
       if (kType == kKvFp16) {
         half8 k[kRuns][R::kSteps];
 #pragma unroll
@@ -227,85 +259,46 @@ __global__ void __launch_bounds__(64 * kWaves, (kWaves == 8 ? 1 : Few<kType, DP>
         });
         next();
       }
-      if (p0 < all_lo || p0 + kKeys - 1 > all_hi)
-        x.template maximum<true>(s, seen_lo - p0, seen_hi - p0, ks);
-      else
-        x.template maximum<false>(s, 0, 0, ks);
+      if (kList) {
+        if (now[0] < kRun || now[1] < kRun)
+          x.template maximum<2>(s, now[0], now[1], ks);
+        else
+          x.template maximum<0>(s, 0, 0, ks);
+      } else if (p0 < all_lo || p0 + kKeys - 1 > all_hi) {
+        x.template maximum<1>(s, seen_lo - p0, seen_hi - p0, ks);
+      } else {
+        x.template maximum<0>(s, 0, 0, ks);
+      }
       x.values(s, vbuf + buf * T::kBytes, vs);
     }
     x.finish(__any(bad));
 
-    // The waves' parts, then their sum: thread (row, piece) takes four elements.
-    float* const part = reinterpret_cast<float*>(vbuf);
-    float2* const ml = reinterpret_cast<float2*>(part + kQ * (DP + 4));
-#pragma unroll
-    for (int k = 0; k < R::kDt; k++)
-      *reinterpret_cast<f32x4*>(part + col * (DP + 4) + R::dim(k, 0)) =
-          f32x4{x.o[k][0], x.o[k][1], x.o[k][2], x.o[k][3]};
-    if (lane < kQ) ml[col] = make_float2(x.m, x.l);
-    if (tid == 0) again = 0;
-    __syncthreads();
-    const int or_ = tid / (4 * kWaves), piece = tid % (4 * kWaves);
-    float w[kWaves], m = -__builtin_inff(), l = 0.0f;
-    auto row_of = [&](int i) { return reinterpret_cast<const float*>(smem + i * T::kWave) + or_ * (DP + 4); };
-    auto ml_of = [&](int i) {
-      return reinterpret_cast<const float2*>(smem + i * T::kWave + kQ * (DP + 4) * 4)[or_];
-    };
-#pragma unroll
-    for (int i = 0; i < kWaves; i++) {
-      w[i] = ml_of(i).x;
-      m = fmaxf(m, w[i]);
-    }
-#pragma unroll
-    for (int i = 0; i < kWaves; i++) {
-      w[i] = w[i] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(w[i] - m);
-      l += ml_of(i).y * w[i];
-    }
-    const bool live = r0 + or_ < rows;
-    const int rr = min(r0 + or_, rows - 1);
-    const size_t orow = (size_t)(sq.first + rr / G) * a.heads + g * G + rr % G;
-    const size_t prow = few_part(a, sq, g, rr, orow) * a.fs.splits + split;
-    const bool parts = a.fs.splits > 1;
-    const float inv = parts ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
-    float* const dst = parts ? a.fp.o + prow * D : a.out + orow * D;
-    float z = l * 0.0f;
-    if (live) {
-      for (int d = 4 * piece; d < D; d += 16 * kWaves) {
-        f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int i = 0; i < kWaves; i++)
-          v += *reinterpret_cast<const f32x4*>(row_of(i) + d) * w[i];
-        v *= inv;
-#pragma unroll
-        for (int j = 0; j < 4; j++) z += v[j] * 0.0f;
-        *reinterpret_cast<f32x4*>(dst + d) = v;
-      }
-      if (parts && piece == 0) a.fp.ml[prow] = make_float2(m, l);
-      if (!parts && (!(z == 0.0f) || past)) atomicOr(&again, 1u << or_);
-    }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (!parts)
-      attn_rows(a, sq, g, r0, again & ((kWaves == 8 ? 0x0101u : 0x1111u) << wave));
-    __syncthreads();
+    few_store<DP, kWaves, T::kWave, kList>(a, sq, g, ti0, r0, rows, split, past, x, smem, again);
   }
 }
 
-template <int kType, int DP, bool kOne, int kWaves>
+template <int kType, int DP, bool kOne, int kWaves, bool kList = false>
 hipError_t launch(const AttnArgs& a, hipStream_t s) {
-  constexpr int kLds = kWaves * Few<kType, DP>::kWave;
-  const size_t grid = (size_t)a.b.batch * a.c.kv_heads * a.fs.splits;
+  const int lds = kWaves * Few<kType, DP>::kWave + (kList ? a.count * (int)sizeof(SeenPage) : 0);
+  const size_t units = kList ? a.b.tokens : a.b.batch;
+  const size_t grid = units * a.c.kv_heads * a.fs.splits;
   if (grid > 0xFFFFFF) return hipErrorInvalidValue;
-  const void* kernel = (const void*)attn_few_kernel<kType, DP, kOne, kWaves>;
-  const hipError_t e = set_lds_limit(kernel, kLds);
+  const void* kernel = (const void*)attn_few_kernel<kType, DP, kOne, kWaves, kList>;
+  const hipError_t e = set_lds_limit(kernel, lds);
   if (e != hipSuccess) return e;
-  attn_few_kernel<kType, DP, kOne, kWaves><<<(unsigned)grid, 64 * kWaves, kLds, s>>>(a);
+  attn_few_kernel<kType, DP, kOne, kWaves, kList><<<(unsigned)grid, 64 * kWaves, lds, s>>>(a);
   return hipGetLastError();
 }
 
 template <int kType, int DP>
 hipError_t run(const AttnArgs& a, hipStream_t s) {
   const bool one = a.c.page_shift >= kRunShift;
+  if (a.selected) {
+    if constexpr (DP <= 128) {
+      if (a.few_waves == 8) return launch<kType, DP, true, 8, true>(a, s);
+    }
+    return launch<kType, DP, true, 4, true>(a, s);
+  }
   if constexpr (DP <= 128) {
     if (a.few_waves == 8)
       return one ? launch<kType, DP, true, 8>(a, s) : launch<kType, DP, false, 8>(a, s);
@@ -317,6 +310,7 @@ hipError_t run(const AttnArgs& a, hipStream_t s) {
 
 hipError_t launch_attn_few(const AttnArgs& a, hipStream_t s) {
   const int D = a.c.head_dim;
+  if (a.c.dtype == kKvFp4) return launch_attn_few4(a, s);
   if (a.c.dtype == kKvFp16)
     return D <= 64    ? run<kKvFp16, 64>(a, s)
            : D <= 96  ? run<kKvFp16, 96>(a, s)

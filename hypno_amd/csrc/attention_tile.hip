@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(256, 2) attn_tile_kernel(AttnArgs a) {
         return *reinterpret_cast<const half8*>(kt + L::at(r, R::NG * st + lane / NQ));
       });
       const float* ks = scales + buf * 2 * BK;
-      x.template maximum<masked>(s, seen_lo - p0, seen_hi - p0, ks);
+      x.template maximum<masked ? 1 : 0>(s, seen_lo - p0, seen_hi - p0, ks);
       x.values(s, vbuf + buf * T::kBytes, ks + BK);
     }
     if (kType == kKvFp16)

@@ -160,8 +160,10 @@ __global__ void __launch_bounds__(kAppendThreads) append_kv_kernel(AppendArgs a)
         const float sf = (float)s;
         uint32_t p = 0;
         if (sf > 0.0f) {
+          float y[8];
 #pragma unroll
-          for (int i = 0; i < 8; i++) p |= fp4_code(x[i] / sf) << 4 * i;
+          for (int i = 0; i < 8; i++) y[i] = x[i] / sf;
+          p = fp4_codes(y);
         }
         uint8_t* dst = (is_k ? (uint8_t*)a.c.k + (size_t)page * a.c.k_page
                              : (uint8_t*)a.c.v + (size_t)page * a.c.v_page) + (tok * D + e0) / 2;

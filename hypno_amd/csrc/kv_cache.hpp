@@ -36,12 +36,13 @@ __device__ __forceinline__ _Float16 fp4_value(uint32_t code) {
   return __builtin_bit_cast(_Float16, bits) * (_Float16)16384.0f;
 }
 
-// The code of y: the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6, halves to the even code.
-__device__ __forceinline__ uint32_t fp4_code(float y) {
-  const float a = fabsf(y);
-  const uint32_t c = (a > 0.25f) + (a >= 0.75f) + (a > 1.25f) + (a >= 1.75f) + (a > 2.5f) +
-                     (a >= 3.5f) + (a > 5.0f);
-  return c | (__float_as_uint(y) >> 28 & 8);
+// The codes of eight finite values: the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 and their
+// negatives, halves to the even code (the conversion's own rounding).
+__device__ __forceinline__ uint32_t fp4_codes(const float (&y)[8]) {
+  uint32_t p = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, y[0], y[1], 1.0f, 0);
+  p = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(p, y[2], y[3], 1.0f, 1);
+  p = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(p, y[4], y[5], 1.0f, 2);
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(p, y[6], y[7], 1.0f, 3);
 }
 
 // Sequence b brings the tokens [cu_q[b], cu_q[b + 1]) of `tokens`, the last ones
@@ -105,10 +106,6 @@ hipError_t launch_key_bounds(const KeyBounds& o, const KvCache& c, const KvBatch
 hipError_t launch_select_pages(int* out, int count, int first, int last, const float* q,
                                size_t q_stride, int heads, const KeyBounds& k, const KvBatch& b,
                                int pages, int num_cus, hipStream_t s);
-hipError_t launch_selected_attention(float* out, const float* q, size_t q_stride, int heads,
-                                     const KvCache& c, const KvBatch& b, float scale,
-                                     const int* selected, int count, hipStream_t s);
-
 // How the positions of a tile of rows are split: into ranges of `chunk`, the last
 // one of `splits` taking what is left.
 struct AttnSplit {
@@ -127,6 +124,17 @@ struct AttnPlan {
   size_t few_places, tile_places;
   bool by_seq;    // attn_few_kernel's rows are counted by sequence, not by token
 };
+// The same for a token's selected pages, whose positions are counted page after page.
+struct SelectedPlan {
+  int waves;  // of a work-group
+  AttnSplit fs;
+  size_t bytes, ml_bytes;
+};
+SelectedPlan selected_plan(const KvCache& c, const KvBatch& b, int heads, int count, int num_cus);
+hipError_t launch_selected_attention(const SelectedPlan& p, float* out, const float* q,
+                                     size_t q_stride, int heads, const KvCache& c,
+                                     const KvBatch& b, float scale, const int* selected, int count,
+                                     void* ws, hipStream_t s);
 AttnPlan attn_plan(const KvCache& c, const KvBatch& b, int heads, int window, int64_t max_kv,
                    int num_cus);
 // ws: plan.bytes, 256-byte aligned, or NULL (no range is split then).
