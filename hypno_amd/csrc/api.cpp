@@ -815,6 +815,10 @@ int kv_args(const char* what, const hypno_hip_kv_cache* c, const hypno_hip_kv_ba
               c->v_scale_page_stride % 8))
     return fail(HYPNO_HIP_EINVAL, "%s: page strides of a 4-bit cache must be multiples of 16, "
                 "of its scales of 8", what);
+  // (its kernels multiply page numbers and strides of 32 bits)
+  if (fp4 && std::max(std::max(kc->k_page, kc->v_page), std::max(kc->ks_page, kc->vs_page)) >
+                 kMaxInt)
+    return fail(HYPNO_HIP_EINVAL, "%s: page strides of a 4-bit cache above 2^31", what);
   if (c->k_page_stride % 8 || c->v_page_stride % 8)
     return fail(HYPNO_HIP_EINVAL, "%s: page strides of k and v must be multiples of 8", what);
   if (mul_overflows(c->pages, 4 * std::max(std::max(kc->k_page, kc->v_page),

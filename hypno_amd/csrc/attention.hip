@@ -2,6 +2,7 @@
 // a call takes, and the sum of what a row's ranges of positions gave (5.6 us for 64 ranges
 // of 32 rows, 15 for four of 16384, 42 MB: 2.8 TB/s).
 #include <cmath>
+#include <cstdlib>
 
 #include "attention.hpp"
 
@@ -181,7 +182,8 @@ AttnPlan attn_plan(const KvCache& c, const KvBatch& b, int heads, int window, in
       // (whole steps of four waves: a run of positions must not lie across two ranges)
       const int64_t fit = (seen + most(few_rows) - 1) / most(few_rows);
       const int64_t chunk = (std::max({least, (int64_t)best, fit}) + 127) / 128 * 128;
-      p.fs.splits = up(seen, chunk);
+      if (getenv("HK_CHUNK")) { const int64_t ch = atoi(getenv("HK_CHUNK")); p.fs = {up(seen, ch), (int)ch}; } else
+      p.fs.splits = up(seen, chunk),
       p.fs.chunk = (int)std::min<int64_t>(chunk, 0x7FFFFFFF);
     } else if (pairs <= num_cus && seen > 128) {
       p.few_waves = 8;
@@ -256,6 +258,7 @@ SelectedPlan selected_plan(const KvCache& c, const KvBatch& b, int heads, int co
     const int64_t splits = std::min(slots / pairs, most);
     const int64_t chunk = (std::max<int64_t>(256, up(positions, splits)) + 127) / 128 * 128;
     p.fs = {up(positions, chunk), (int)chunk};
+    if (getenv("HK_CHUNK")) { const int64_t ch = atoi(getenv("HK_CHUNK")); p.fs = {up(positions, ch), (int)ch}; }
   } else if (pairs <= num_cus && positions > 128) {
     p.waves = 8;
   }

@@ -67,9 +67,10 @@ struct Seq {
 
 // (the same in all lanes)
 __device__ __forceinline__ Seq seq_of(const KvBatch& b, int i) {
-  const int first = __builtin_amdgcn_readfirstlane(cu_at(b, i));
-  const int end = __builtin_amdgcn_readfirstlane(cu_at(b, i + 1));
-  const int kv = __builtin_amdgcn_readfirstlane(load_global<int>(b.kv_lens + i));
+  i = __builtin_amdgcn_readfirstlane(i);
+  const int first = min(max(load_const<int>(b.cu_q + i), 0), b.tokens);
+  const int end = min(max(load_const<int>(b.cu_q + i + 1), 0), b.tokens);
+  const int kv = load_const<int>(b.kv_lens + i);
   return {i, first, max(end - first, 0), max(kv, 0)};
 }
 
@@ -86,16 +87,17 @@ __device__ __forceinline__ int first_seen(const AttnArgs& a, const Seq& s, int i
 // A run of kRun positions from a multiple of it lies in one page, if pages have as many.
 constexpr int kRunShift = 4, kRun = 1 << kRunShift;
 
-// Positions that the rows [r0, r1) of a sequence read, from the start of a run (of the
-// page's start, where pages are shorter): those before the first that is seen are in its
-// page.
+// Positions that the rows [r0, r1) of a sequence read, from the start of a run (of two in
+// 4-bit caches; of the page, where pages are shorter): those before the first that is seen
+// are in its page.
 struct Span {
   int lo, hi;
 };
 __device__ __forceinline__ Span span_of(const AttnArgs& a, const Seq& s, int r0, int r1) {
   const int lo = first_seen(a, s, r0 / a.group), hi = s.kv - s.n + (r1 - 1) / a.group + 1;
   if (hi <= lo) return {0, 0};
-  return {lo & -(1 << min(a.c.page_shift, kRunShift)), hi};
+  const int shift = a.c.dtype == kKvFp4 ? kRunShift + 1 : kRunShift;
+  return {lo & -(1 << min(a.c.page_shift, shift)), hi};
 }
 
 // Ranges that a span is split into (0: nothing is seen).

@@ -50,18 +50,19 @@ __device__ __forceinline__ int seen_pages(const AttnArgs& a, int b, int pos, con
   return __builtin_amdgcn_readfirstlane(n);
 }
 
-// A run of kRun positions in a selected page, or where the page ends before it, the last one
-// that is seen: its first slot, and the last of its positions that is seen.
+// A run of kLen positions in a selected page, or where what is seen of it ends before, its last
+// one that is seen: its first slot, and the last of its positions that is seen.
 struct SeenRun {
   int page, slot, last;
-  int seen;  // positions of the run that was asked for that are seen (0 to kRun)
+  int seen;  // positions of the run that was asked for that are seen (0 to kLen)
 };
+template <int kLen = kRun>
 __device__ __forceinline__ SeenRun seen_run(const AttnArgs& a, const SeenPage* list, int p) {
   const SeenPage x = list[p >> a.c.page_shift];
   const int page = __builtin_amdgcn_readfirstlane(x.page);
   const int end = __builtin_amdgcn_readfirstlane(x.seen);
-  const int slot = p & ((1 << a.c.page_shift) - 1), start = min(slot, (end - 1) & -kRun);
-  return {page, start, min(end - 1 - start, kRun - 1), min(max(end - slot, 0), kRun)};
+  const int slot = p & ((1 << a.c.page_shift) - 1), start = min(slot, (end - 1) & -kLen);
+  return {page, start, min(end - 1 - start, kLen - 1), min(max(end - slot, 0), kLen)};
 }
 
 // Bits of the kFewQ rows that wave `wave` computes again, where that is needed.
@@ -128,9 +129,12 @@ __device__ __forceinline__ void few_store(const AttnArgs& a, const Seq& sq, int 
     if (parts && piece == 0) a.fp.ml[prow] = make_float2(m, l);
     if (!parts && (!(z == 0.0f) || past)) atomicOr(&again, 1u << or_);
   }
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  // (rows again after all that is stored of them)
+  if (parts && r0 + kFewQ >= rows) return;
   __syncthreads();
-  if (!parts) {
+  if (again) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
     uint32_t left = again & again_mask<kWaves>(wave);
     if (kList) {
       const int* const selected =
@@ -141,7 +145,7 @@ __device__ __forceinline__ void few_store(const AttnArgs& a, const Seq& sq, int 
       attn_rows(a, sq, g, r0, left);
     }
   }
-  __syncthreads();
+  if (r0 + kFewQ < rows) __syncthreads();
 }
 
 }  // namespace hypno

@@ -16,15 +16,18 @@ namespace hypno {
 
 namespace {
 
-constexpr int kQ = kFewQ, kKeys = kFewKeys, kRuns = kKeys / kRun;
+constexpr int kQ = kFewQ, kKeys = kFewKeys;
 
-template <int DP>
+// kLen: keys of a tile in one page, the whole tile's where pages have as many.
+template <int DP, int kLen>
 struct Few4 {
-  static constexpr int kAhead = DP > 128 ? 2 : 3;
-  static constexpr int kCopies = DP > 128 ? 2 : 1;  // instructions of a run's codes
-  static constexpr int kCodes = kRun * DP / 2, kScales = kRun * DP / kFp4Group * 2;  // of a run
+  static constexpr int kAhead = 1;
+  static constexpr int kRuns = kKeys / kLen;
+  // Bytes of a run, and instructions that copy them, 16 and 4 bytes a lane.
+  static constexpr int kCodes = kLen * DP / 2, kScales = kLen * DP / kFp4Group * 2;
+  static constexpr int kCodeCopies = (kCodes + 1023) / 1024, kScaleCopies = (kScales + 255) / 256;
   static constexpr int kTile = 2 * kRuns * (kCodes + kScales);
-  static constexpr int kLoads = 2 * kRuns * (kCopies + 1);
+  static constexpr int kLoads = 2 * kRuns * (kCodeCopies + kScaleCopies);
   static constexpr int kStage = (kAhead + 1) * kTile;
   static constexpr int kWave = kStage > few_part_bytes<DP>() ? kStage : few_part_bytes<DP>();
 };
@@ -47,10 +50,11 @@ __device__ __forceinline__ void wait_loads() {
 #endif
 }
 
-template <int DP, int kWaves, bool kList>
-__global__ void __launch_bounds__(64 * kWaves, kWaves == 8 ? 1 : DP > 128 ? 1 : 2)
+template <int DP, int kLen, int kWaves, bool kList>
+__global__ void __launch_bounds__(64 * kWaves, kWaves == 8 ? 1 : DP > 128 ? 1 : 3)
     attn_few4_kernel(AttnArgs a) {
-  typedef Few4<DP> T;
+  typedef Few4<DP, kLen> T;
+  constexpr int kRuns = T::kRuns;
   typedef Rows<kKvFp16, kQ, DP, kKeys> R;
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   __shared__ uint32_t again;
@@ -83,11 +87,19 @@ __global__ void __launch_bounds__(64 * kWaves, kWaves == 8 ? 1 : DP > 128 ? 1 : 
   uint8_t* const ring = smem + wave * T::kWave;
   // In a tile: K's codes run by run [16][D / 2], V's, K's scales run by run [B][16], V's.
   constexpr int kV = kRuns * T::kCodes, kKs = 2 * kV, kVs = kKs + kRuns * T::kScales;
-  const int pieces = D / 2;  // of 16 bytes, of a run's codes
-  const uint32_t scale_off = (((lane / 8) << shift) * 2) + lane % 8 * 4;
+  const bool same = a.c.k_page == a.c.v_page && a.c.ks_page == a.c.vs_page;
+  const int row_bytes = D / 2;
+  const int* const table = a.b.page_table + (size_t)b * a.b.width;
+  // Where the codes and scales of a tile's first and second 16 keys are.
+  auto codes_of = [&](int half) __attribute__((always_inline)) {
+    return half * 16 * (kLen == 16 ? DP / 2 : row_bytes);
+  };
+  auto scales_of = [&](int half) __attribute__((always_inline)) {
+    return half * (kLen == 16 ? T::kScales : 32);
+  };
   // A lane's first element of step s of a score's sum: quarter by quarter of each 128.
   constexpr int kPart = DP / 4 < 32 ? DP / 4 : 32;
-  const auto element = [&](int s) __attribute__((always_inline)) {
+  auto element = [&](int s) __attribute__((always_inline)) {
     return 8 * s / kPart * 4 * kPart + kPart * grp + 8 * s % kPart;
   };
 
@@ -110,24 +122,24 @@ __global__ void __launch_bounds__(64 * kWaves, kWaves == 8 ? 1 : DP > 128 ? 1 : 
     const int seen_lo = first_seen(a, sq, ti), seen_hi = min(sq.kv - sq.n + ti, hi - 1);
     const int all_lo = first_seen(a, sq, (r1 - 1) / G);
     const int all_hi = min(sq.kv - sq.n + r0 / G, hi - 1);
-    bool bad = false;
-    // Run i of the tile at p0: its page (-1: none), first slot, and the positions of it that
-    // are there to be seen (0: it is another run again).
+    // Run i of a tile: its page (-1: none), first slot, and the positions of it that are there
+    // to be seen (0: it is another run again).
     int pid[kRuns] = {}, slot[kRuns] = {};
+    uint32_t bad = 0;
     const int tiles = (hi - lo + kKeys - 1) / kKeys;
-    const int mine = max(0, (tiles - wave + kWaves - 1) / kWaves);
-    auto place = [&](int p0, int i) __attribute__((always_inline)) {
-      return lo + (p0 * kWaves + wave) * kKeys + kRun * i;  // (p0: the wave's tile)
+    const int mine = max(0, (tiles - wave + kWaves - 1) / kWaves);  // this wave's
+    auto place = [&](int tile) __attribute__((always_inline)) {
+      return lo + (tile * kWaves + wave) * kKeys;
     };
     auto look_up = [&](int tile) __attribute__((always_inline)) {
 #pragma unroll
       for (int i = 0; i < kRuns; i++) {
-        const int p = min(place(tile, i), (hi - 1) & -kRun);
+        const int p = min(place(tile) + kLen * i, (hi - 1) & -kLen);
         if (kList) {
-          const SeenRun run = seen_run(a, list, p);
+          const SeenRun run = seen_run<kLen>(a, list, p);
           pid[i] = run.page, slot[i] = run.slot;
         } else {
-          pid[i] = load_const<int>(a.b.page_table + (size_t)b * a.b.width + (p >> shift));
+          pid[i] = load_const<int>(table + (p >> shift));
           slot[i] = p & mask;
         }
       }
@@ -135,21 +147,38 @@ __global__ void __launch_bounds__(64 * kWaves, kWaves == 8 ? 1 : DP > 128 ? 1 : 
     auto issue = [&](uint8_t* to) __attribute__((always_inline)) {
 #pragma unroll
       for (int i = 0; i < kRuns; i++) {
-        const int pg = __builtin_amdgcn_readfirstlane(page_of(a, pid[i], bad));
-        const uint8_t* const kp = kg + (size_t)pg * a.c.k_page + (uint32_t)(slot[i] * pieces);
-        const uint8_t* const vp = vg + (size_t)pg * a.c.v_page + (uint32_t)(slot[i] * pieces);
-        const _Float16* const ksp = ksg + (size_t)pg * a.c.ks_page + slot[i];
-        const _Float16* const vsp = vsg + (size_t)pg * a.c.vs_page + slot[i];
-#pragma unroll
-        for (int c = 0; c < T::kCopies; c++)
-          if (c * 64 + lane < pieces) {
-            dma16<!kList>(kp, c * 1024 + lane * 16, to + i * T::kCodes + c * 1024);
-            dma16<!kList>(vp, c * 1024 + lane * 16, to + kV + i * T::kCodes + c * 1024);
-          }
-        if (lane < 8 * B) {
-          dma4(ksp, scale_off, to + kKs + i * T::kScales);
-          dma4(vsp, scale_off, to + kVs + i * T::kScales);
+        const bool none = (uint32_t)pid[i] >= (uint32_t)a.c.pages;
+        bad |= none;
+        const uint32_t pg = none ? 0 : pid[i], first = slot[i] * row_bytes;
+        // (strides are below 2^31; K's and V's are mostly the same)
+        const uint64_t ko = (uint64_t)pg * (uint32_t)a.c.k_page + first;
+        const uint64_t kso = (uint64_t)pg * (uint32_t)a.c.ks_page + slot[i];
+        uint64_t vo = ko, vso = kso;
+        if (!same) {
+          asm volatile("" ::: "memory");  // (not computed on every way)
+          vo = (uint64_t)pg * (uint32_t)a.c.v_page + first;
+          vso = (uint64_t)pg * (uint32_t)a.c.vs_page + slot[i];
         }
+        const uint8_t *const kp = kg + ko, *const vp = vg + vo;
+        const _Float16 *const ksp = ksg + kso, *const vsp = vsg + vso;
+        to += i * T::kCodes;
+#pragma unroll
+        for (int c = 0; c < T::kCodeCopies; c++)
+          if ((c * 64 + lane) * 16 < kLen * row_bytes) {
+            dma16<!kList>(kp, c * 1024 + lane * 16, to + c * 1024);
+            dma16<!kList>(vp, c * 1024 + lane * 16, to + kV + c * 1024);
+          }
+        to -= i * (T::kCodes - T::kScales);
+#pragma unroll
+        for (int c = 0; c < T::kScaleCopies; c++) {
+          const int j = c * 64 + lane, blk = j / (kLen / 2);
+          if (blk < B) {
+            const uint32_t off = ((blk << shift) + j % (kLen / 2) * 2) * 2;
+            dma4(ksp, off, to + kKs + c * 256);
+            dma4(vsp, off, to + kVs + c * 256);
+          }
+        }
+        to -= i * T::kScales;
       }
     };
 
@@ -167,76 +196,81 @@ __global__ void __launch_bounds__(64 * kWaves, kWaves == 8 ? 1 : DP > 128 ? 1 : 
     R x;
     x.init_of(r0 + col < rows ? a.q + (size_t)t * a.q_stride + (size_t)h * D : nullptr, D, a.scale,
               element);
-    if (mine < T::kAhead) to = ring + T::kAhead * T::kTile;  // (not used)
     const uint8_t* at = ring;
     for (int tile = 0; tile < mine; tile++) {
-      const int p0 = place(tile, 0);
+      const int p0 = place(tile);
       if (tile + T::kAhead <= mine)
         wait_loads<(T::kAhead - 1) * T::kLoads>();
       else
         wait_loads<0>();
-      if (tile + T::kAhead < mine) {
-        issue(to);
-        to = to == ring + T::kAhead * T::kTile ? ring : to + T::kTile;
-        look_up(tile + T::kAhead + 1);
-      }
       // Positions of the runs that are there to be seen, and the rest's scales of V: 0, as
       // the codes are finite and their weights 0.
       int there[kRuns];
       bool whole = true;
 #pragma unroll
       for (int i = 0; i < kRuns; i++) {
-        const int p = place(tile, i);
-        there[i] = p >= hi ? 0 : kList ? seen_run(a, list, p).seen : min(hi - p, kRun);
-        whole &= there[i] == kRun;
+        const int p = p0 + kLen * i;
+        there[i] = p >= hi ? 0 : kList ? seen_run<kLen>(a, list, p).seen : min(hi - p, kLen);
+        whole &= there[i] == kLen;
       }
       if (!whole) {
 #pragma unroll
         for (int i = 0; i < kRuns; i++)
-          for (int k = lane; k < B * kRun; k += 64)
-            if (k % kRun >= there[i])
+          for (int k = lane; k < B * kLen; k += 64)
+            if (k % kLen >= there[i])
               *reinterpret_cast<_Float16*>(const_cast<uint8_t*>(at) + kVs + i * T::kScales + k * 2) =
                   (_Float16)0.0f;
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       }
-
-      typename R::acc s[kRuns];
+      // All that this tile needs of LDS is on its way before the copies of a later one.
+      constexpr int kQuarters = DP / 4 / kPart;  // of a key's codes in a lane
+      typedef uint32_t codes_t __attribute__((ext_vector_type(kPart / 8)));
+      codes_t kc[2][kQuarters];
+      _Float16 ks[2][kQuarters];
 #pragma unroll
-      for (int i = 0; i < kRuns; i++) {
-        s[i] = typename R::acc{};
-        u32x4 k[R::kSteps];
+      for (int i = 0; i < 2; i++)
 #pragma unroll
-        for (int c = 0; c < DP / 4 / kPart; c++) {
+        for (int c = 0; c < kQuarters; c++) {
           const int e = c * 4 * kPart + kPart * grp, blk = e < D ? e / kFp4Group : 0;
-          const uint8_t* const src = at + i * T::kCodes + col * (D / 2) + (e < D ? e / 2 : 0);
-          const _Float16 sc = *reinterpret_cast<const _Float16*>(at + kKs + i * T::kScales +
-                                                                 (blk * kRun + col) * 2);
-          const half2v two = {sc, sc};
-          if constexpr (kPart == 32) {
-            const u32x4 codes = *reinterpret_cast<const u32x4*>(src);
-#pragma unroll
-            for (int j = 0; j < 4; j++) k[c * 4 + j] = fp4_to_f16(codes[j], two);
-          } else {
-            const uint2 codes = *reinterpret_cast<const uint2*>(src);
-            k[0] = fp4_to_f16(codes.x, two);
-            k[1] = fp4_to_f16(codes.y, two);
-          }
+          kc[i][c] = *reinterpret_cast<const codes_t*>(at + codes_of(i) + col * row_bytes +
+                                                       (e < D ? e / 2 : 0));
+          ks[i][c] = *reinterpret_cast<const _Float16*>(at + kKs + scales_of(i) +
+                                                        (blk * kLen + col) * 2);
         }
-#pragma unroll
-        for (int st = 0; st < R::kSteps; st++) s[i] = Mfma<kQ>::mul(f16x8(k[st]), x.qh[st], s[i]);
-#pragma unroll
-        for (int st = 0; st < R::kSteps; st++) s[i] = Mfma<kQ>::mul(f16x8(k[st]), x.ql[st], s[i]);
+      if (tile + T::kAhead < mine) {
+        issue(to);
+        to = to == ring + T::kAhead * T::kTile ? ring : to + T::kTile;
+        look_up(tile + T::kAhead + 1);
       }
-      if (kList) {
-        if (whole)
-          x.template maximum<0>(s, 0, 0, nullptr);
-        else
-          x.template maximum<2>(s, there[0], there[1], nullptr);
-      } else if (p0 < all_lo || p0 + kKeys - 1 > all_hi) {
-        x.template maximum<1>(s, seen_lo - p0, seen_hi - p0, nullptr);
-      } else {
-        x.template maximum<0>(s, 0, 0, nullptr);
+      typename R::acc s[2];
+#pragma unroll
+      for (int i = 0; i < 2; i++) s[i] = typename R::acc{};
+#pragma unroll
+      for (int st = 0; st < R::kSteps; st++) {
+        const int c = 8 * st / kPart;
+        half8 k[2];
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+          k[i] = f16x8(fp4_to_f16(kc[i][c][st % (kPart / 8)], half2v{ks[i][c], ks[i][c]}));
+#pragma unroll
+        for (int i = 0; i < 2; i++) s[i] = Mfma<kQ>::mul(k[i], x.qh[st], s[i]);
+#pragma unroll
+        for (int i = 0; i < 2; i++) s[i] = Mfma<kQ>::mul(k[i], x.ql[st], s[i]);
+        __builtin_amdgcn_sched_barrier(0);
       }
+      // Keys that a row does not see.  (Apart from the maximum: two ways to that one have the
+      // compiler copy all of o.)
+      if (kList ? !whole : p0 < all_lo || p0 + kKeys - 1 > all_hi) {
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+          for (int r = 0; r < 4; r++) {
+            const int key = 16 * i + 4 * grp + r, p = p0 + key;
+            if (kList ? key % kLen >= there[i / (kLen / 16)] : p < seen_lo || p > seen_hi)
+              s[i][r] = -__builtin_inff();
+          }
+      }
+      x.template maximum<0>(s, 0, 0, nullptr);
 
       // Weights, two fp16 parts each, in the order of V's keys: run by run four a lane.
       const float off = R::kTop - (x.m == -__builtin_inff() ? 0.0f : x.m);
@@ -255,22 +289,22 @@ __global__ void __launch_bounds__(64 * kWaves, kWaves == 8 ? 1 : DP > 128 ? 1 : 
         wh[i] = hi16, wl[i] = lo16;
       }
       x.l += sum;
-      // Channels 32 blk + col and 16 on, of keys 4 grp to 4 grp + 3 of both runs: row j of
-      // the transposed 16 x 16 codes is key j % 4 of run j / 4 % 2 and half j / 8.
-      const int j = lane % 16;
-      const uint8_t* const vsrc = at + kV + j / 4 % 2 * T::kCodes + (4 * grp + j % 4) * (D / 2) +
-                                  j / 8 * 8;
+      // Channels 32 blk + col and 16 on, of keys 4 grp to 4 grp + 3 of both halves of the tile:
+      // row j of the transposed 16 x 16 codes is key j % 4 of half j / 4 % 2, and from j = 8
+      // on 16 channels on.
+      const uint8_t* const vsrc = at + kV + codes_of(col / 4 % 2) + (4 * grp + col % 4) * row_bytes +
+                                  col / 8 * 8;
 #pragma unroll
       for (int blk = 0; blk < DP / kFp4Group; blk++) {
-        const int here = blk < B ? blk : 0;
+        // (past D: whatever is there, for channels that nobody reads)
         typedef int int2v __attribute__((ext_vector_type(2)));
         const auto codes = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
-            (__attribute__((address_space(3))) int2v*)(vsrc + here * 16));
-        uint2 sc[kRuns];
+            (__attribute__((address_space(3))) int2v*)(vsrc + blk * 16));
+        uint2 sc[2];
 #pragma unroll
-        for (int i = 0; i < kRuns; i++)
-          sc[i] = *reinterpret_cast<const uint2*>(at + kVs + i * T::kScales +
-                                                  (here * kRun + 4 * grp) * 2);
+        for (int i = 0; i < 2; i++)
+          sc[i] = *reinterpret_cast<const uint2*>(at + kVs + scales_of(i) +
+                                                  (blk * kLen + 4 * grp) * 2);
         const half2v scale[4] = {
             __builtin_bit_cast(half2v, sc[0].x), __builtin_bit_cast(half2v, sc[0].y),
             __builtin_bit_cast(half2v, sc[1].x), __builtin_bit_cast(half2v, sc[1].y)};
@@ -292,25 +326,27 @@ __global__ void __launch_bounds__(64 * kWaves, kWaves == 8 ? 1 : DP > 128 ? 1 : 
       }
       at = at == ring + T::kAhead * T::kTile ? ring : at + T::kTile;
     }
-    x.finish(__any(bad));
+    x.finish(bad != 0);
     few_store<DP, kWaves, T::kWave, kList>(a, sq, g, ti0, r0, rows, split, past, x, smem, again);
   }
 }
 
-template <int DP, int kWaves, bool kList>
+template <int DP, int kLen, int kWaves, bool kList>
 hipError_t launch(const AttnArgs& a, hipStream_t s) {
-  const int lds = kWaves * Few4<DP>::kWave + (kList ? a.count * (int)sizeof(SeenPage) : 0);
+  const int lds = kWaves * Few4<DP, kLen>::kWave + (kList ? a.count * (int)sizeof(SeenPage) : 0);
   const size_t grid = (size_t)(kList ? a.b.tokens : a.b.batch) * a.c.kv_heads * a.fs.splits;
   if (grid > 0xFFFFFF) return hipErrorInvalidValue;
-  const hipError_t e = set_lds_limit((const void*)attn_few4_kernel<DP, kWaves, kList>, lds);
+  const hipError_t e = set_lds_limit((const void*)attn_few4_kernel<DP, kLen, kWaves, kList>, lds);
   if (e != hipSuccess) return e;
-  attn_few4_kernel<DP, kWaves, kList><<<(unsigned)grid, 64 * kWaves, lds, s>>>(a);
+  attn_few4_kernel<DP, kLen, kWaves, kList><<<(unsigned)grid, 64 * kWaves, lds, s>>>(a);
   return hipGetLastError();
 }
 
 template <int DP, int kWaves>
 hipError_t run(const AttnArgs& a, hipStream_t s) {
-  return a.selected ? launch<DP, kWaves, true>(a, s) : launch<DP, kWaves, false>(a, s);
+  if (a.c.page_shift > kRunShift)
+    return a.selected ? launch<DP, 32, kWaves, true>(a, s) : launch<DP, 32, kWaves, false>(a, s);
+  return a.selected ? launch<DP, 16, kWaves, true>(a, s) : launch<DP, 16, kWaves, false>(a, s);
 }
 
 }  // namespace

@@ -463,8 +463,8 @@ typedef struct hypno_hip_kv_cache {
   size_t page_size;           /* a power of two, at most 2^16 (FP4: at least 16) */
   size_t head_dim;            /* a multiple of 8 (FP4: of 32), at most 256 */
   /* Elements (of k and v of FP4: bytes) from one page to the next, of k, v, k_scale and
-   * v_scale (0: no gap between pages; of k and v multiples of 8, FP4: of 16, and of the
-   * scales of FP4 multiples of 8). */
+   * v_scale (0: no gap between pages; of k and v multiples of 8.  FP4: below 2^31, of k
+   * and v multiples of 16, of the scales of 8). */
   size_t k_page_stride, v_page_stride, k_scale_page_stride, v_scale_page_stride;
 } hypno_hip_kv_cache;
 
