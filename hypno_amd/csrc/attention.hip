@@ -2,7 +2,6 @@
 // a call takes, and the sum of what a row's ranges of positions gave (5.6 us for 64 ranges
 // of 32 rows, 15 for four of 16384, 42 MB: 2.8 TB/s).
 #include <cmath>
-#include <cstdlib>
 
 #include "attention.hpp"
 
@@ -159,10 +158,11 @@ AttnPlan attn_plan(const KvCache& c, const KvBatch& b, int heads, int window, in
   // work-group takes them all: the kernel that joins ranges costs 4 us and its launch.
   // Beyond, one sequence gets a work-group for each one that the chip holds at a time.
   // Lengths of several may differ, so that the last range to end counts: against the
-  // start of a range (about 130 positions' time) the best length grows with the root of
-  // all work.  (us at 32/8 heads of 128, ranges of 128 / 256 / 512 / none: one sequence
+  // start of a range (about 130 positions' time, 250 of 4-bit ones) the best length grows
+  // with the root of all work.  (us at 32/8 heads of 128, ranges of 128 / 256 / 512 / none: one sequence
   // of 3000: 11.1 / 12.0 / 14.1 / -; 8 of up to 6000: 44 / 35 / 32 / -; 64 of up to 2000:
-  // - / 67 / 58 / 53.)
+  // - / 67 / 58 / 53.  4-bit, 64 of up to 8192, ranges of 512 / 1024 / 1536 / 2048: 92 / 82 /
+  // 82 / 84; 2 of 16000, 256 / 512 / 1024: 20.0 / 18.1 / 18.7.)
   p.fs = {1, 0x7FFFFFFF};
   p.few_waves = 4;
   const size_t token_rows = (size_t)b.tokens * heads, place = (size_t)c.head_dim * 4 + 8;
@@ -177,13 +177,13 @@ AttnPlan attn_plan(const KvCache& c, const KvBatch& b, int heads, int window, in
     const int64_t pairs = (int64_t)b.batch * c.kv_heads, slots = 2 * num_cus;
     if (seen > (pairs >= slots ? 2048 : 1024)) {
       const double each = (double)pairs * seen / slots;
-      const double best = b.batch > 1 ? std::sqrt(128.0 * each) : each;
+      const double start = c.dtype == kKvFp4 ? 256.0 : 128.0;
+      const double best = b.batch > 1 ? std::sqrt(start * each) : each;
       const int64_t least = std::min<int64_t>(std::max<int64_t>(8 * pairs, 128), 512);
       // (whole steps of four waves: a run of positions must not lie across two ranges)
       const int64_t fit = (seen + most(few_rows) - 1) / most(few_rows);
       const int64_t chunk = (std::max({least, (int64_t)best, fit}) + 127) / 128 * 128;
-      if (getenv("HK_CHUNK")) { const int64_t ch = atoi(getenv("HK_CHUNK")); p.fs = {up(seen, ch), (int)ch}; } else
-      p.fs.splits = up(seen, chunk),
+      p.fs.splits = up(seen, chunk);
       p.fs.chunk = (int)std::min<int64_t>(chunk, 0x7FFFFFFF);
     } else if (pairs <= num_cus && seen > 128) {
       p.few_waves = 8;
@@ -258,7 +258,6 @@ SelectedPlan selected_plan(const KvCache& c, const KvBatch& b, int heads, int co
     const int64_t splits = std::min(slots / pairs, most);
     const int64_t chunk = (std::max<int64_t>(256, up(positions, splits)) + 127) / 128 * 128;
     p.fs = {up(positions, chunk), (int)chunk};
-    if (getenv("HK_CHUNK")) { const int64_t ch = atoi(getenv("HK_CHUNK")); p.fs = {up(positions, ch), (int)ch}; }
   } else if (pairs <= num_cus && positions > 128) {
     p.waves = 8;
   }

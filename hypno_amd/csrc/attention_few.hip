@@ -273,7 +273,7 @@ __global__ void __launch_bounds__(64 * kWaves, (kWaves == 8 ? 1 : Few<kType, DP>
     }
     x.finish(__any(bad));
 
-    few_store<DP, kWaves, T::kWave, kList>(a, sq, g, ti0, r0, rows, split, past, x, smem, again);
+    few_store<DP, kWaves, T::kWave, kQ, kList>(a, sq, g, ti0, r0, rows, split, past, x, smem, again);
   }
 }
 

@@ -72,9 +72,9 @@ __device__ __forceinline__ uint32_t again_mask(int wave) {
 }
 
 // The waves' parts (x, each in kWave bytes of smem) to the output, or the range's place:
-// thread (row, piece) takes four elements.  Rows r0 and on of `rows`; kList: they are the
-// heads of token ti.
-template <int DP, int kWaves, int kWave, bool kList, typename R>
+// thread (row, piece) takes four elements.  Rows r0 and on of `rows`, kPass of them at most;
+// kList: they are the heads of token ti.
+template <int DP, int kWaves, int kWave, int kPass, bool kList, typename R>
 __device__ __forceinline__ void few_store(const AttnArgs& a, const Seq& sq, int g, int ti, int r0,
                                           int rows, int split, bool past, const R& x,
                                           uint8_t* smem, uint32_t& again) {
@@ -107,7 +107,7 @@ __device__ __forceinline__ void few_store(const AttnArgs& a, const Seq& sq, int 
     w[i] = w[i] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(w[i] - m);
     l += ml_of(i).y * w[i];
   }
-  const bool live = r0 + or_ < rows;
+  const bool live = or_ < kPass && r0 + or_ < rows;
   const int rr = min(r0 + or_, rows - 1);
   const size_t orow = kList ? (size_t)(sq.first + ti) * a.heads + g * G + rr
                             : (size_t)(sq.first + rr / G) * a.heads + g * G + rr % G;
@@ -130,7 +130,7 @@ __device__ __forceinline__ void few_store(const AttnArgs& a, const Seq& sq, int 
     if (!parts && (!(z == 0.0f) || past)) atomicOr(&again, 1u << or_);
   }
   // (rows again after all that is stored of them)
-  if (parts && r0 + kFewQ >= rows) return;
+  if (parts && r0 + kPass >= rows) return;
   __syncthreads();
   if (again) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -145,7 +145,7 @@ __device__ __forceinline__ void few_store(const AttnArgs& a, const Seq& sq, int 
       attn_rows(a, sq, g, r0, left);
     }
   }
-  if (r0 + kFewQ < rows) __syncthreads();
+  if (r0 + kPass < rows) __syncthreads();
 }
 
 }  // namespace hypno

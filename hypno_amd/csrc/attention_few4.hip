@@ -50,8 +50,17 @@ __device__ __forceinline__ void wait_loads() {
 #endif
 }
 
-template <int DP, int kLen, int kWaves, bool kList>
-__global__ void __launch_bounds__(64 * kWaves, kWaves == 8 ? 1 : DP > 128 ? 1 : 3)
+// Sum of a lane's value and that of the lane eight columns on.
+__device__ __forceinline__ float both_halves(float x) {
+  return x + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x128, 0xF, 0xF,
+                                                        false));  // row_ror:8
+}
+
+// kPass: rows that go through the tiles together, 16, or 8 whose two parts of q (and of the
+// weights) are columns of one product: half the products, and registers for a work-group more
+// on a CU.
+template <int DP, int kLen, int kPass, int kWaves, bool kList>
+__global__ void __launch_bounds__(64 * kWaves, kWaves == 8 ? 2 : DP > 128 ? 2 : kPass == 8 ? 4 : 3)
     attn_few4_kernel(AttnArgs a) {
   typedef Few4<DP, kLen> T;
   constexpr int kRuns = T::kRuns;
@@ -103,9 +112,10 @@ __global__ void __launch_bounds__(64 * kWaves, kWaves == 8 ? 1 : DP > 128 ? 1 : 
     return 8 * s / kPart * 4 * kPart + kPart * grp + 8 * s % kPart;
   };
 
-  for (int r0 = 0; r0 < rows; r0 += kQ) {
-    const int r1 = min(r0 + kQ, rows);
-    const Span span = kList ? Span{0, seen} : span_of(a, sq, r0, r1);
+  for (int r0 = 0; r0 < rows; r0 += kPass) {
+    const int r1 = min(r0 + kPass, rows), s0 = r0 & -kQ;
+    // (the ranges are those of 16 rows, as in the kernel that joins them)
+    const Span span = kList ? Span{0, seen} : span_of(a, sq, s0, min(s0 + kQ, rows));
     int lo = past ? 0 : span.lo, hi = past ? 0 : span.hi;
     if (kList) {
       lo = (int)min((int64_t)split * a.fs.chunk, (int64_t)hi);
@@ -116,7 +126,7 @@ __global__ void __launch_bounds__(64 * kWaves, kWaves == 8 ? 1 : DP > 128 ? 1 : 
       if (split + 1 < a.fs.splits) hi = (int)min((int64_t)hi, start + a.fs.chunk);
       lo = (int)start;
     }
-    const int row = min(r0 + col, rows - 1);
+    const int row = min(r0 + col % kPass, rows - 1);
     const int ti = kList ? ti0 : row / G, h = g * G + (kList ? row : row % G);
     const int t = sq.first + ti;
     const int seen_lo = first_seen(a, sq, ti), seen_hi = min(sq.kv - sq.n + ti, hi - 1);
@@ -194,8 +204,12 @@ __global__ void __launch_bounds__(64 * kWaves, kWaves == 8 ? 1 : DP > 128 ? 1 : 
         }
     }
     R x;
-    x.init_of(r0 + col < rows ? a.q + (size_t)t * a.q_stride + (size_t)h * D : nullptr, D, a.scale,
+    x.init_of(r0 + col % kPass < rows ? a.q + (size_t)t * a.q_stride + (size_t)h * D : nullptr, D, a.scale,
               element);
+    if (kPass == 8) {
+#pragma unroll
+      for (int st = 0; st < R::kSteps; st++) x.qh[st] = col < 8 ? x.qh[st] : x.ql[st];
+    }
     const uint8_t* at = ring;
     for (int tile = 0; tile < mine; tile++) {
       const int p0 = place(tile);
@@ -255,8 +269,14 @@ __global__ void __launch_bounds__(64 * kWaves, kWaves == 8 ? 1 : DP > 128 ? 1 : 
 #pragma unroll
         for (int i = 0; i < 2; i++) s[i] = Mfma<kQ>::mul(k[i], x.qh[st], s[i]);
 #pragma unroll
-        for (int i = 0; i < 2; i++) s[i] = Mfma<kQ>::mul(k[i], x.ql[st], s[i]);
+        for (int i = 0; i < 2 && kPass == 16; i++) s[i] = Mfma<kQ>::mul(k[i], x.ql[st], s[i]);
         __builtin_amdgcn_sched_barrier(0);
+      }
+      if (kPass == 8) {
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+          for (int r = 0; r < 4; r++) s[i][r] = both_halves(s[i][r]);
       }
       // Keys that a row does not see.  (Apart from the maximum: two ways to that one have the
       // compiler copy all of o.)
@@ -286,7 +306,7 @@ __global__ void __launch_bounds__(64 * kWaves, kWaves == 8 ? 1 : DP > 128 ? 1 : 
         sum += w[0] + w[1];
         uint32_t hi16, lo16;
         split_f16(w[0], w[1], neg, hi16, lo16);
-        wh[i] = hi16, wl[i] = lo16;
+        wh[i] = kPass == 16 || col < 8 ? hi16 : lo16, wl[i] = lo16;
       }
       x.l += sum;
       // Channels 32 blk + col and 16 on, of keys 4 grp to 4 grp + 3 of both halves of the tile:
@@ -321,32 +341,46 @@ __global__ void __launch_bounds__(64 * kWaves, kWaves == 8 ? 1 : DP > 128 ? 1 : 
             y[i] = __builtin_bit_cast(uint32_t, (half2v)(v[i] * scale[i]));
           const int n = 2 * blk + half;
           x.o[n] = Mfma<kQ>::mul(f16x8(y), f16x8(wh), x.o[n]);
-          x.o[n] = Mfma<kQ>::mul(f16x8(y), f16x8(wl), x.o[n]);
+          if (kPass == 16) x.o[n] = Mfma<kQ>::mul(f16x8(y), f16x8(wl), x.o[n]);
         }
       }
       at = at == ring + T::kAhead * T::kTile ? ring : at + T::kTile;
     }
     x.finish(bad != 0);
-    few_store<DP, kWaves, T::kWave, kList>(a, sq, g, ti0, r0, rows, split, past, x, smem, again);
+    if (kPass == 8) {
+#pragma unroll
+      for (int n = 0; n < R::kDt; n++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) x.o[n][r] = both_halves(x.o[n][r]);
+    }
+    few_store<DP, kWaves, T::kWave, kPass, kList>(a, sq, g, ti0, r0, rows, split, past, x, smem, again);
   }
 }
 
-template <int DP, int kLen, int kWaves, bool kList>
+template <int DP, int kLen, int kPass, int kWaves, bool kList>
 hipError_t launch(const AttnArgs& a, hipStream_t s) {
   const int lds = kWaves * Few4<DP, kLen>::kWave + (kList ? a.count * (int)sizeof(SeenPage) : 0);
   const size_t grid = (size_t)(kList ? a.b.tokens : a.b.batch) * a.c.kv_heads * a.fs.splits;
   if (grid > 0xFFFFFF) return hipErrorInvalidValue;
-  const hipError_t e = set_lds_limit((const void*)attn_few4_kernel<DP, kLen, kWaves, kList>, lds);
+  const hipError_t e = set_lds_limit((const void*)attn_few4_kernel<DP, kLen, kPass, kWaves, kList>, lds);
   if (e != hipSuccess) return e;
-  attn_few4_kernel<DP, kLen, kWaves, kList><<<(unsigned)grid, 64 * kWaves, lds, s>>>(a);
+  attn_few4_kernel<DP, kLen, kPass, kWaves, kList><<<(unsigned)grid, 64 * kWaves, lds, s>>>(a);
   return hipGetLastError();
+}
+
+template <int DP, int kLen, int kPass, int kWaves>
+hipError_t run(const AttnArgs& a, hipStream_t s) {
+  return a.selected ? launch<DP, kLen, kPass, kWaves, true>(a, s)
+                    : launch<DP, kLen, kPass, kWaves, false>(a, s);
 }
 
 template <int DP, int kWaves>
 hipError_t run(const AttnArgs& a, hipStream_t s) {
+  // (a sequence with more rows than a pass goes through its keys once for each)
+  const bool one = a.group <= 8 && (a.selected || a.b.tokens <= a.b.batch);
   if (a.c.page_shift > kRunShift)
-    return a.selected ? launch<DP, 32, kWaves, true>(a, s) : launch<DP, 32, kWaves, false>(a, s);
-  return a.selected ? launch<DP, 16, kWaves, true>(a, s) : launch<DP, 16, kWaves, false>(a, s);
+    return one ? run<DP, 32, 8, kWaves>(a, s) : run<DP, 32, 16, kWaves>(a, s);
+  return one ? run<DP, 16, 8, kWaves>(a, s) : run<DP, 16, 16, kWaves>(a, s);
 }
 
 }  // namespace
