@@ -188,15 +188,31 @@ __device__ __forceinline__ void wave_lds_sync() {
 #endif
 }
 
+// Wave-wide (the lanes of one) or work-group-wide waits for LDS.
+template <bool kTeam>
+__device__ __forceinline__ void lds_sync() {
+  if (kTeam)
+    __syncthreads();
+  else
+    wave_lds_sync();
+}
+
 // One work-group a kv head of up to 16 / group tokens of a sequence: scores of their
-// pages into LDS, 16 pages by 16 rows (token, head) a wave at a time, then for each token
-// the largest.  kTeam: all waves search one token's keys, else each wave its own tokens'.
+// pages into LDS, 16 pages by 16 rows (token, head) a product, then for each token the key
+// of the last page that is taken, eight bits at a time from the top by counting.  kTeam: all
+// waves look at one token's keys, else each wave at its own tokens'.
+//
+// Latency is what there is to save: a page's number, its bounds, the counts are reads that
+// depend on each other, so that a wave asks for four products' pages at a time, and for
+// the next four's numbers with them.
 template <int DP, int kWaves, bool kTeam>
 __global__ void __launch_bounds__(64 * kWaves) select_pages_kernel(SelectArgs a) {
-  constexpr int kSteps = 2 * DP / 64, kPitch = 2 * DP + 16;
+  constexpr int kSteps = 2 * DP / 64, kPitch = 2 * DP + 16, kAtOnce = DP <= 128 ? 4 : kTeam ? 1 : 2;
   __shared__ __attribute__((aligned(16))) uint8_t codes[16 * kPitch];
   __shared__ float row_scale[16], part[kWaves][16][17];
-  __shared__ int counts[2][kWaves];
+  __shared__ __attribute__((aligned(16))) int hist[kTeam ? 1 : kWaves][256];
+  __shared__ uint2 ends[kWaves];
+  __shared__ int2 counts[kWaves];
   extern __shared__ uint32_t keys[];  // [tokens][pitch]
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int KV = a.k.kv_heads, G = a.group, D = a.k.head_dim, shift = a.k.page_shift;
@@ -212,14 +228,26 @@ __global__ void __launch_bounds__(64 * kWaves) select_pages_kernel(SelectArgs a)
   const int most = min(a.most, a.b.width);
   const int top = (int)min((int64_t)most, ((pos0 + nt - 1) >> shift) + 1 - a.last);
   const int* const table = a.b.page_table + (size_t)b * a.b.width;
+  // A wave's pages: 16 kAtOnce in a row, then those 16 kAtOnce kWaves on; lane % 16 of each 16.
+  constexpr int kStride = 16 * kAtOnce * kWaves;
+  const int start = a.first + 16 * kAtOnce * wave;
+  auto look_up = [&](int (&page)[kAtOnce], int p0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < kAtOnce; i++) {
+      const int p = p0 + 16 * i + lane % 16;
+      page[i] = p < top ? load_global<int>(table + p) : -1;
+    }
+  };
+  int page[kAtOnce];
+  look_up(page, start);
 
   for (int h0 = 0; h0 < G && top > a.first; h0 += 16) {
     // The rows' codes, [negative part][positive part]; 16 lanes a row.
     if (wave < 4) {
       const int r = tid / 16, sub = tid % 16;
       const int tok = G <= 16 ? r / G : 0, h = G <= 16 ? r % G : h0 + r;
-      const bool live = tok < nt && h < G && (G > 16 || r < nt * G);
-      float x[DP / 128 + 1][8];
+      const bool live = tok < nt && h < G;
+      float x[(DP + 127) / 128][8];
       uint32_t mb = 0;
 #pragma unroll
       for (int j = 0; j < (DP + 127) / 128; j++) {
@@ -261,104 +289,188 @@ __global__ void __launch_bounds__(64 * kWaves) select_pages_kernel(SelectArgs a)
     for (int s = 0; s < kSteps; s++)
       q[s] = *reinterpret_cast<const i32x4*>(codes + lane % 16 * kPitch + 64 * s + lane / 16 * 16);
     const float qs = row_scale[lane % 16];
-    for (int p0 = a.first + 16 * wave; p0 < top; p0 += 16 * kWaves) {
-      const int p = p0 + lane % 16;
-      int page = p < top ? load_global<int>(table + p) : -1;
-      const bool there = page >= 0 && page < a.k.pages;
-      page = there ? page : 0;
-      i32x4 acc = {0, 0, 0, 0};
-      if (a.k.pages) {  // (none: nothing is read)
-        const int8_t* const src = a.k.codes + (size_t)page * a.k.page + (size_t)2 * g * D;
-        i32x4 k[kSteps];
+    if (h0) look_up(page, start);
+    for (int p0 = start; p0 < top; p0 += kStride) {
+      i32x4 k[kAtOnce][kSteps];
+      float ks[kAtOnce];
+      bool there[kAtOnce];
 #pragma unroll
-        for (int s = 0; s < kSteps; s++) {
-          // Sixteen channels from d on of one bound; those past D meet zeros.
-          const int c = 64 * s + lane / 16 * 16, d = c % DP;
-          const int8_t* const at = src + (c < DP ? 0 : D) + (d < D ? d : 0);
-          if (D % 16 == 0) {
-            k[s] = __builtin_bit_cast(i32x4, load_global<u32x4a8>(at));
-          } else {
-            const uint2 lo = load_global<uint2>(at);
-            const uint2 hi = load_global<uint2>(d + 8 < D ? at + 8 : at);
-            k[s] = i32x4{(int)lo.x, (int)lo.y, (int)hi.x, (int)hi.y};
+      for (int i = 0; i < kAtOnce; i++) {
+        there[i] = page[i] >= 0 && page[i] < a.k.pages;
+        const int id = there[i] ? page[i] : 0;
+        const int8_t* const src = a.k.codes + (size_t)id * a.k.page + (size_t)2 * g * D;
+#pragma unroll
+        for (int s = 0; s < kSteps; s++) k[i][s] = i32x4{0, 0, 0, 0};
+        if (a.k.pages && p0 + 16 * i < top) {
+#pragma unroll
+          for (int s = 0; s < kSteps; s++) {
+            // Sixteen channels from d on of one bound; those past D meet zeros.
+            const int c = 64 * s + lane / 16 * 16, d = c % DP;
+            const int8_t* const at = src + (c < DP ? 0 : D) + (d < D ? d : 0);
+            if (D % 16 == 0) {
+              k[i][s] = __builtin_bit_cast(i32x4, load_global<u32x4a8>(at));
+            } else {
+              const uint2 lo = load_global<uint2>(at);
+              const uint2 hi = load_global<uint2>(d + 8 < D ? at + 8 : at);
+              k[i][s] = i32x4{(int)lo.x, (int)lo.y, (int)hi.x, (int)hi.y};
+            }
           }
         }
+        ks[i] = there[i] ? load_global<float>(a.k.scale + (size_t)id * a.k.s_page + g) : 0.0f;
+      }
+      look_up(page, p0 + kStride);
+#pragma unroll
+      for (int i = 0; i < kAtOnce; i++) {
+        const int p = p0 + 16 * i + lane % 16;
+        if (p0 + 16 * i >= top) continue;
+        i32x4 acc = {0, 0, 0, 0};
 #pragma unroll
         for (int s = 0; s < kSteps; s++)
-          acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[s], q[s], acc, 0, 0, 0);
-      }
-      const float ks = there ? load_global<float>(a.k.scale + (size_t)page * a.k.s_page + g) : 0.0f;
+          acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[i][s], q[s], acc, 0, 0, 0);
 #pragma unroll
-      for (int i = 0; i < 4; i++) part[wave][lane / 16 * 4 + i][lane % 16] = (float)acc[i] * qs;
-      wave_lds_sync();
-      for (int tok = lane / 16; tok < nt; tok += 4) {
-        const float* const rows = part[wave][lane % 16] + (G <= 16 ? tok * G : 0);
-        float m = rows[0];
-        for (int h = 1; h < min(G - h0, 16); h++) m = fmaxf(m, rows[h]);
-        uint32_t key = key_of(m * ks);
-        if (!there || p > ((pos0 + tok) >> shift) - a.last) key = 0;
-        if (p < top) {
-          uint32_t* const to = keys + (size_t)tok * a.pitch + p;
-          *to = h0 ? max(*to, key) : key;
+        for (int j = 0; j < 4; j++) part[wave][lane / 16 * 4 + j][lane % 16] = (float)acc[j] * qs;
+        wave_lds_sync();
+        for (int tok = lane / 16; tok < nt; tok += 4) {
+          const float* const rows = part[wave][lane % 16] + (G <= 16 ? tok * G : 0);
+          float m = rows[0];
+          for (int h = 1; h < min(G - h0, 16); h++) m = fmaxf(m, rows[h]);
+          uint32_t key = key_of(m * ks[i]);
+          if (!there[i] || p > ((pos0 + tok) >> shift) - a.last) key = 0;
+          if (p < top) {
+            uint32_t* const to = keys + (size_t)tok * a.pitch + p;
+            *to = h0 ? max(*to, key) : key;
+          }
         }
+        wave_lds_sync();
       }
-      wave_lds_sync();
     }
     __syncthreads();
   }
 
-  // Each token's largest, in the pages' order.
-  int at = 0;  // of counts
+  const int threads = kTeam ? 64 * kWaves : 64, at = kTeam ? tid : lane;
+  int* const bins = hist[kTeam ? 0 : wave];
   for (int tok = kTeam ? 0 : wave; tok < nt; tok += kTeam ? 1 : kWaves) {
     const int64_t pos = pos0 + tok;
     const int own = pos < 0 ? -1 : (int)(pos >> shift);
-    const int hi = min(most, own + 1 - a.last), need = a.count - a.first - a.last;
+    const int lo = a.first, hi = min(most, own + 1 - a.last);
     const uint32_t* const key = keys + (size_t)tok * a.pitch;
-    auto above = [&](uint32_t least) __attribute__((always_inline)) {
-      int c = 0;
-      for (int p = a.first + (kTeam ? tid : lane); p - (kTeam ? tid : lane) < hi;
-           p += kTeam ? 64 * kWaves : 64)
-        c += __popcll(__ballot(p < hi && key[p] >= least));
-      if (!kTeam) return c;
-      if (lane == 0) counts[at][wave] = c;
-      __syncthreads();
-      c = 0;
-#pragma unroll
-      for (int w = 0; w < kWaves; w++) c += counts[at][w];
-      at ^= 1;
-      return c;
-    };
-    // The key of the last one that is taken: the largest that `need` reach.
-    uint32_t least = 1;
-    int ties = 0x7FFFFFFF;  // of those with this key that are taken
-    if (hi > a.first && above(1) > need) {
-      int c = 0;
-      least = 0;
-      for (uint32_t bit = 0x80000000u; bit && c != need; bit >>= 1) {
-        const int x = above(least | bit);
-        if (x >= need) least |= bit, c = x;
-      }
-      if (c != need) ties = need - (least == 0xFFFFFFFFu ? 0 : above(least + 1));
+    // Candidates, the smallest and largest key, over all threads.
+    int all = 0;
+    uint32_t low = 0xFFFFFFFFu, high = 0;
+    for (int p = lo + at; p - at < hi; p += threads) {
+      const uint32_t k = p < hi ? key[p] : 0;
+      all += __popcll(__ballot(k != 0));
+      low = min(low, k ? k : 0xFFFFFFFFu);
+      high = max(high, k);
     }
-    if (kTeam && wave) continue;
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) {
+      low = min(low, (uint32_t)__shfl_xor((int)low, off, 64));
+      high = max(high, (uint32_t)__shfl_xor((int)high, off, 64));
+    }
+    if (kTeam) {
+      if (lane == 0) ends[wave] = make_uint2(low, high), counts[wave].x = all;
+      __syncthreads();
+      all = 0;
+      for (int w = 0; w < kWaves; w++) {
+        low = min(low, ends[w].x);
+        high = max(high, ends[w].y);
+        all += counts[w].x;
+      }
+    }
+    // Keys above `least` are taken, and `ties` of those that are `least`; `left` of what
+    // agrees with `least` in the bits before `bits` are to be.
+    const int need = a.count - a.first - a.last;
+    uint32_t least = all ? low : 1;
+    int ties = 0x7FFFFFFF, left = need;
+    if (all > need && need > 0 && high > low) {
+      // From the first bit in which keys differ on, up to eight bits at a time.
+      int bits = 32 - __clz((int)(high - low));
+      least = 0;  // (of keys - low)
+      while (bits > 0) {
+        const int width = min(bits, 8), down = bits - width;
+        for (int i = at; i < 256; i += threads) bins[i] = 0;
+        lds_sync<kTeam>();
+        for (int p = lo + at; p < hi; p += threads) {
+          const uint32_t k = key[p];
+          if (k && ((uint64_t)(k - low) >> bits) == ((uint64_t)least >> bits))
+            atomicAdd(&bins[((k - low) >> down) & ((1u << width) - 1)], 1);
+        }
+        lds_sync<kTeam>();
+        // The bin in which the left-th from the top lies; a lane has four.
+        const int4 c = *reinterpret_cast<const int4*>(bins + 4 * lane);
+        int above = c.x + c.y + c.z + c.w;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+          const int x = __shfl_down(above, off, 64);
+          above += lane + off < 64 ? x : 0;
+        }
+        const int in = 63 - __clzll((long long)__ballot(above >= left));
+        const int4 d = make_int4(__shfl(c.x, in, 64), __shfl(c.y, in, 64), __shfl(c.z, in, 64),
+                                 __shfl(c.w, in, 64));
+        int over = __shfl(above, in, 64) - (d.x + d.y + d.z + d.w), bin = 4 * in + 3, here = d.w;
+        if (over + here < left) over += here, bin--, here = d.z;
+        if (over + here < left) over += here, bin--, here = d.y;
+        if (over + here < left) over += here, bin--, here = d.x;
+        left -= over;
+        least |= (uint32_t)bin << down;
+        bits = down;
+        lds_sync<kTeam>();
+        if (here == left) break;  // all of the bin
+      }
+      if (bits == 0) ties = left;
+      least += low;
+      // (of a whole bin all keys are at least its first)
+    } else if (all > need) {
+      ties = need;
+    }
+    // In the pages' order; kTeam: each wave a part of them, after how many the others take.
+    const int per = kTeam ? (max(hi - lo, 0) + threads - 1) / threads * 64 : max(hi - lo, 0);
+    const int p_lo = kTeam ? min(lo + wave * per, max(hi, lo)) : lo;
+    const int p_hi = kTeam ? min(p_lo + per, hi) : hi;
     int* const out = a.out + ((size_t)(t0 + tok) * KV + g) * a.count;
     int put = min(a.first, own + 1);
-    if (lane < put) out[lane] = lane;
-    for (int i = lane + 64; i < put; i += 64) out[i] = i;
-    for (int p0 = a.first; p0 < hi && need > 0; p0 += 64) {
+    const int head = put;
+    int total = 0;
+    if (kTeam) {
+      int more = 0, same = 0;
+      for (int p0 = p_lo; p0 < p_hi; p0 += 64) {
+        const int p = p0 + lane;
+        const uint32_t k = p < p_hi ? key[p] : 0;
+        more += __popcll(__ballot(k > least));
+        same += __popcll(__ballot(k && k == least));
+      }
+      __syncthreads();
+      if (lane == 0) counts[wave] = make_int2(more, same);
+      __syncthreads();
+      int before = 0;  // that are `least`, in the waves before
+      for (int w = 0; w < kWaves; w++) {
+        const int2 c = counts[w];
+        const int take = need > 0 ? c.x + min(c.y, max(ties - before, 0)) : 0;
+        if (w < wave) put += take;
+        total += take;
+        if (w == wave) same = before;
+        before += c.y;
+      }
+      ties = max(ties - same, 0);
+    }
+    for (int p0 = p_lo; p0 < p_hi && need > 0; p0 += 64) {
       const int p = p0 + lane;
-      const uint32_t k = p < hi ? key[p] : 0;
-      const uint64_t same = __ballot(k == least), before = (1ull << lane) - 1;
-      const bool take = k > least || (k == least && k && __popcll(same & before) < ties);
+      const uint32_t k = p < p_hi ? key[p] : 0;
+      const uint64_t same = __ballot(k && k == least), before = (1ull << lane) - 1;
+      const bool take = k > least || (k && k == least && __popcll(same & before) < ties);
       const uint64_t taken = __ballot(take);
       if (take) out[put + __popcll(taken & before)] = p;
       put += __popcll(taken);
       ties -= min(ties, (int)__popcll(same));
     }
-    const int tail = max(own + 1 - a.last, min(a.first, own + 1));
-    for (int p = tail + lane; p <= own; p += 64) out[put + p - tail] = p;
+    if (kTeam) put = head + total;
+    const int tail = max(own + 1 - a.last, head);
+    for (int i = at; i < head; i += threads) out[i] = i;
+    for (int p = tail + at; p <= own; p += threads) out[put + p - tail] = p;
     put += own + 1 - tail;
-    for (int i = put + lane; i < a.count; i += 64) out[i] = -1;
+    for (int i = put + at; i < a.count; i += threads) out[i] = -1;
+    if (kTeam) __syncthreads();  // (before the next token's counts)
   }
 }
 
