@@ -566,20 +566,6 @@ struct Rows {
   }
 };
 
-// Eight 4-bit codes times their scale (twice in a register) -> eight fp16, each rounded
-// once.
-__device__ __forceinline__ u32x4 fp4_to_f16(uint32_t x, half2v scale) {
-  u32x4 r;
-  const half2v v[4] = {
-      __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(x, 1.0f, 0),
-      __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(x, 1.0f, 1),
-      __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(x, 1.0f, 2),
-      __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(x, 1.0f, 3)};
-#pragma unroll
-  for (int i = 0; i < 4; i++) r[i] = __builtin_bit_cast(uint32_t, (half2v)(v[i] * scale));
-  return r;
-}
-
 // Launchers of the kernels' files.
 hipError_t launch_attn_tile(const AttnArgs& a, hipStream_t s);
 hipError_t launch_attn_few(const AttnArgs& a, hipStream_t s);

@@ -149,6 +149,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_kv_kernel(AppendArgs a)
       }
     } else if (kType == kKvFp4) {
       // A group of 32 elements is four lanes.
+      if (!__any(live && !is_q)) continue;
       uint32_t mb = 0;
 #pragma unroll
       for (int i = 0; i < 8; i++) mb = max(mb, __float_as_uint(x[i]) & 0x7FFFFFFFu);
@@ -160,9 +161,16 @@ __global__ void __launch_bounds__(kAppendThreads) append_kv_kernel(AppendArgs a)
         const float sf = (float)s;
         uint32_t p = 0;
         if (sf > 0.0f) {
+          // x / s rounded to fp32, as a division gives it, in three operations: with r = 1 / s
+          // rounded and y = x r, y + (x - y s) r is (Markstein's theorem; nothing underflows
+          // where |x / s| is near a border of the grid).
+          const float r = 1.0f / sf;
           float y[8];
 #pragma unroll
-          for (int i = 0; i < 8; i++) y[i] = x[i] / sf;
+          for (int i = 0; i < 8; i++) {
+            y[i] = x[i] * r;
+            y[i] = copysignf(fmaf(fmaf(-y[i], sf, x[i]), r, y[i]), x[i]);  // (-0 as well)
+          }
           p = fp4_codes(y);
         }
         uint8_t* dst = (is_k ? (uint8_t*)a.c.k + (size_t)page * a.c.k_page

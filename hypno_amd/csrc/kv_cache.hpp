@@ -36,6 +36,20 @@ __device__ __forceinline__ _Float16 fp4_value(uint32_t code) {
   return __builtin_bit_cast(_Float16, bits) * (_Float16)16384.0f;
 }
 
+// Eight 4-bit codes times their scale (twice in a register) -> eight fp16, each rounded
+// once.
+__device__ __forceinline__ u32x4 fp4_to_f16(uint32_t x, half2v scale) {
+  u32x4 r;
+  const half2v v[4] = {
+      __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(x, 1.0f, 0),
+      __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(x, 1.0f, 1),
+      __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(x, 1.0f, 2),
+      __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(x, 1.0f, 3)};
+#pragma unroll
+  for (int i = 0; i < 4; i++) r[i] = __builtin_bit_cast(uint32_t, (half2v)(v[i] * scale));
+  return r;
+}
+
 // The codes of eight finite values: the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 and their
 // negatives, halves to the even code (the conversion's own rounding).
 __device__ __forceinline__ uint32_t fp4_codes(const float (&y)[8]) {

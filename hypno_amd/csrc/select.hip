@@ -19,10 +19,10 @@ namespace hypno {
 namespace {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x4a8 __attribute__((ext_vector_type(4), aligned(8)));
 typedef float f32x4a4 __attribute__((ext_vector_type(4), aligned(4)));
 
 constexpr int kMaxDim = 256;
+constexpr int kTeamWaves = 8;
 
 // The code of x with scale s > 0.
 __device__ __forceinline__ uint32_t code8(float x, float s) {
@@ -77,8 +77,10 @@ __device__ __forceinline__ void load_keys(float (&x)[8], const BoundsArgs& a, in
     const size_t at = ((size_t)(g * (D / kFp4Group) + e0 / kFp4Group) << a.c.page_shift) + slot;
     const _Float16 s = load_global<_Float16>((const _Float16*)a.c.k_scale +
                                              (size_t)page * a.c.ks_page + at);
+    const u32x4 y = fp4_to_f16(v, half2v{s, s});
 #pragma unroll
-    for (int i = 0; i < 8; i++) x[i] = (float)(_Float16)(fp4_value(v >> 4 * i) * s);
+    for (int i = 0; i < 8; i++)
+      x[i] = (float)__builtin_bit_cast(_Float16, (uint16_t)(y[i / 2] >> 16 * (i % 2)));
   }
 }
 
@@ -166,6 +168,7 @@ struct SelectArgs {
   const float* q;
   size_t q_stride;
   int heads, group, count, first, last;
+  int rows;    // of a token in a product: 1, 2, 4, 8 or 16, the group's heads or more
   int most;    // pages of a sequence that have a score at most
   int pitch;   // of a token's keys in LDS
   int tokens;  // of a work-group
@@ -188,6 +191,29 @@ __device__ __forceinline__ void wave_lds_sync() {
 #endif
 }
 
+// Over the wave's lanes, by moves between neighbours, not through LDS: the sums up to each
+// lane, and the largest.
+template <int kCtrl, int kRows>
+__device__ __forceinline__ uint32_t moved(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, kCtrl, kRows, 0xF, false);
+}
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
+  x += moved<0x111, 0xF>(x);  // row_shr:1, 2, 4, 8
+  x += moved<0x112, 0xF>(x);
+  x += moved<0x114, 0xF>(x);
+  x += moved<0x118, 0xF>(x);
+  x += moved<0x142, 0xA>(x);  // row_bcast:15, 31
+  return x + moved<0x143, 0xC>(x);
+}
+__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
+  x = max(x, moved<0x111, 0xF>(x));
+  x = max(x, moved<0x112, 0xF>(x));
+  x = max(x, moved<0x114, 0xF>(x));
+  x = max(x, moved<0x118, 0xF>(x));
+  x = max(x, moved<0x142, 0xA>(x));
+  return (uint32_t)__builtin_amdgcn_readlane((int)max(x, moved<0x143, 0xC>(x)), 63);
+}
+
 // Wave-wide (the lanes of one) or work-group-wide waits for LDS.
 template <bool kTeam>
 __device__ __forceinline__ void lds_sync() {
@@ -197,19 +223,25 @@ __device__ __forceinline__ void lds_sync() {
     wave_lds_sync();
 }
 
-// One work-group a kv head of up to 16 / group tokens of a sequence: scores of their
-// pages into LDS, 16 pages by 16 rows (token, head) a product, then for each token the key
-// of the last page that is taken, eight bits at a time from the top by counting.  kTeam: all
-// waves look at one token's keys, else each wave at its own tokens'.
+// One work-group a kv head of up to 16 / rows tokens of a sequence: scores of their pages
+// into LDS, 16 rows (token, head) by 16 pages a product, so that a lane has up to four heads
+// of a page; then for each token the key of the last page that is taken, eight bits at a time
+// from the top by counting.  kTeam: all waves look at one token's keys, else each wave at its
+// own tokens'.
 //
 // Latency is what there is to save: a page's number, its bounds, the counts are reads that
 // depend on each other, so that a wave asks for four products' pages at a time, and for
-// the next four's numbers with them.
+// the next four's numbers with them.  A page's two bounds are one piece of memory, 128 bytes
+// of which eight lanes read; lanes that each read of another page, as the product takes
+// them, take four times as long (16 us for 2048 pages), so that they change places in LDS.
 template <int DP, int kWaves, bool kTeam>
-__global__ void __launch_bounds__(64 * kWaves) select_pages_kernel(SelectArgs a) {
-  constexpr int kSteps = 2 * DP / 64, kPitch = 2 * DP + 16, kAtOnce = DP <= 128 ? 4 : kTeam ? 1 : 2;
+__global__ void __launch_bounds__(64 * kWaves, DP > 128 ? 2 : kTeam ? 2 : 4)
+    select_pages_kernel(SelectArgs a) {
+  constexpr int kSteps = 2 * DP / 64, kPitch = 2 * DP + 16, kAtOnce = (kTeam ? 4 : 2) / (DP > 128 ? 2 : 1);
+  constexpr int kUnits = 2 * DP / 128;  // of 128 bytes of the bounds
   __shared__ __attribute__((aligned(16))) uint8_t codes[16 * kPitch];
-  __shared__ float row_scale[16], part[kWaves][16][17];
+  __shared__ __attribute__((aligned(16))) float row_scale[16];
+  __shared__ __attribute__((aligned(16))) uint8_t stage[kWaves][16 * 128];
   __shared__ __attribute__((aligned(16))) int hist[kTeam ? 1 : kWaves][256];
   __shared__ uint2 ends[kWaves];
   __shared__ int2 counts[kWaves];
@@ -228,7 +260,8 @@ __global__ void __launch_bounds__(64 * kWaves) select_pages_kernel(SelectArgs a)
   const int most = min(a.most, a.b.width);
   const int top = (int)min((int64_t)most, ((pos0 + nt - 1) >> shift) + 1 - a.last);
   const int* const table = a.b.page_table + (size_t)b * a.b.width;
-  // A wave's pages: 16 kAtOnce in a row, then those 16 kAtOnce kWaves on; lane % 16 of each 16.
+  // A wave's pages: 16 kAtOnce in a row, then those 16 kAtOnce kWaves on; a lane looks up
+  // lane % 16 of each 16, and reads of lane / 8 and 8 on.
   constexpr int kStride = 16 * kAtOnce * kWaves;
   const int start = a.first + 16 * kAtOnce * wave;
   auto look_up = [&](int (&page)[kAtOnce], int p0) __attribute__((always_inline)) {
@@ -242,11 +275,12 @@ __global__ void __launch_bounds__(64 * kWaves) select_pages_kernel(SelectArgs a)
   look_up(page, start);
 
   for (int h0 = 0; h0 < G && top > a.first; h0 += 16) {
-    // The rows' codes, [negative part][positive part]; 16 lanes a row.
+    // The rows' codes, [negative part][positive part][zeros]; 16 lanes a row.
     if (wave < 4) {
       const int r = tid / 16, sub = tid % 16;
-      const int tok = G <= 16 ? r / G : 0, h = G <= 16 ? r % G : h0 + r;
-      const bool live = tok < nt && h < G;
+      // (rows past the group's heads: its first again, which changes no maximum)
+      const int tok = r / a.rows, h = h0 + r % a.rows < G ? h0 + r % a.rows : h0;
+      const bool live = tok < nt;
       float x[(DP + 127) / 128][8];
       uint32_t mb = 0;
 #pragma unroll
@@ -278,8 +312,9 @@ __global__ void __launch_bounds__(64 * kWaves) select_pages_kernel(SelectArgs a)
             (x[j][i] < 0.0f ? neg : pos)[i / 4] |= c;
           }
         }
-        *reinterpret_cast<uint2*>(codes + r * kPitch + e) = make_uint2(neg[0], neg[1]);
-        *reinterpret_cast<uint2*>(codes + r * kPitch + DP + e) = make_uint2(pos[0], pos[1]);
+        uint8_t* const row = codes + r * kPitch;
+        *reinterpret_cast<uint2*>(row + (e < D ? e : 2 * e)) = make_uint2(neg[0], neg[1]);
+        *reinterpret_cast<uint2*>(row + (e < D ? D + e : 2 * e + 8)) = make_uint2(pos[0], pos[1]);
       }
       if (sub == 0) row_scale[r] = s;
     }
@@ -288,60 +323,72 @@ __global__ void __launch_bounds__(64 * kWaves) select_pages_kernel(SelectArgs a)
 #pragma unroll
     for (int s = 0; s < kSteps; s++)
       q[s] = *reinterpret_cast<const i32x4*>(codes + lane % 16 * kPitch + 64 * s + lane / 16 * 16);
-    const float qs = row_scale[lane % 16];
+    const f32x4a4 qs = *reinterpret_cast<const f32x4a4*>(row_scale + lane / 16 * 4);
+    // The lane's 16 bytes of each unit (past the bounds: their first, which meet zeros), their
+    // place in `stage`, and those of the product's: of page lane % 16, of the unit's first half.
+    int off[kUnits];
+#pragma unroll
+    for (int u = 0; u < kUnits; u++) off[u] = 128 * u + lane % 8 * 16 < 2 * D ? 128 * u + lane % 8 * 16 : 0;
+    uint8_t* const put = stage[wave] + lane / 8 * 128 + ((lane % 8 ^ lane / 8) << 4);
+    const uint8_t* const get = stage[wave] + lane % 16 * 128;
+    const int get_at = (lane / 16 ^ lane % 8) << 4;
     if (h0) look_up(page, start);
     for (int p0 = start; p0 < top; p0 += kStride) {
-      i32x4 k[kAtOnce][kSteps];
+      u32x4 k[kAtOnce][kUnits][2];
       float ks[kAtOnce];
       bool there[kAtOnce];
 #pragma unroll
       for (int i = 0; i < kAtOnce; i++) {
         there[i] = page[i] >= 0 && page[i] < a.k.pages;
         const int id = there[i] ? page[i] : 0;
-        const int8_t* const src = a.k.codes + (size_t)id * a.k.page + (size_t)2 * g * D;
 #pragma unroll
-        for (int s = 0; s < kSteps; s++) k[i][s] = i32x4{0, 0, 0, 0};
-        if (a.k.pages && p0 + 16 * i < top) {
+        for (int j = 0; j < 2; j++) {
+          const int8_t* const src = a.k.codes +
+                                    (size_t)__shfl(id, lane / 8 + 8 * j, 64) * a.k.page +
+                                    (size_t)2 * g * D;
 #pragma unroll
-          for (int s = 0; s < kSteps; s++) {
-            // Sixteen channels from d on of one bound; those past D meet zeros.
-            const int c = 64 * s + lane / 16 * 16, d = c % DP;
-            const int8_t* const at = src + (c < DP ? 0 : D) + (d < D ? d : 0);
-            if (D % 16 == 0) {
-              k[i][s] = __builtin_bit_cast(i32x4, load_global<u32x4a8>(at));
-            } else {
-              const uint2 lo = load_global<uint2>(at);
-              const uint2 hi = load_global<uint2>(d + 8 < D ? at + 8 : at);
-              k[i][s] = i32x4{(int)lo.x, (int)lo.y, (int)hi.x, (int)hi.y};
-            }
-          }
+          for (int u = 0; u < kUnits; u++) k[i][u][j] = load_global<u32x4>(src + off[u]);
         }
-        ks[i] = there[i] ? load_global<float>(a.k.scale + (size_t)id * a.k.s_page + g) : 0.0f;
+        ks[i] = load_global<float>(a.k.scale + (size_t)id * a.k.s_page + g);
       }
       look_up(page, p0 + kStride);
 #pragma unroll
       for (int i = 0; i < kAtOnce; i++) {
         const int p = p0 + 16 * i + lane % 16;
-        if (p0 + 16 * i >= top) continue;
         i32x4 acc = {0, 0, 0, 0};
 #pragma unroll
-        for (int s = 0; s < kSteps; s++)
-          acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[i][s], q[s], acc, 0, 0, 0);
+        for (int u = 0; u < kUnits; u++) {
+          // (pages 8 on have the order of the first eight)
+          *reinterpret_cast<u32x4*>(put) = k[i][u][0];
+          *reinterpret_cast<u32x4*>(put + 8 * 128) = k[i][u][1];
+          wave_lds_sync();
+          i32x4 x[2];
 #pragma unroll
-        for (int j = 0; j < 4; j++) part[wave][lane / 16 * 4 + j][lane % 16] = (float)acc[j] * qs;
-        wave_lds_sync();
-        for (int tok = lane / 16; tok < nt; tok += 4) {
-          const float* const rows = part[wave][lane % 16] + (G <= 16 ? tok * G : 0);
-          float m = rows[0];
-          for (int h = 1; h < min(G - h0, 16); h++) m = fmaxf(m, rows[h]);
-          uint32_t key = key_of(m * ks[i]);
-          if (!there[i] || p > ((pos0 + tok) >> shift) - a.last) key = 0;
-          if (p < top) {
-            uint32_t* const to = keys + (size_t)tok * a.pitch + p;
-            *to = h0 ? max(*to, key) : key;
-          }
+          for (int s = 0; s < 2; s++)
+            x[s] = *reinterpret_cast<const i32x4*>(get + (get_at ^ s << 6));
+          wave_lds_sync();
+#pragma unroll
+          for (int s = 0; s < 2; s++)
+            acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(q[2 * u + s], x[s], acc, 0, 0, 0);
         }
-        wave_lds_sync();
+        // Rows lane / 16 * 4 on of page lane % 16.
+        float m[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) m[j] = (float)acc[j] * qs[j];
+        if (a.rows >= 2) m[0] = fmaxf(m[0], m[1]), m[1] = fmaxf(m[2], m[3]);
+        if (a.rows >= 4) m[0] = fmaxf(m[0], m[1]);
+        if (a.rows >= 8) m[0] = fmaxf(m[0], __shfl_xor(m[0], 16, 64));
+        if (a.rows >= 16) m[0] = fmaxf(m[0], __shfl_xor(m[0], 32, 64));
+        const int tokens = a.rows >= 4 ? 1 : 4 / a.rows;  // of a lane
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const int tok = lane / 16 * 4 / a.rows + j;
+          if (j >= tokens || tok >= nt || p >= top) continue;
+          uint32_t key = key_of(m[j] * ks[i]);
+          if (!there[i] || p > ((pos0 + tok) >> shift) - a.last) key = 0;
+          uint32_t* const to = keys + (size_t)tok * a.pitch + p;
+          *to = h0 ? max(*to, key) : key;
+        }
       }
     }
     __syncthreads();
@@ -354,20 +401,32 @@ __global__ void __launch_bounds__(64 * kWaves) select_pages_kernel(SelectArgs a)
     const int own = pos < 0 ? -1 : (int)(pos >> shift);
     const int lo = a.first, hi = min(most, own + 1 - a.last);
     const uint32_t* const key = keys + (size_t)tok * a.pitch;
+    // The candidates' keys, some a thread at once (0 past them); all lanes go through it.
+    auto each = [&](auto&& f) __attribute__((always_inline)) {
+      constexpr int kKeysAtOnce = 8;
+      for (int p0 = lo; p0 < hi; p0 += kKeysAtOnce * threads) {
+        uint32_t k[kKeysAtOnce];
+#pragma unroll
+        for (int i = 0; i < kKeysAtOnce; i++) {
+          const int p = p0 + i * threads + at;
+          k[i] = key[p < hi ? p : lo];
+          k[i] = p < hi ? k[i] : 0;
+        }
+#pragma unroll
+        for (int i = 0; i < kKeysAtOnce; i++)
+          if (p0 + i * threads < hi) f(k[i]);
+      }
+    };
     // Candidates, the smallest and largest key, over all threads.
     int all = 0;
     uint32_t low = 0xFFFFFFFFu, high = 0;
-    for (int p = lo + at; p - at < hi; p += threads) {
-      const uint32_t k = p < hi ? key[p] : 0;
+    each([&](uint32_t k) __attribute__((always_inline)) {
       all += __popcll(__ballot(k != 0));
       low = min(low, k ? k : 0xFFFFFFFFu);
       high = max(high, k);
-    }
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) {
-      low = min(low, (uint32_t)__shfl_xor((int)low, off, 64));
-      high = max(high, (uint32_t)__shfl_xor((int)high, off, 64));
-    }
+    });
+    low = ~wave_max(~low);
+    high = wave_max(high);
     if (kTeam) {
       if (lane == 0) ends[wave] = make_uint2(low, high), counts[wave].x = all;
       __syncthreads();
@@ -378,49 +437,45 @@ __global__ void __launch_bounds__(64 * kWaves) select_pages_kernel(SelectArgs a)
         all += counts[w].x;
       }
     }
-    // Keys above `least` are taken, and `ties` of those that are `least`; `left` of what
-    // agrees with `least` in the bits before `bits` are to be.
+    // Keys above `least` are taken, and `ties` of those that are `least`; `left` of the keys
+    // that agree with it in the bits from `bits` on are to be.
     const int need = a.count - a.first - a.last;
     uint32_t least = all ? low : 1;
     int ties = 0x7FFFFFFF, left = need;
     if (all > need && need > 0 && high > low) {
       // From the first bit in which keys differ on, up to eight bits at a time.
       int bits = 32 - __clz((int)(high - low));
-      least = 0;  // (of keys - low)
-      while (bits > 0) {
+      uint32_t span = 0xFFFFFFFFu;  // the keys' differences from `from` are at most this
+      uint32_t from = low;
+      while (true) {
         const int width = min(bits, 8), down = bits - width;
         for (int i = at; i < 256; i += threads) bins[i] = 0;
         lds_sync<kTeam>();
-        for (int p = lo + at; p < hi; p += threads) {
-          const uint32_t k = key[p];
-          if (k && ((uint64_t)(k - low) >> bits) == ((uint64_t)least >> bits))
-            atomicAdd(&bins[((k - low) >> down) & ((1u << width) - 1)], 1);
-        }
+        // (the largest first)
+        each([&](uint32_t k) __attribute__((always_inline)) {
+          const uint32_t d = k - from;
+          if (k >= from && d <= span) atomicAdd(&bins[(d >> down) ^ 255], 1);
+        });
         lds_sync<kTeam>();
-        // The bin in which the left-th from the top lies; a lane has four.
+        // The bin in which the left-th lies; a lane has four.
         const int4 c = *reinterpret_cast<const int4*>(bins + 4 * lane);
-        int above = c.x + c.y + c.z + c.w;
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-          const int x = __shfl_down(above, off, 64);
-          above += lane + off < 64 ? x : 0;
-        }
-        const int in = 63 - __clzll((long long)__ballot(above >= left));
-        const int4 d = make_int4(__shfl(c.x, in, 64), __shfl(c.y, in, 64), __shfl(c.z, in, 64),
-                                 __shfl(c.w, in, 64));
-        int over = __shfl(above, in, 64) - (d.x + d.y + d.z + d.w), bin = 4 * in + 3, here = d.w;
-        if (over + here < left) over += here, bin--, here = d.z;
-        if (over + here < left) over += here, bin--, here = d.y;
-        if (over + here < left) over += here, bin--, here = d.x;
-        left -= over;
-        least |= (uint32_t)bin << down;
+        const int upto = (int)wave_scan(c.x + c.y + c.z + c.w);
+        const int in = __ffsll((long long)__ballot(upto >= left)) - 1;
+        const int c0 = __builtin_amdgcn_readlane(c.x, in), c1 = __builtin_amdgcn_readlane(c.y, in);
+        const int c2 = __builtin_amdgcn_readlane(c.z, in), c3 = __builtin_amdgcn_readlane(c.w, in);
+        left -= __builtin_amdgcn_readlane(upto, in) - (c0 + c1 + c2 + c3);
+        int bin = 4 * in, here = c0;
+        if (left > here) left -= here, bin++, here = c1;
+        if (left > here) left -= here, bin++, here = c2;
+        if (left > here) left -= here, bin++, here = c3;
+        from += (uint32_t)(bin ^ 255) << down;
         bits = down;
         lds_sync<kTeam>();
-        if (here == left) break;  // all of the bin
+        if (here == left || bits == 0) break;  // (all of the bin, or one key's)
+        span = (1u << bits) - 1;
       }
+      least = from;
       if (bits == 0) ties = left;
-      least += low;
-      // (of a whole bin all keys are at least its first)
     } else if (all > need) {
       ties = need;
     }
@@ -477,13 +532,13 @@ __global__ void __launch_bounds__(64 * kWaves) select_pages_kernel(SelectArgs a)
 template <int DP>
 hipError_t run_select(const SelectArgs& a, size_t lds, bool team, hipStream_t s) {
   const size_t grid = ((size_t)a.b.tokens / a.tokens + a.b.batch) * a.k.kv_heads;
-  if (grid > 0x7FFFFFFF) return hipErrorInvalidValue;
-  const void* fn = team ? (const void*)select_pages_kernel<DP, 16, true>
+  if (grid > (team ? 0xFFFFFFFFu / (64 * kTeamWaves) : 0xFFFFFF)) return hipErrorInvalidValue;
+  const void* fn = team ? (const void*)select_pages_kernel<DP, kTeamWaves, true>
                         : (const void*)select_pages_kernel<DP, 4, false>;
   const hipError_t e = set_lds_limit(fn, (int)lds);
   if (e != hipSuccess) return e;
   if (team)
-    select_pages_kernel<DP, 16, true><<<(unsigned)grid, 1024, lds, s>>>(a);
+    select_pages_kernel<DP, kTeamWaves, true><<<(unsigned)grid, 64 * kTeamWaves, lds, s>>>(a);
   else
     select_pages_kernel<DP, 4, false><<<(unsigned)grid, 256, lds, s>>>(a);
   return hipGetLastError();
@@ -511,11 +566,13 @@ hipError_t launch_key_bounds(const KeyBounds& o, const KvCache& c, const KvBatch
 hipError_t launch_select_pages(int* out, int count, int first, int last, const float* q,
                                size_t q_stride, int heads, const KeyBounds& k, const KvBatch& b,
                                int pages, int num_cus, hipStream_t s) {
-  SelectArgs a = {k, b, out, q, q_stride, heads, heads / k.kv_heads, count, first, last, pages,
+  if (k.pages == 0) pages = 0;  // (nothing has a score)
+  SelectArgs a = {k, b, out, q, q_stride, heads, heads / k.kv_heads, count, first, last, 1, pages,
                   (pages + 3) / 4 * 4, 1};
-  a.tokens = std::max(1, 16 / a.group);
+  while (a.rows < 16 && a.rows < a.group) a.rows *= 2;
   const size_t room = 128 << 10;
-  a.tokens = (int)std::min<size_t>(a.tokens, std::max<size_t>(1, room / 4 / std::max(a.pitch, 1)));
+  a.tokens = (int)std::min<size_t>(16 / a.rows,
+                                   std::max<size_t>(1, room / 4 / std::max(a.pitch, 1)));
   const size_t groups = ((size_t)b.tokens / a.tokens + b.batch) * k.kv_heads;
   const bool team = pages > 2048 || (pages > 256 && groups <= (size_t)num_cus);
   const size_t lds = (size_t)a.tokens * a.pitch * 4;
