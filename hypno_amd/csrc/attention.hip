@@ -15,6 +15,7 @@ __global__ void __launch_bounds__(64) attn_rows_kernel(AttnArgs a) {
   const int b = find_seq(a.b, t, 0, 0);
   if (b < 0 || b >= a.b.batch) return;
   const Seq sq = seq_of(a.b, b);
+  if (t < sq.first || t - sq.first >= sq.n) return;  // (cu_q that does not ascend)
   attn_row(a, sq, t - sq.first, h,
            a.selected ? a.selected + ((size_t)t * a.c.kv_heads + h / a.group) * a.count : nullptr,
            a.count);

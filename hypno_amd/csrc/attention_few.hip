@@ -63,6 +63,7 @@ __global__ void __launch_bounds__(64 * kWaves, (kWaves == 8 ? 1 : Few<kType, DP>
   if (kList && (b < 0 || b >= a.b.batch)) return;
   const Seq sq = seq_of(a.b, b);
   const int ti0 = kList ? unit - sq.first : 0;  // (the token in its sequence)
+  if (kList && (ti0 < 0 || ti0 >= sq.n)) return;  // (cu_q that does not ascend)
   const int rows = kList ? G : sq.n * G;
   if (!kList && rows > a.few) return;
   const bool past = too_long(a, sq);

@@ -110,6 +110,12 @@ __global__ void __launch_bounds__(256, 2) attn_tile_kernel(AttnArgs a) {
     ch[i] = 8 * ((j % L::kCh) ^ L::swz(rr[i]));
     if (ch[i] >= D) ch[i] = 0;  // (columns past D: products with zeros, outputs not used)
   }
+  // 4-bit: the row of a wave's group j.  Rows four apart follow each other, as their pieces
+  // then lie in different banks when they are stored.
+  auto group_row = [&](int j) __attribute__((always_inline)) {
+    const int r = j / (DP / kFp4Group);
+    return r % (kMine / 4) * 4 + r / (kMine / 4);
+  };
   auto look_up = [&](int p0) __attribute__((always_inline)) {
     if (kOne) {
       id = load_const<int>(a.b.page_table + (size_t)b * a.b.width +
@@ -139,7 +145,7 @@ __global__ void __launch_bounds__(256, 2) attn_tile_kernel(AttnArgs a) {
       for (int i = 0; i < T::kNg; i++) {
         // (lanes past the groups, and groups past D: the row's first)
         const int j = min(i * 64 + lane, T::kG - 1), blk = j % (DP / kFp4Group);
-        const int tok = min(p0 + wave * kMine + j / (DP / kFp4Group), hi - 1) & mask;
+        const int tok = min(p0 + wave * kMine + group_row(j), hi - 1) & mask;
         const int at = blk < B ? blk : 0;
         const uint32_t off = __umul24(tok, D / 2) + at * 16, so = (at << a.c.page_shift) + tok;
         kr4[i] = load_global<u32x4>(kp + off);
@@ -197,7 +203,7 @@ __global__ void __launch_bounds__(256, 2) attn_tile_kernel(AttnArgs a) {
       for (int i = 0; i < T::kNg; i++) {
         const int j = i * 64 + lane, blk = j % (DP / kFp4Group);
         if (T::kG % 64 && j >= T::kG) continue;
-        const int r = wave * kMine + j / (DP / kFp4Group);
+        const int r = wave * kMine + group_row(j);
         const half2v ks = {ks4[i], ks4[i]}, vs = {vs4[i], vs4[i]};
 #pragma unroll
         for (int c = 0; c < 4; c++) {

@@ -211,6 +211,37 @@ def test_long_context():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("page", [16, 32])
+@pytest.mark.parametrize("window", [0, 3000, 4999])
+def test_ranges(page, window):
+    """Ranges where pages are a run or two, and from the start of a window on; sequences of
+    several tokens among as many as there are tokens."""
+    for seqs in ([(1, 7777)], [(1, 9000), (1, 33), (1, 4100)],
+                 [(5, 5300), (0, 10), (0, 0), (3, 6001), (0, 5), (0, 7), (1, 40), (0, 3), (0, 1)]):
+        for heads, kv_heads, dim in ((4, 1, 64), (7, 1, 128), (9, 1, 32)):
+            bt = Batch4(seqs, page, 20, kv_heads=kv_heads, dim=dim)
+            q = queries(bt.tokens, heads, dim, 20)
+            check(run_attend(bt, q, window=window), *attend(q, bt, window=window))
+
+
+@pytest.mark.gpu
+def test_cu_q_that_does_not_ascend():
+    """Nothing is read or written out of place; what the outputs hold is not said."""
+    import torch
+    bt = Batch4([(1, 100), (1, 40), (2, 60)], 16, 21)
+    q = torch.from_numpy(queries(4, 4, 64, 21)).cuda()
+    x = torch.randn(4, 2, 64, device="cuda")
+    sel = torch.zeros(4, 2, 3, dtype=torch.int32, device="cuda")
+    for cu in ([0, 3, 1, 4], [4, 3, 2, 1], [0, -5, 90, 4], [2, 2, 0, 2 ** 31 - 1]):
+        a = bt.gpu()
+        a["cu_q"] = torch.tensor(cu, dtype=torch.int32, device="cuda")
+        hk.append_kv(q, x, x, **a)
+        hk.paged_attention(q, **a)
+        hk.selected_attention(q, selected=sel, **a)
+    torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
 def test_captured():
     """append and attention in a graph, replayed over other tokens with eager work between."""
     import torch
