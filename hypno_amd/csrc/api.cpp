@@ -1587,8 +1587,11 @@ int hypno_hip_select_pages_dev(int32_t* selected, size_t count, size_t first, si
     st = device_state(&ds);
     if (st) return st;
   }
-  hipError_t e = launch_select_pages(selected, (int)count, (int)first, (int)last, q, q_stride,
-                                     (int)heads, o, b, (int)pages, ds->cus, (hipStream_t)stream);
+  const SelectPlan p = select_plan((int)heads, o, b, (int)pages, ds->cus);
+  WsLock ws;
+  if (p.bytes) (void)try_workspace(ds, (hipStream_t)stream, p.bytes, ws);
+  hipError_t e = launch_select_pages(p, selected, (int)count, (int)first, (int)last, q, q_stride,
+                                     (int)heads, o, b, ws.p, (hipStream_t)stream);
   return e == hipSuccess ? HYPNO_HIP_OK : hip_fail(e, "select_pages launch");
 }
 

@@ -116,10 +116,19 @@ constexpr int kMaxSelected = 1024;
 
 hipError_t launch_key_bounds(const KeyBounds& o, const KvCache& c, const KvBatch& b, int num_cus,
                              hipStream_t s);
+// How a call's tokens and pages are split over work-groups, and the workspace that takes.
+struct SelectPlan {
+  int pages;       // of a sequence
+  int pitch, rows, tokens, splits, chunk;
+  bool team;
+  size_t bytes;
+};
 // `pages`: of a sequence, at most kMaxScored.
-hipError_t launch_select_pages(int* out, int count, int first, int last, const float* q,
-                               size_t q_stride, int heads, const KeyBounds& k, const KvBatch& b,
-                               int pages, int num_cus, hipStream_t s);
+SelectPlan select_plan(int heads, const KeyBounds& k, const KvBatch& b, int pages, int num_cus);
+// ws: plan.bytes, or NULL (one kernel then).
+hipError_t launch_select_pages(const SelectPlan& p, int* out, int count, int first, int last,
+                               const float* q, size_t q_stride, int heads, const KeyBounds& k,
+                               const KvBatch& b, void* ws, hipStream_t s);
 // How the positions of a tile of rows are split: into ranges of `chunk`, the last
 // one of `splits` taking what is left.
 struct AttnSplit {

@@ -172,7 +172,12 @@ struct SelectArgs {
   int most;    // pages of a sequence that have a score at most
   int pitch;   // of a token's keys in LDS
   int tokens;  // of a work-group
+  int splits, chunk;  // of pages, whose scores a work-group of the first of two kernels takes
+  uint32_t* scores;   // [tokens][kv_heads][pitch], between the two
 };
+
+// What a launch does: both steps, or one of them.
+constexpr int kBoth = 0, kScores = 1, kChoice = 2;
 
 // Scores as whole numbers in their order, from 1 on; 0: no candidate.  (What is no
 // number, and infinities, as the largest finite one: below what is always selected.)
@@ -234,7 +239,7 @@ __device__ __forceinline__ void lds_sync() {
 // the next four's numbers with them.  A page's two bounds are one piece of memory, 128 bytes
 // of which eight lanes read; lanes that each read of another page, as the product takes
 // them, take four times as long (16 us for 2048 pages), so that they change places in LDS.
-template <int DP, int kWaves, bool kTeam>
+template <int DP, int kWaves, bool kTeam, int kStep>
 __global__ void __launch_bounds__(64 * kWaves, DP > 128 ? 2 : kTeam ? 2 : 4)
     select_pages_kernel(SelectArgs a) {
   constexpr int kSteps = 2 * DP / 64, kPitch = 2 * DP + 16, kAtOnce = (kTeam ? 4 : 2) / (DP > 128 ? 2 : 1);
@@ -248,7 +253,8 @@ __global__ void __launch_bounds__(64 * kWaves, DP > 128 ? 2 : kTeam ? 2 : 4)
   extern __shared__ uint32_t keys[];  // [tokens][pitch]
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int KV = a.k.kv_heads, G = a.group, D = a.k.head_dim, shift = a.k.page_shift;
-  const int g = blockIdx.x % KV, slot = blockIdx.x / KV;
+  const int slots = gridDim.x / KV / (kStep == kScores ? a.splits : 1);
+  const int g = blockIdx.x % KV, slot = blockIdx.x / KV % slots, split = blockIdx.x / KV / slots;
   const int b = find_seq(a.b, slot, 1, a.tokens);
   if (b < 0 || b >= a.b.batch) return;
   const int first = cu_at(a.b, b), n = cu_at(a.b, b + 1) - first;
@@ -258,12 +264,20 @@ __global__ void __launch_bounds__(64 * kWaves, DP > 128 ? 2 : kTeam ? 2 : 4)
   // The page of token i of the tile is (pos0 + i) >> shift: -1 and less if it has no place.
   const int64_t pos0 = (int64_t)load_global<int>(a.b.kv_lens + b) - n + i0;
   const int most = min(a.most, a.b.width);
-  const int top = (int)min((int64_t)most, ((pos0 + nt - 1) >> shift) + 1 - a.last);
+  int top = (int)min((int64_t)most, ((pos0 + nt - 1) >> shift) + 1 - a.last), bottom = a.first;
+  if (kStep == kScores) {
+    bottom = (int)min((int64_t)a.first + (int64_t)split * a.chunk, (int64_t)max(top, a.first));
+    top = (int)min((int64_t)top, (int64_t)bottom + a.chunk);
+  }
+  // Keys of the tile's token i: [pitch] from `keys_of` on, `keys_step` apart.
+  uint32_t* const all_keys = a.scores + ((size_t)t0 * KV + g) * a.pitch;
+  uint32_t* const keys_of = kStep == kScores ? all_keys : keys;
+  const size_t keys_step = kStep == kScores ? (size_t)KV * a.pitch : a.pitch;
   const int* const table = a.b.page_table + (size_t)b * a.b.width;
   // A wave's pages: 16 kAtOnce in a row, then those 16 kAtOnce kWaves on; a lane looks up
   // lane % 16 of each 16, and reads of lane / 8 and 8 on.
   constexpr int kStride = 16 * kAtOnce * kWaves;
-  const int start = a.first + 16 * kAtOnce * wave;
+  const int start = bottom + 16 * kAtOnce * wave;
   auto look_up = [&](int (&page)[kAtOnce], int p0) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < kAtOnce; i++) {
@@ -272,9 +286,9 @@ __global__ void __launch_bounds__(64 * kWaves, DP > 128 ? 2 : kTeam ? 2 : 4)
     }
   };
   int page[kAtOnce];
-  look_up(page, start);
+  if (kStep != kChoice) look_up(page, start);
 
-  for (int h0 = 0; h0 < G && top > a.first; h0 += 16) {
+  for (int h0 = 0; kStep != kChoice && h0 < G && top > bottom; h0 += 16) {
     // The rows' codes, [negative part][positive part][zeros]; 16 lanes a row.
     if (wave < 4) {
       const int r = tid / 16, sub = tid % 16;
@@ -386,11 +400,20 @@ __global__ void __launch_bounds__(64 * kWaves, DP > 128 ? 2 : kTeam ? 2 : 4)
           if (j >= tokens || tok >= nt || p >= top) continue;
           uint32_t key = key_of(m[j] * ks[i]);
           if (!there[i] || p > ((pos0 + tok) >> shift) - a.last) key = 0;
-          uint32_t* const to = keys + (size_t)tok * a.pitch + p;
+          uint32_t* const to = keys_of + tok * keys_step + p;
           *to = h0 ? max(*to, key) : key;
         }
       }
     }
+    __syncthreads();
+  }
+
+  if (kStep == kScores) return;
+  if (kStep == kChoice) {
+    for (int tok = 0; tok < nt; tok++)
+      for (int p = bottom + tid; p < top; p += 64 * kWaves)
+        keys[(size_t)tok * a.pitch + p] =
+            load_global<uint32_t>(all_keys + (size_t)tok * KV * a.pitch + p);
     __syncthreads();
   }
 
@@ -529,19 +552,26 @@ __global__ void __launch_bounds__(64 * kWaves, DP > 128 ? 2 : kTeam ? 2 : 4)
   }
 }
 
-template <int DP>
-hipError_t run_select(const SelectArgs& a, size_t lds, bool team, hipStream_t s) {
-  const size_t grid = ((size_t)a.b.tokens / a.tokens + a.b.batch) * a.k.kv_heads;
-  if (grid > (team ? 0xFFFFFFFFu / (64 * kTeamWaves) : 0xFFFFFF)) return hipErrorInvalidValue;
-  const void* fn = team ? (const void*)select_pages_kernel<DP, kTeamWaves, true>
-                        : (const void*)select_pages_kernel<DP, 4, false>;
-  const hipError_t e = set_lds_limit(fn, (int)lds);
+template <int DP, int kWaves, bool kTeam, int kStep>
+hipError_t run_step(const SelectArgs& a, hipStream_t s) {
+  const size_t groups = ((size_t)a.b.tokens / a.tokens + a.b.batch) * a.k.kv_heads;
+  const size_t grid = kStep == kScores ? groups * a.splits : groups;
+  const size_t lds = kStep == kScores ? 0 : (size_t)a.tokens * a.pitch * 4;
+  if (grid > 0xFFFFFFFFu / (64 * kWaves)) return hipErrorInvalidValue;
+  const hipError_t e =
+      set_lds_limit((const void*)select_pages_kernel<DP, kWaves, kTeam, kStep>, (int)lds);
   if (e != hipSuccess) return e;
-  if (team)
-    select_pages_kernel<DP, kTeamWaves, true><<<(unsigned)grid, 64 * kTeamWaves, lds, s>>>(a);
-  else
-    select_pages_kernel<DP, 4, false><<<(unsigned)grid, 256, lds, s>>>(a);
+  select_pages_kernel<DP, kWaves, kTeam, kStep><<<(unsigned)grid, 64 * kWaves, lds, s>>>(a);
   return hipGetLastError();
+}
+
+template <int DP>
+hipError_t run_select(const SelectArgs& a, bool team, hipStream_t s) {
+  if (a.splits > 1) {
+    const hipError_t e = run_step<DP, 4, false, kScores>(a, s);
+    return e == hipSuccess ? run_step<64, kTeamWaves, true, kChoice>(a, s) : e;
+  }
+  return team ? run_step<DP, kTeamWaves, true, kBoth>(a, s) : run_step<DP, 4, false, kBoth>(a, s);
 }
 
 }  // namespace
@@ -563,22 +593,39 @@ hipError_t launch_key_bounds(const KeyBounds& o, const KvCache& c, const KvBatch
   return hipGetLastError();
 }
 
-hipError_t launch_select_pages(int* out, int count, int first, int last, const float* q,
-                               size_t q_stride, int heads, const KeyBounds& k, const KvBatch& b,
-                               int pages, int num_cus, hipStream_t s) {
-  if (k.pages == 0) pages = 0;  // (nothing has a score)
-  SelectArgs a = {k, b, out, q, q_stride, heads, heads / k.kv_heads, count, first, last, 1, pages,
-                  (pages + 3) / 4 * 4, 1};
-  while (a.rows < 16 && a.rows < a.group) a.rows *= 2;
-  const size_t room = 128 << 10;
-  a.tokens = (int)std::min<size_t>(16 / a.rows,
-                                   std::max<size_t>(1, room / 4 / std::max(a.pitch, 1)));
-  const size_t groups = ((size_t)b.tokens / a.tokens + b.batch) * k.kv_heads;
-  const bool team = pages > 2048 || (pages > 256 && groups <= (size_t)num_cus);
-  const size_t lds = (size_t)a.tokens * a.pitch * 4;
-  return k.head_dim <= 64    ? run_select<64>(a, lds, team, s)
-         : k.head_dim <= 128 ? run_select<128>(a, lds, team, s)
-                             : run_select<256>(a, lds, team, s);
+SelectPlan select_plan(int heads, const KeyBounds& k, const KvBatch& b, int pages, int num_cus) {
+  SelectPlan p = {};
+  p.pages = k.pages ? pages : 0;  // (none: nothing has a score)
+  p.pitch = (p.pages + 3) / 4 * 4;
+  p.rows = 1;
+  while (p.rows < 16 && p.rows < heads / k.kv_heads) p.rows *= 2;
+  p.tokens = std::max(1, std::min(16 / p.rows, kMaxScored / std::max(p.pitch, 1)));
+  const size_t groups = ((size_t)b.tokens / p.tokens + b.batch) * k.kv_heads;
+  // Single tokens, and many pages: all of a work-group's waves look for one token's pages.
+  p.team = p.pages > 2048 || (p.pages > 256 && (groups <= (size_t)num_cus || b.tokens <= b.batch));
+  // Few work-groups: the pages' scores by as many as the chip holds, 128 pages or more each,
+  // and the choice by a kernel after them (one token over 2048 pages 19.9 us in one kernel).
+  p.splits = 1;
+  if (p.team && p.pages >= 1024 && 2 * groups <= (size_t)num_cus) {
+    const int n = (int)std::min<size_t>((size_t)num_cus / groups, (p.pages + 127) / 128);
+    p.chunk = ((p.pages + n - 1) / n + 127) / 128 * 128;
+    p.splits = (p.pages + p.chunk - 1) / p.chunk;
+    p.bytes = (size_t)b.tokens * k.kv_heads * p.pitch * 4;
+  }
+  return p;
+}
+
+hipError_t launch_select_pages(const SelectPlan& p, int* out, int count, int first, int last,
+                               const float* q, size_t q_stride, int heads, const KeyBounds& k,
+                               const KvBatch& b, void* ws, hipStream_t s) {
+  SelectArgs a = {};
+  a.k = k, a.b = b, a.out = out, a.q = q, a.q_stride = q_stride, a.heads = heads;
+  a.group = heads / k.kv_heads, a.count = count, a.first = first, a.last = last;
+  a.rows = p.rows, a.most = p.pages, a.pitch = p.pitch, a.tokens = p.tokens;
+  a.splits = ws ? p.splits : 1, a.chunk = p.chunk, a.scores = (uint32_t*)ws;
+  return k.head_dim <= 64    ? run_select<64>(a, p.team, s)
+         : k.head_dim <= 128 ? run_select<128>(a, p.team, s)
+                             : run_select<256>(a, p.team, s);
 }
 
 }  // namespace hypno
