@@ -3,9 +3,11 @@ appended with their rotation, attention over the pages, the gated MLP.  A prompt
 through in two chunks and tokens follow one by one (each the layer's last output, in
 place of an embedded token); the same rows as one prompt have to give the same outputs.
 
-    python examples/paged_decode.py [--prompt 500] [--tokens 20] [--int8]
+    python examples/paged_decode.py [--prompt 500] [--tokens 20] [--int8 | --fp4] [--pages N]
 
-The layer has TinyLlama-1.1B's sizes and random weights.
+With --pages, tokens after the prompt read only the N pages of their context that
+score highest (the first and the last two always); while N is all of them the
+outputs are the same.  The layer has TinyLlama-1.1B's sizes and random weights.
 """
 import argparse
 import os
@@ -40,35 +42,51 @@ class Layer:
         hk.batch_matmul(y, q, hk.DType.Q4_0, x, n, m, x.shape[0])
         return y
 
-    def __call__(self, x, cache, table, kv_lens, cu_q, max_kv_len):
-        """x: the new tokens' rows; kv_lens counts them already."""
+    def __call__(self, x, cache, bounds, table, kv_lens, cu_q, max_kv_len, pages=0):
+        """x: the new tokens' rows; kv_lens counts them already.  pages: that each token
+        reads (0: all)."""
         t = x.shape[0]
         y = self.product(hk.rms_norm(x, self.norms[0], EPS, t), self.qkv).view(t, -1, DIM)
         q, k, v = y.split([HEADS, KV_HEADS, KV_HEADS], 1)
-        q = hk.append_kv(q, k, v, page_table=table, kv_lens=kv_lens, cu_q=cu_q,
-                         inv_freq=self.inv_freq, **cache)
-        a = hk.paged_attention(q, page_table=table, kv_lens=kv_lens, cu_q=cu_q,
-                               max_kv_len=max_kv_len, **cache)
+        batch = dict(page_table=table, kv_lens=kv_lens, cu_q=cu_q)
+        q = hk.append_kv(q, k, v, inv_freq=self.inv_freq, **batch, **cache)
+        hk.key_bounds(cache["k_cache"], *bounds, **batch, k_scale=cache.get("k_scale"))
+        if pages:
+            chosen = hk.select_pages(q, *bounds, PAGE, **batch, count=pages, last=2,
+                                     max_kv_len=max_kv_len)
+            a = hk.selected_attention(q, selected=chosen, **batch, **cache)
+        else:
+            a = hk.paged_attention(q, max_kv_len=max_kv_len, **batch, **cache)
         x = x + self.product(a.view(t, -1), self.o)
         y = hk.rms_norm(x, self.norms[1], EPS, t)
         return x + self.product(hk.silu_mul(self.product(y, self.gate), self.product(y, self.up)),
                                 self.down)
 
 
-def new_cache(pages, int8):
-    shape = (pages, KV_HEADS, PAGE, DIM)
-    dtype = torch.int8 if int8 else torch.float16
+def new_cache(pages, kind):
+    """A cache and the bounds of its keys."""
+    shape, scales = (pages, KV_HEADS, PAGE, DIM), None
+    dtype = {"fp16": torch.float16, "int8": torch.int8, "fp4": torch.uint8}[kind]
+    if kind == "int8":
+        scales = torch.zeros(shape[:3], device="cuda")
+    elif kind == "fp4":
+        shape = (*shape[:3], DIM // 2)
+        scales = torch.zeros(pages, KV_HEADS, DIM // 32, PAGE, dtype=torch.float16, device="cuda")
     c = {n: torch.zeros(shape, dtype=dtype, device="cuda") for n in ("k_cache", "v_cache")}
-    if int8:
-        c.update({n: torch.zeros(shape[:3], device="cuda") for n in ("k_scale", "v_scale")})
-    return c
+    if scales is not None:
+        c.update({n: scales.clone() for n in ("k_scale", "v_scale")})
+    return c, (torch.zeros(pages, KV_HEADS, 2, DIM, dtype=torch.int8, device="cuda"),
+               torch.zeros(pages, KV_HEADS, device="cuda"))
 
 
 def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("--prompt", type=int, default=500)
     ap.add_argument("--tokens", type=int, default=20)
-    ap.add_argument("--int8", action="store_true")
+    kinds = ap.add_mutually_exclusive_group()
+    kinds.add_argument("--int8", dest="kind", action="store_const", const="int8", default="fp16")
+    kinds.add_argument("--fp4", dest="kind", action="store_const", const="fp4")
+    ap.add_argument("--pages", type=int, default=0)
     a = ap.parse_args()
     total = a.prompt + a.tokens
     pages = -(-total // PAGE)
@@ -80,7 +98,7 @@ def main():
     def ints(*x):
         return torch.tensor(x, dtype=torch.int32, device="cuda")
 
-    cache, out, done = new_cache(pages, a.int8), [], 0
+    (cache, bounds), out, done = new_cache(pages, a.kind), [], 0
     half = a.prompt // 2
     chunks = [rows[:half], rows[half:]] if half else [rows]
     for i in range(len(chunks) + a.tokens):
@@ -88,14 +106,19 @@ def main():
         if i >= len(chunks):
             rows = torch.cat([rows, x])
         done += x.shape[0]
-        out.append(layer(x, cache, table, ints(done), ints(0, x.shape[0]), done))
+        out.append(layer(x, cache, bounds, table, ints(done), ints(0, x.shape[0]), done,
+                         a.pages if i >= len(chunks) else 0))
     out = torch.cat(out)
-    whole = layer(rows, new_cache(pages, a.int8), table, ints(total), ints(0, total), total)
+    whole = layer(rows, *new_cache(pages, a.kind), table, ints(total), ints(0, total), total)
     # The products of many rows take activations in fp16 (2e-3 in the L2 norm), those of
-    # one row in fp32; 8-bit codes of values that differ so differ by a step at most.
+    # one row in fp32; 8-bit codes of values that differ so differ by a step at most, and
+    # one in a hundred 4-bit ones by a step, half of a value: 5e-2 in the L2 norm.
     err = ((out - whole).norm() / whole.norm()).item()
     print(f"prompt of {a.prompt} and {a.tokens} tokens against one prompt: {err:.1e}")
-    if not err < 1e-2:
+    if 0 < a.pages < pages:
+        print(f"with {a.pages} of {pages} pages")
+        return
+    if not err < (5e-2 if a.kind == "fp4" else 1e-2):
         sys.exit("outputs differ")
     print("agree")
 

@@ -235,14 +235,15 @@ __device__ __forceinline__ void lds_sync() {
 // own tokens'.
 //
 // Latency is what there is to save: a page's number, its bounds, the counts are reads that
-// depend on each other, so that a wave asks for four products' pages at a time, and for
-// the next four's numbers with them.  A page's two bounds are one piece of memory, 128 bytes
+// depend on each other, so that a wave asks for two products' pages at a time, and for the
+// next two's numbers with them (four: a third of the waves less, and 5 to 10% longer where
+// work-groups fill the chip).  A page's two bounds are one piece of memory, 128 bytes
 // of which eight lanes read; lanes that each read of another page, as the product takes
 // them, take four times as long (16 us for 2048 pages), so that they change places in LDS.
 template <int DP, int kWaves, bool kTeam, int kStep>
-__global__ void __launch_bounds__(64 * kWaves, DP > 128 ? 2 : kTeam ? 2 : 4)
+__global__ void __launch_bounds__(64 * kWaves, DP > 128 ? 2 : 4)
     select_pages_kernel(SelectArgs a) {
-  constexpr int kSteps = 2 * DP / 64, kPitch = 2 * DP + 16, kAtOnce = (kTeam ? 4 : 2) / (DP > 128 ? 2 : 1);
+  constexpr int kSteps = 2 * DP / 64, kPitch = 2 * DP + 16, kAtOnce = DP > 128 ? 1 : 2;
   constexpr int kUnits = 2 * DP / 128;  // of 128 bytes of the bounds
   __shared__ __attribute__((aligned(16))) uint8_t codes[16 * kPitch];
   __shared__ __attribute__((aligned(16))) float row_scale[16];

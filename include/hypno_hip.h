@@ -544,7 +544,9 @@ int hypno_hip_key_bounds_dev(const hypno_hip_key_bounds* bounds, const hypno_hip
  * the largest one.  Pages that are none of the cache's, or past the table or max_kv_len,
  * have no score.  A token at a negative position selects nothing; rows of no sequence are
  * left alone.  max_kv_len: an upper bound of kv_lens (0: table_width * page_size), at most
- * 32768 pages.  count: at most 1024; first + last at most count. */
+ * 32768 pages.  count: at most 1024; first + last at most count.  Few tokens' scores of many
+ * pages use the stream's workspace; under capture, without one that is large enough, they do
+ * not (the choice is the same). */
 int hypno_hip_select_pages_dev(int32_t* selected, size_t count, size_t first, size_t last,
                                const float* q, size_t q_stride, size_t heads,
                                const hypno_hip_key_bounds* bounds,
@@ -553,7 +555,7 @@ int hypno_hip_select_pages_dev(int32_t* selected, size_t count, size_t first, si
 /* paged_attention over the positions p <= the token's own that are in one of the pages
  * selected[t][g][0..count) (of kv head g = h / (heads / kv_heads)): numbers below 0 or
  * past the token's own page are passed over, and a page that is named twice counts twice.
- * Arithmetic, zeros and NaN as there; pages of 16 tokens at least. */
+ * Arithmetic, zeros, NaN and workspace as there; pages of 16 tokens at least. */
 int hypno_hip_selected_attention_dev(float* out, const float* q, size_t q_stride, size_t heads,
                                      const hypno_hip_kv_cache* cache,
                                      const hypno_hip_kv_batch* batch, float scale,

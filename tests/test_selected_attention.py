@@ -3,12 +3,16 @@ and codes bit for bit, attention within test_paged_attention's bounds; runs of t
 together, and their refusals."""
 import ctypes
 import math
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
 
 import hypno_amd as hk
 from hypno_amd import _lib, attention
+from conftest import ROOT
 from test_fp4_cache import Batch4
 from test_paged_attention import EPS, O, Q, Batch, _kv, check, queries
 
@@ -550,6 +554,83 @@ def test_together(kind):
         assert torch.equal(got[0], want)
         # (the graph's positions may be split into other ranges)
         assert torch.allclose(got[1], ref, rtol=1e-4, atol=1e-5)
+
+
+def long_step(bt, seed):
+    """A function that chooses pages of a long context and attends to them and to all, and
+    what it gives, checked."""
+    import torch
+    q, a = torch.from_numpy(queries(bt.tokens, 4, bt.dim, seed)).cuda(), bt.gpu()
+    bounds = old_bounds(bt, seed)
+    codes, scale = (torch.from_numpy(x).cuda() for x in bounds)
+    where = {n: a[n] for n in ("page_table", "kv_lens", "cu_q")}
+
+    def step():
+        sel = hk.select_pages(q, codes, scale, bt.page, count=90, **where)
+        return sel, hk.selected_attention(q, selected=sel, **a), hk.paged_attention(q, **a)
+
+    want = [x.clone() for x in step()]
+    x, sel = q.cpu().numpy(), want[0].cpu().numpy()
+    assert np.array_equal(sel, select(bt, x, *bounds, 90))
+    check(want[1].cpu().numpy(), *attend_selected(x, bt, sel))
+    return step, want
+
+
+def same(got, want):
+    import torch
+    assert torch.equal(got[0], want[0])
+    for x, y in zip(got[1:], want[1:]):  # (other ranges of positions)
+        assert torch.allclose(x, y, rtol=1e-4, atol=1e-5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+def test_captured_without_a_workspace(kind):
+    """On a stream that never had one: neither pages nor positions are split."""
+    import torch
+    step, want = long_step(batch(kind, [(1, 40000)], 16, 58, kv_heads=1), 58)
+    side = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        got = step()
+    for _ in range(3):
+        for x in got:
+            x.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        same(got, want)
+        same(step(), want)
+
+
+@pytest.mark.gpu
+def test_streams_side_by_side():
+    """Each stream has a workspace of its own."""
+    import torch
+    steps = [long_step(batch(k, [(1, 30000 + 3000 * i)], 16, 59 + i, kv_heads=1), 59 + i)
+             for i, k in enumerate(KINDS)]
+    streams = [torch.cuda.Stream() for _ in steps]
+    torch.cuda.synchronize()
+    got = [[] for _ in steps]
+    for _ in range(5):
+        for (step, _), stream, out in zip(steps, streams, got):
+            with torch.cuda.stream(stream):
+                out.append(step())
+    torch.cuda.synchronize()
+    for (_, want), out in zip(steps, got):
+        for x in out:
+            assert all(torch.equal(y, z) for y, z in zip(x, want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("args", [["--fp4"], ["--pages", "5"], ["--fp4", "--pages", "4"],
+                                  ["--int8", "--pages", "3"]], ids=" ".join)
+def test_example(args):
+    """examples/paged_decode.py: a layer's prompt and tokens through all operators."""
+    p = subprocess.run([sys.executable, os.path.join(ROOT, "examples", "paged_decode.py"),
+                        "--prompt", "70", "--tokens", "5", *args], capture_output=True, text=True,
+                       timeout=100)
+    assert p.returncode == 0, p.stderr
+    assert ("agree" if args in (["--fp4"], ["--pages", "5"]) else "pages") in p.stdout
 
 
 # --- arguments ------------------------------------------------------------------------------------
