@@ -3,13 +3,22 @@
 // sequence and a range of its positions, its waves run through tiles of 32 keys on their
 // own and add up at the end) on codes that stay 4 bits wide up to the registers.
 //
-// A run of 16 keys of a kv head is one piece of memory, codes as well as each group's
-// scales: whole runs are copied into a wave's own LDS, kAhead tiles before they are used.
-// K: lane (key, quarter) reads its quarter of the key's codes, which has one scale or two,
-// as they are; q is held in the same order.  V: the 4-bit transposing read gives a lane
-// eight keys' codes of two channels, the scales lie key by key already.  Both become fp16
-// code * scale, rounded once (the values that the cache stands for), two a conversion and
-// a product.
+// A run of keys of a kv head in one page is one piece of memory, codes as well as each
+// group's scales: whole runs are copied into a wave's own LDS, a tile before they are used
+// (two or three ahead: no more bytes a second, and LDS for fewer work-groups; 87 us below
+// become 107).  What is copied past the last key is masked, its scales of V set to 0.
+// K: lane (key, quarter) reads its quarter of the key's codes as they are, each eight of
+// which have one scale; q is held in the same order.  V: the 4-bit transposing read gives a
+// lane eight keys' codes of two channels, the scales lie key by key already.  Both become
+// fp16 code * scale, rounded once (the values that the cache stands for), two a conversion
+// and a product: 128 of some 210 vector operations a tile.
+//
+// Bound: HBM for long contexts (from 524288 to 1048576 positions of 8 kv heads of 128, 604 MB
+// more take 99 us more: 6.1 TB/s); starts, ends and the join for shorter ones.  One token over
+// 131072 (151 MB) 33 us and 5 to join, 64 sequences of up to 8192 (340 MB) 77 and 5, 4.1 TB/s;
+// with every product twice (kPass 16, three work-groups a CU) the latter takes 91.  700
+// positions of 32/4 heads of 64: 8.0 us, dependent reads of the sequence's place, its page and
+// keys, three tiles, the waves' sum.
 #include "attention_few.hpp"
 
 namespace hypno {

@@ -16,6 +16,8 @@
 //  * Rows of one kv head from all of its query heads: K and V are read once for the group,
 //    and a causal tile ends after 128 / group tokens.
 //  * Work-groups of one kv head share an XCD's L2 (see the order in the kernel).
+//  * 4-bit codes become fp16 values on their way into LDS, 64 vector operations a tile for a
+//    thread's 32 keys and 32 values: 512 tokens over 16384 266 us, of fp16 ones 254.
 // A prompt of 2048: 80 us; its longest work-group's 32 tiles one after the other are 60
 // of it, the last of them alone on a CU whose short work-group has ended.  512 tokens over
 // 16384: 258 us, 15 of them to join four ranges.

@@ -15,7 +15,8 @@
 // x / s in fp32.
 //
 // Bound: HBM for prompts (2048 tokens, 32/8 heads of 128, 92 MB: 20.6 us, 4.5 TB/s, a
-// large copy's 4.9; 999 tokens into an 8-bit cache 9.8, 1.2 TB/s), latency for few tokens (one: 4.2 us, of which an empty kernel is
+// large copy's 4.9; into a 4-bit one, 85 MB, 23.5, where an fp16 one takes 22.9 on the same
+// card; 999 tokens into an 8-bit cache 9.8, 1.2 TB/s), latency for few tokens (one: 4.2 us, of which an empty kernel is
 // about two): the batch's arrays and the page are two dependent reads, and the sines in 64
 // bits some hundred operations of one wave.  One work-group a token, so that these are
 // computed once for all its heads (a work-group for each 16 of its rows: the prompt takes

@@ -12,6 +12,12 @@
 // in any order, so that the choice depends on no sum's order:
 //   score = bounds' scale * max over the kv head's query heads of q's scale * (whole number)
 // with these two products in fp32.
+//
+// Bound: latency.  Bounds of the 131 pages of 8192 new 4-bit tokens (4.8 MB) 7.6 us, of 64
+// sequences' last pages 8.4: a sequence's place, its page and the keys are reads that depend
+// on each other.  Pages for one token of 2048 (4.2 MB) 12 us in two kernels, for 512 tokens of
+// 512 (their bounds 134 MB out of L2, 8 us of it) 20, for 2048 tokens 67, for 64 tokens of
+// 1150 each (151 MB) 46.
 #include "kv_cache.hpp"
 
 namespace hypno {
