@@ -5,8 +5,8 @@
 //
 // A run of keys of a kv head in one page is one piece of memory, codes as well as each
 // group's scales: whole runs are copied into a wave's own LDS, a tile before they are used
-// (two or three ahead: no more bytes a second, and LDS for fewer work-groups; 87 us below
-// become 107).  What is copied past the last key is masked, its scales of V set to 0.
+// (two ahead leave LDS for two work-groups a CU, not four: 64 sequences of up to 8192 in ranges
+// of 1024 take 107 us, not 87).  What is copied past the last key is masked, its scales of V set to 0.
 // K: lane (key, quarter) reads its quarter of the key's codes as they are, each eight of
 // which have one scale; q is held in the same order.  V: the 4-bit transposing read gives a
 // lane eight keys' codes of two channels, the scales lie key by key already.  Both become
@@ -15,8 +15,8 @@
 //
 // Bound: HBM for long contexts (from 524288 to 1048576 positions of 8 kv heads of 128, 604 MB
 // more take 99 us more: 6.1 TB/s); starts, ends and the join for shorter ones.  One token over
-// 131072 (151 MB) 33 us and 5 to join, 64 sequences of up to 8192 (340 MB) 77 and 5, 4.1 TB/s;
-// with every product twice (kPass 16, three work-groups a CU) the latter takes 91.  700
+// 131072 (151 MB) 33 us and 5 to join, 64 sequences of up to 8192 (340 MB) 77 and 5; in ranges
+// of 1024 87 in all, and 91 with every product twice (kPass 16, three work-groups a CU).  700
 // positions of 32/4 heads of 64: 8.0 us, dependent reads of the sequence's place, its page and
 // keys, three tiles, the waves' sum.
 #include "attention_few.hpp"
@@ -30,15 +30,13 @@ constexpr int kQ = kFewQ, kKeys = kFewKeys;
 // kLen: keys of a tile in one page, the whole tile's where pages have as many.
 template <int DP, int kLen>
 struct Few4 {
-  static constexpr int kAhead = 1;
   static constexpr int kRuns = kKeys / kLen;
   // Bytes of a run, and instructions that copy them, 16 and 4 bytes a lane.
   static constexpr int kCodes = kLen * DP / 2, kScales = kLen * DP / kFp4Group * 2;
   static constexpr int kCodeCopies = (kCodes + 1023) / 1024, kScaleCopies = (kScales + 255) / 256;
   static constexpr int kTile = 2 * kRuns * (kCodes + kScales);
-  static constexpr int kLoads = 2 * kRuns * (kCodeCopies + kScaleCopies);
-  static constexpr int kStage = (kAhead + 1) * kTile;
-  static constexpr int kWave = kStage > few_part_bytes<DP>() ? kStage : few_part_bytes<DP>();
+  // Two tiles; afterwards the wave's part.
+  static constexpr int kWave = 2 * kTile > few_part_bytes<DP>() ? 2 * kTile : few_part_bytes<DP>();
 };
 
 // Four bytes a lane, as dma16.
@@ -49,13 +47,6 @@ __device__ __forceinline__ void dma4(const void* base, uint32_t off, uint8_t* ld
                :
                : "{m0}"(at), "v"(off), "s"(base)
                : "memory");
-#endif
-}
-
-template <int kCount>
-__device__ __forceinline__ void wait_loads() {
-#if defined(__HIP_DEVICE_COMPILE__)
-  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"(kCount) : "memory");
 #endif
 }
 
@@ -202,31 +193,23 @@ __global__ void __launch_bounds__(64 * kWaves, kWaves == 8 ? 2 : DP > 128 ? 2 : 
       }
     };
 
-    uint8_t* to = ring;
     if (mine > 0) {
       look_up(0);
-#pragma unroll
-      for (int i = 0; i < T::kAhead; i++)
-        if (i < mine) {
-          issue(to);
-          to += T::kTile;
-          look_up(i + 1);
-        }
+      issue(ring);
+      look_up(1);
     }
     R x;
-    x.init_of(r0 + col % kPass < rows ? a.q + (size_t)t * a.q_stride + (size_t)h * D : nullptr, D, a.scale,
-              element);
+    x.init_of(r0 + col % kPass < rows ? a.q + (size_t)t * a.q_stride + (size_t)h * D : nullptr, D,
+              a.scale, element);
     if (kPass == 8) {
 #pragma unroll
       for (int st = 0; st < R::kSteps; st++) x.qh[st] = col < 8 ? x.qh[st] : x.ql[st];
     }
-    const uint8_t* at = ring;
     for (int tile = 0; tile < mine; tile++) {
       const int p0 = place(tile);
-      if (tile + T::kAhead <= mine)
-        wait_loads<(T::kAhead - 1) * T::kLoads>();
-      else
-        wait_loads<0>();
+      uint8_t* const at = ring + tile % 2 * T::kTile;
+      // (this tile's copies, and all reads of the one before)
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
       // Positions of the runs that are there to be seen, and the rest's scales of V: 0, as
       // the codes are finite and their weights 0.
       int there[kRuns];
@@ -242,8 +225,7 @@ __global__ void __launch_bounds__(64 * kWaves, kWaves == 8 ? 2 : DP > 128 ? 2 : 
         for (int i = 0; i < kRuns; i++)
           for (int k = lane; k < B * kLen; k += 64)
             if (k % kLen >= there[i])
-              *reinterpret_cast<_Float16*>(const_cast<uint8_t*>(at) + kVs + i * T::kScales + k * 2) =
-                  (_Float16)0.0f;
+              *reinterpret_cast<_Float16*>(at + kVs + i * T::kScales + k * 2) = (_Float16)0.0f;
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       }
       // All that this tile needs of LDS is on its way before the copies of a later one.
@@ -261,10 +243,9 @@ __global__ void __launch_bounds__(64 * kWaves, kWaves == 8 ? 2 : DP > 128 ? 2 : 
           ks[i][c] = *reinterpret_cast<const _Float16*>(at + kKs + scales_of(i) +
                                                         (blk * kLen + col) * 2);
         }
-      if (tile + T::kAhead < mine) {
-        issue(to);
-        to = to == ring + T::kAhead * T::kTile ? ring : to + T::kTile;
-        look_up(tile + T::kAhead + 1);
+      if (tile + 1 < mine) {
+        issue(ring + (tile + 1) % 2 * T::kTile);
+        look_up(tile + 2);
       }
       typename R::acc s[2];
 #pragma unroll
@@ -354,7 +335,6 @@ __global__ void __launch_bounds__(64 * kWaves, kWaves == 8 ? 2 : DP > 128 ? 2 : 
           if (kPass == 16) x.o[n] = Mfma<kQ>::mul(f16x8(y), f16x8(wl), x.o[n]);
         }
       }
-      at = at == ring + T::kAhead * T::kTile ? ring : at + T::kTile;
     }
     x.finish(bad != 0);
     if (kPass == 8) {
