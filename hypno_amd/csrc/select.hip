@@ -416,7 +416,7 @@ __global__ void __launch_bounds__(64 * kWaves, DP > 128 ? 2 : 4)
   }
 
   if (kStep == kScores) return;
-  if (kStep == kChoice) {
+  if (kStep == kChoice && kTeam) {
     for (int tok = 0; tok < nt; tok++)
       for (int p = bottom + tid; p < top; p += 64 * kWaves)
         keys[(size_t)tok * a.pitch + p] =
@@ -430,7 +430,8 @@ __global__ void __launch_bounds__(64 * kWaves, DP > 128 ? 2 : 4)
     const int64_t pos = pos0 + tok;
     const int own = pos < 0 ? -1 : (int)(pos >> shift);
     const int lo = a.first, hi = min(most, own + 1 - a.last);
-    const uint32_t* const key = keys + (size_t)tok * a.pitch;
+    const uint32_t* const key = kStep == kChoice && !kTeam ? all_keys + (size_t)tok * KV * a.pitch
+                                                           : keys + (size_t)tok * a.pitch;
     // The candidates' keys, some a thread at once (0 past them); all lanes go through it.
     auto each = [&](auto&& f) __attribute__((always_inline)) {
       constexpr int kKeysAtOnce = 8;
@@ -563,7 +564,8 @@ template <int DP, int kWaves, bool kTeam, int kStep>
 hipError_t run_step(const SelectArgs& a, hipStream_t s) {
   const size_t groups = ((size_t)a.b.tokens / a.tokens + a.b.batch) * a.k.kv_heads;
   const size_t grid = kStep == kScores ? groups * a.splits : groups;
-  const size_t lds = kStep == kScores ? 0 : (size_t)a.tokens * a.pitch * 4;
+  const size_t lds =
+      kStep == kScores || (kStep == kChoice && !kTeam) ? 0 : (size_t)a.tokens * a.pitch * 4;
   if (grid > 0xFFFFFFFFu / (64 * kWaves)) return hipErrorInvalidValue;
   const hipError_t e =
       set_lds_limit((const void*)select_pages_kernel<DP, kWaves, kTeam, kStep>, (int)lds);
@@ -573,12 +575,15 @@ hipError_t run_step(const SelectArgs& a, hipStream_t s) {
 }
 
 template <int DP>
-hipError_t run_select(const SelectArgs& a, bool team, hipStream_t s) {
-  if (a.splits > 1) {
-    const hipError_t e = run_step<DP, 4, false, kScores>(a, s);
-    return e == hipSuccess ? run_step<64, kTeamWaves, true, kChoice>(a, s) : e;
+hipError_t run_select(const SelectPlan& p, SelectArgs& a, hipStream_t s) {
+  if (a.scores) {
+    hipError_t e = run_step<DP, 4, false, kScores>(a, s);
+    if (e != hipSuccess) return e;
+    a.tokens = p.team ? 1 : 4;
+    return p.team ? run_step<64, kTeamWaves, true, kChoice>(a, s)
+                  : run_step<64, 4, false, kChoice>(a, s);
   }
-  return team ? run_step<DP, kTeamWaves, true, kBoth>(a, s) : run_step<DP, 4, false, kBoth>(a, s);
+  return p.team ? run_step<DP, kTeamWaves, true, kBoth>(a, s) : run_step<DP, 4, false, kBoth>(a, s);
 }
 
 }  // namespace
@@ -600,39 +605,61 @@ hipError_t launch_key_bounds(const KeyBounds& o, const KvCache& c, const KvBatch
   return hipGetLastError();
 }
 
+// Bytes of the scores between two kernels at most.
+constexpr size_t kMaxScores = (size_t)1 << 30;
+
 SelectPlan select_plan(int heads, const KeyBounds& k, const KvBatch& b, int pages, int num_cus) {
   SelectPlan p = {};
   p.pages = k.pages ? pages : 0;  // (none: nothing has a score)
   p.pitch = (p.pages + 3) / 4 * 4;
   p.rows = 1;
   while (p.rows < 16 && p.rows < heads / k.kv_heads) p.rows *= 2;
-  p.tokens = std::max(1, std::min(16 / p.rows, kMaxScored / std::max(p.pitch, 1)));
-  const size_t groups = ((size_t)b.tokens / p.tokens + b.batch) * k.kv_heads;
-  // Single tokens, and many pages: all of a work-group's waves look for one token's pages.
-  p.team = p.pages > 2048 || (p.pages > 256 && (groups <= (size_t)num_cus || b.tokens <= b.batch));
-  // Few work-groups: the pages' scores by as many as the chip holds, 128 pages or more each,
-  // and the choice by a kernel after them (one token over 2048 pages 19.9 us in one kernel).
+  const size_t rows = (size_t)b.tokens * k.kv_heads, most = 16 / p.rows;
+  const size_t groups = ((size_t)b.tokens / most + b.batch) * k.kv_heads;
   p.splits = 1;
-  if (p.team && p.pages >= 1024 && 2 * groups <= (size_t)num_cus) {
+  p.chunk = (p.pages + 127) / 128 * 128;
+  // One kernel, with the scores in LDS, or two and a workspace: where there are few
+  // work-groups, so that as many as the chip holds score 128 pages or more each (us, one / two:
+  // one token over 2048 pages 19.9 / 12.1, over 4096 32.5 / 13.8), and for chunks whose
+  // scores would leave LDS for few waves (512 tokens of 8 kv heads and 4 heads each over 4096
+  // pages 250 / 137, of 16 kv heads over 1024 90 / 49; 2048 of the first over 2048, in 32 KB, 236
+  // / 248).
+  const bool few = p.pages >= 1024 && 2 * groups <= (size_t)num_cus;
+  const bool big = b.tokens > b.batch && most * p.pitch * 4 > 40 << 10;
+  if (few) {
     const int n = (int)std::min<size_t>((size_t)num_cus / groups, (p.pages + 127) / 128);
     p.chunk = ((p.pages + n - 1) / n + 127) / 128 * 128;
     p.splits = (p.pages + p.chunk - 1) / p.chunk;
-    p.bytes = (size_t)b.tokens * k.kv_heads * p.pitch * 4;
+  }
+  if ((few || big) && rows * p.pitch * 4 <= kMaxScores) {
+    p.tokens = (int)most;
+    p.team = rows <= 2 * (size_t)num_cus;
+    p.bytes = rows * p.pitch * 4;
   }
   return p;
 }
 
-hipError_t launch_select_pages(const SelectPlan& p, int* out, int count, int first, int last,
+// In one kernel, as for what else has no workspace: as many tokens a work-group as LDS has room for, and where these are one or
+// two, all of its waves look for one token's pages.
+static void one_kernel(SelectPlan& p, const KvBatch& b) {
+  p.splits = 1;
+  p.tokens = std::max(1, std::min(16 / p.rows, kMaxScored / std::max(p.pitch, 1)));
+  p.team = p.pages > 256 && (p.tokens <= 2 || b.tokens <= b.batch);
+}
+
+hipError_t launch_select_pages(const SelectPlan& plan, int* out, int count, int first, int last,
                                const float* q, size_t q_stride, int heads, const KeyBounds& k,
                                const KvBatch& b, void* ws, hipStream_t s) {
+  SelectPlan p = plan;
+  if (!ws || !p.bytes) one_kernel(p, b);
   SelectArgs a = {};
   a.k = k, a.b = b, a.out = out, a.q = q, a.q_stride = q_stride, a.heads = heads;
   a.group = heads / k.kv_heads, a.count = count, a.first = first, a.last = last;
   a.rows = p.rows, a.most = p.pages, a.pitch = p.pitch, a.tokens = p.tokens;
-  a.splits = ws ? p.splits : 1, a.chunk = p.chunk, a.scores = (uint32_t*)ws;
-  return k.head_dim <= 64    ? run_select<64>(a, p.team, s)
-         : k.head_dim <= 128 ? run_select<128>(a, p.team, s)
-                             : run_select<256>(a, p.team, s);
+  a.splits = p.splits, a.chunk = p.chunk, a.scores = p.bytes ? (uint32_t*)ws : nullptr;
+  return k.head_dim <= 64    ? run_select<64>(p, a, s)
+         : k.head_dim <= 128 ? run_select<128>(p, a, s)
+                             : run_select<256>(p, a, s);
 }
 
 }  // namespace hypno

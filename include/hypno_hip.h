@@ -545,8 +545,8 @@ int hypno_hip_key_bounds_dev(const hypno_hip_key_bounds* bounds, const hypno_hip
  * have no score.  A token at a negative position selects nothing; rows of no sequence are
  * left alone.  max_kv_len: an upper bound of kv_lens (0: table_width * page_size), at most
  * 32768 pages.  count: at most 1024; first + last at most count.  Few tokens' scores of many
- * pages use the stream's workspace; under capture, without one that is large enough, they do
- * not (the choice is the same). */
+ * pages, and those of chunks, use the stream's workspace (1 GB at most); under capture,
+ * without one that is large enough, they do not (the choice is the same). */
 int hypno_hip_select_pages_dev(int32_t* selected, size_t count, size_t first, size_t last,
                                const float* q, size_t q_stride, size_t heads,
                                const hypno_hip_key_bounds* bounds,

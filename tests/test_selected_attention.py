@@ -241,6 +241,16 @@ def test_select_of_many(n, kv, page, count):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv_heads,n,kv", [(2, 2, 40, 3000), (3, 1, 300, 8000), (4, 1, 70, 5100),
+                                                 (20, 1, 33, 21000)])
+def test_select_of_chunks(heads, kv_heads, n, kv):
+    """Chunks over many pages: scores by one kernel and the choice by another, a wave a token."""
+    bt = Batch([(n, kv), (1, kv // 2), (n // 2, kv // 3)], 2, 49, kv_heads=kv_heads, dim=16)
+    q, b = queries(bt.tokens, heads, 16, 49), old_bounds(bt)
+    assert np.array_equal(run_select(bt, q, *b, 40, 1, 2), select(bt, q, *b, 40, 1, 2))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("kv", [500, 9000])
 def test_select_ties(kv):
     """Equal scores: the lower page.  Scores that are 0 with either sign are equal."""
