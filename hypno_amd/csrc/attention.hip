@@ -203,7 +203,10 @@ AttnPlan attn_plan(const KvCache& c, const KvBatch& b, int heads, int window, in
     const double tile_us = ((c.head_dim > 128 ? 2 : 1) * 0.8 + dim / 128.0) *
                            (c.dtype == kKvInt8 ? 1.2 : 1.0);
     double best = 1e30;
-    for (int n = 1; n <= 64; n++) {
+    // (4-bit: up to 256, as one kv head's 64 leave most CUs without work: five tokens over
+    // 100000 positions of 8/1 heads of 256 89 us with 64, 43 so)
+    const int most_ranges = c.dtype == kKvFp4 ? 256 : 64;
+    for (int n = 1; n <= most_ranges; n++) {
       const int64_t chunk = (up(seen, n) + 63) / 64 * 64;
       const int splits = up(seen, chunk);
       if (splits > most(token_rows)) break;

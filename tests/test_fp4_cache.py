@@ -202,7 +202,8 @@ def test_far_pages(n):
 @pytest.mark.gpu
 def test_long_context():
     """Ranges of one sequence's positions, and of several of different lengths."""
-    for seqs in ([(1, 20011)], [(1, 9001), (1, 3), (1, 5005), (1, 64)], [(2, 6000), (7, 4100)]):
+    for seqs in ([(1, 20011)], [(1, 9001), (1, 3), (1, 5005), (1, 64)], [(2, 6000), (7, 4100)],
+                 [(5, 60000)]):
         bt = Batch4(seqs, 64, 18, kv_heads=1, dim=128)
         q = queries(bt.tokens, 4, 128, 18)
         ref, tol = attend(q, bt)
