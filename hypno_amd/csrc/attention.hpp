@@ -9,7 +9,8 @@
 // so that a lane holds one row's scores and its part of one row's output, and the
 // scores' registers are the second product's operand as they are.
 //
-// Arithmetic: the cache's values are fp16 or 8-bit codes, both exact as MFMA operands.
+// Arithmetic: the cache's values are fp16 (4-bit codes times their scale as well) or 8-bit
+// codes, both exact as MFMA operands.
 // q (scaled by a power of two per row) goes in as two fp16, 22 bits, every product
 // twice.  The weights times the values' scale go in as three bf16, all of an fp32, beside
 // 8-bit values: a code of 0 beside the largest weight leaves an element to the smallest.
