@@ -109,6 +109,24 @@ struct KeyBounds {
   int pages, kv_heads, page_shift, head_dim;
 };
 
+// The pages that hold a batch's new tokens, numbered over all sequences: where the numbers of
+// sequence b begin, whose first token is `first` (n tokens are in floor((n - 1) / page_size) + 2
+// pages at most).
+__host__ __device__ inline int64_t first_number(int first, int b, int shift) {
+  return (first >> shift) + 2 * (int64_t)b;
+}
+
+// Which of its pages `number` stands for in sequence b, which brings the tokens [first, end)
+// of the kv that it holds; -1: none with a new token and a place in a table of `width`
+// pages.  (Where cu_q does not ascend a number may come before the sequence's own.)
+__host__ __device__ inline int page_of_number(int64_t number, int b, int first, int end, int kv,
+                                              int shift, int width) {
+  const int64_t own = number - first_number(first, b, shift), kept = (int64_t)kv - (end - first);
+  if (own < 0 || end <= first || kv <= 0) return -1;
+  const int64_t at = ((kept > 0 ? kept : 0) >> shift) + own;
+  return at <= (kv - 1) >> shift && at < width ? (int)at : -1;
+}
+
 // Pages of a sequence that scores are kept of at most (in LDS).
 constexpr int kMaxScored = 32768;
 // Pages that a token reads at most.

@@ -44,16 +44,14 @@ struct BoundsArgs {
   int lane_shift;  // 1 << lane_shift lanes a key, each with 8 channels
 };
 
-// The sequence whose pages' numbers reach `slot`, where sequence i's start at
-// floor(cu_q[i] / page_size) + 2 i (n tokens are in floor((n - 1) / page_size) + 2 pages at
-// most).
-__device__ __forceinline__ int seq_of_page(const BoundsArgs& a, int slot) {
+// The last sequence whose pages' numbers begin at `number` or before.
+__device__ __forceinline__ int seq_of_page(const BoundsArgs& a, int64_t number) {
   const int lane = threadIdx.x & 63;
   int count = 0;
   for (int i0 = 0; i0 <= a.b.batch; i0 += 64) {
     const int i = i0 + lane;
     bool in = false;
-    if (i <= a.b.batch) in = (cu_at(a.b, i) >> a.c.page_shift) + 2 * (int64_t)i <= slot;
+    if (i <= a.b.batch) in = first_number(cu_at(a.b, i), i, a.c.page_shift) <= number;
     count += __popcll(__ballot(in));
   }
   return count - 1;
@@ -99,18 +97,16 @@ __global__ void __launch_bounds__(256) key_bounds_kernel(BoundsArgs a) {
   const int D = a.c.head_dim, KV = a.c.kv_heads;
   const int unit = tid & ((1 << a.lane_shift) - 1), row = tid >> a.lane_shift;
   const int e0 = 8 * unit, rows = 256 >> a.lane_shift;
-  const int64_t slots = (cu_at(a.b, a.b.batch) >> a.c.page_shift) + 2 * (int64_t)a.b.batch;
-  for (int64_t w = blockIdx.x; w < slots * KV; w += gridDim.x) {
+  const int64_t numbers = first_number(cu_at(a.b, a.b.batch), a.b.batch, a.c.page_shift);
+  for (int64_t w = blockIdx.x; w < numbers * KV; w += gridDim.x) {
     // (all lanes decide the same)
-    const int slot = (int)(w / KV), g = (int)(w % KV);
-    const int b = seq_of_page(a, slot);
+    const int64_t number = w / KV;
+    const int g = (int)(w % KV), b = seq_of_page(a, number);
     if (b < 0 || b >= a.b.batch) continue;
-    const int first = cu_at(a.b, b), n = cu_at(a.b, b + 1) - first;
     const int kv = load_global<int>(a.b.kv_lens + b);
-    if (n <= 0 || kv <= 0) continue;
-    const int at = (int)(max((int64_t)kv - n, (int64_t)0) >> a.c.page_shift) + slot -
-                   ((first >> a.c.page_shift) + 2 * b);
-    if (at > (kv - 1) >> a.c.page_shift || at >= a.b.width) continue;
+    const int at = page_of_number(number, b, cu_at(a.b, b), cu_at(a.b, b + 1), kv, a.c.page_shift,
+                                  a.b.width);
+    if (at < 0) continue;
     const int page = load_global<int>(a.b.page_table + (size_t)b * a.b.width + at);
     if (page < 0 || page >= a.c.pages) continue;
     const int keys = min(1 << a.c.page_shift, kv - (at << a.c.page_shift));
