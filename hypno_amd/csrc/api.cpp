@@ -13,7 +13,6 @@
 #include <map>
 #include <memory>
 #include <mutex>
-#include <set>
 #include <string>
 #include <vector>
 
@@ -701,14 +700,15 @@ bool gemm_folded() { return g_gemm_numerics.load() == HYPNO_HIP_GEMM_FOLDED; }
 
 hipError_t set_lds_limit(const void* kernel, int bytes) {
   static std::mutex mu;
-  static std::set<std::pair<const void*, int>> done;
+  static std::map<std::pair<const void*, int>, int> limits;
   int dev = 0;
   hipError_t e = hipGetDevice(&dev);
   if (e != hipSuccess) return e;
   std::lock_guard<std::mutex> g(mu);
-  if (done.count({kernel, dev})) return hipSuccess;
+  int& limit = limits.try_emplace({kernel, dev}, -1).first->second;
+  if (bytes <= limit) return hipSuccess;
   e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e == hipSuccess) done.insert({kernel, dev});
+  if (e == hipSuccess) limit = bytes;
   return e;
 }
 

@@ -501,8 +501,8 @@ int hip_status(hipError_t e, const char* what);
 // (hypno_hip_set_gemm_numerics(HYPNO_HIP_GEMM_EXACT)).
 bool gemm_folded();
 
-// Raises `kernel`'s dynamic-LDS limit to `bytes` on the current device, once
-// per (kernel, device); safe to call from several threads (api.cpp).
+// Raises `kernel`'s dynamic-LDS limit on the current device to `bytes`, where no
+// call before asked for as much; safe to call from several threads (api.cpp).
 hipError_t set_lds_limit(const void* kernel, int bytes);
 
 }  // namespace hypno
