@@ -802,7 +802,7 @@ int kv_args(const char* what, const hypno_hip_kv_cache* c, const hypno_hip_kv_ba
     return fail(HYPNO_HIP_EINVAL, "%s: a 4-bit cache's scales must be 16-byte aligned", what);
   const size_t tokens = c->kv_heads * c->page_size, page = kv_page_elems(*c),
                sp = fp4 ? tokens * (c->head_dim / kFp4Group) : tokens;
-  *kc = KvCache{(int)c->dtype, c->k, c->v, (float*)c->k_scale, (float*)c->v_scale,
+  *kc = KvCache{(int)c->dtype, c->k, c->v, c->k_scale, c->v_scale,
                 c->k_page_stride ? c->k_page_stride : page,
                 c->v_page_stride ? c->v_page_stride : page,
                 c->k_scale_page_stride ? c->k_scale_page_stride : sp,

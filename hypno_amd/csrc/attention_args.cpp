@@ -85,7 +85,7 @@ bool cache(PyObject* k, PyObject* v, PyObject* ks, PyObject* vs, int dev, hypno_
   if (!kst || !vst || kst->sizes() != want || vst->sizes() != want) return false;
   const int64_t ksp = page_stride(*kst), vsp = page_stride(*vst);
   if (ksp < 0 || vsp < 0) return false;
-  c.k_scale = kst->data_ptr(), c.v_scale = vst->data_ptr();
+  c.k_scale = (float*)kst->data_ptr(), c.v_scale = (float*)vst->data_ptr();
   c.k_scale_page_stride = (size_t)ksp, c.v_scale_page_stride = (size_t)vsp;
   return true;
 }

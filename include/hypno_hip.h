@@ -455,10 +455,10 @@ typedef struct hypno_hip_kv_cache {
   uint32_t dtype;             /* HYPNO_HIP_KV_* */
   void* k;                    /* [pages][kv_heads][page_size][head_dim], 16-byte aligned */
   void* v;                    /* (FP4: the last is head_dim / 2 bytes) */
-  void* k_scale;              /* INT8: float [pages][kv_heads][page_size]; FP16: NULL;
-                               * FP4: fp16 [pages][kv_heads][head_dim / 32][page_size],
-                               * 16-byte aligned */
-  void* v_scale;
+  float* k_scale;             /* INT8: [pages][kv_heads][page_size]; FP16: NULL; FP4: the
+                               * address, cast, of fp16 ones [pages][kv_heads][head_dim / 32]
+                               * [page_size], 16-byte aligned */
+  float* v_scale;
   size_t pages, kv_heads;
   size_t page_size;           /* a power of two, at most 2^16 (FP4: at least 16) */
   size_t head_dim;            /* a multiple of 8 (FP4: of 32), at most 256 */
