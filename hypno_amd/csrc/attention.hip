@@ -160,10 +160,10 @@ AttnPlan attn_plan(const KvCache& c, const KvBatch& b, int heads, int window, in
   // Beyond, one sequence gets a work-group for each one that the chip holds at a time.
   // Lengths of several may differ, so that the last range to end counts: against the
   // start of a range (about 130 positions' time, 250 of 4-bit ones) the best length grows
-  // with the root of all work.  (us at 32/8 heads of 128, ranges of 128 / 256 / 512 / none: one sequence
-  // of 3000: 11.1 / 12.0 / 14.1 / -; 8 of up to 6000: 44 / 35 / 32 / -; 64 of up to 2000:
-  // - / 67 / 58 / 53.  4-bit, 64 of up to 8192, ranges of 512 / 1024 / 1536 / 2048: 92 / 82 /
-  // 82 / 84; 2 of 16000, 256 / 512 / 1024: 20.0 / 18.1 / 18.7.)
+  // with the root of all work.  (us at 32/8 heads of 128, ranges of 128 / 256 / 512 / none:
+  // one sequence of 3000: 11.1 / 12.0 / 14.1 / -; 8 of up to 6000: 44 / 35 / 32 / -; 64 of up
+  // to 2000: - / 67 / 58 / 53.  4-bit, 64 of up to 8192, ranges of 512 / 1024 / 1536 / 2048:
+  // 92 / 82 / 82 / 84; 2 of 16000, 256 / 512 / 1024: 20.0 / 18.1 / 18.7.)
   p.fs = {1, 0x7FFFFFFF};
   p.few_waves = 4;
   const size_t token_rows = (size_t)b.tokens * heads, place = (size_t)c.head_dim * 4 + 8;
@@ -203,8 +203,10 @@ AttnPlan attn_plan(const KvCache& c, const KvBatch& b, int heads, int window, in
     const double tile_us = ((c.head_dim > 128 ? 2 : 1) * 0.8 + dim / 128.0) *
                            (c.dtype == kKvInt8 ? 1.2 : 1.0);
     double best = 1e30;
-    // (4-bit: up to 256, as one kv head's 64 leave most CUs without work: five tokens over
-    // 100000 positions of 8/1 heads of 256 89 us with 64, 43 so)
+    // (One kv head's 64 leave most CUs without work: five tokens over 100000 positions of 8/1
+    // heads of 256, 4-bit, 89 us, and 43 with up to 256.  The same holds for the other types,
+    // which keep the ranges, and with them the roundings, that they had; more were not
+    // measured there.)
     const int most_ranges = c.dtype == kKvFp4 ? 256 : 64;
     for (int n = 1; n <= most_ranges; n++) {
       const int64_t chunk = (up(seen, n) + 63) / 64 * 64;

@@ -1,8 +1,9 @@
 // The tensors of append_kv, paged_attention, key_bounds, select_pages and
-// selected_attention (attention.py) to the structs and arguments of include/hypno_hip.h.  What the Python functions check one attribute at a
-// time (5 to 7 us a call, more than a token's kernel takes) is read from the tensors
-// here, 1 to 2 us.  Only calls that are right are made: for any other the answer is
-// NotImplemented, and the Python functions say what is wrong with it.
+// selected_attention (attention.py) to the structs and arguments of include/hypno_hip.h.
+// What the Python functions check one attribute at a time (5 to 7 us a call, more than a
+// token's kernel takes) is read from the tensors here, 1 to 2 us.  Only calls that are
+// right are made: for any other the answer is NotImplemented, and the Python functions
+// say what is wrong with it.
 #include <ATen/ATen.h>
 #include <torch/csrc/autograd/python_variable.h>
 

@@ -5,8 +5,8 @@
 //
 // A run of keys of a kv head in one page is one piece of memory, codes as well as each
 // group's scales: whole runs are copied into a wave's own LDS, a tile before they are used
-// (two ahead leave LDS for two work-groups a CU, not four: 64 sequences of up to 8192 in ranges
-// of 1024 take 107 us, not 87).  What is copied past the last key is masked, its scales of V set to 0.
+// (two ahead leave LDS for two work-groups a CU, not four, and take 64 sequences of up to 8192
+// a quarter longer).  What is copied past the last key is masked, its scales of V set to 0.
 // K: lane (key, quarter) reads its quarter of the key's codes as they are, each eight of
 // which have one scale; q is held in the same order.  V: the 4-bit transposing read gives a
 // lane eight keys' codes of two channels, the scales lie key by key already.  Both become
@@ -15,10 +15,10 @@
 //
 // Bound: HBM for long contexts (from 524288 to 1048576 positions of 8 kv heads of 128, 604 MB
 // more take 99 us more: 6.1 TB/s); starts, ends and the join for shorter ones.  One token over
-// 131072 (151 MB) 33 us and 5 to join, 64 sequences of up to 8192 (340 MB) 77 and 5; in ranges
-// of 1024 87 in all, and 91 with every product twice (kPass 16, three work-groups a CU).  700
-// positions of 32/4 heads of 64: 8.0 us, dependent reads of the sequence's place, its page and
-// keys, three tiles, the waves' sum.
+// 131072 (151 MB) 33 to 36 us and 5 to join, 64 sequences of up to 8192 (340 MB) 82 to 84 in
+// all, 5 to 6 of them to join, and 87.5 with every product twice (kPass 16, three work-groups
+// a CU, beside 84).  700 positions of 32/4 heads of 64: 8.0 us, dependent reads of the
+// sequence's place, its page and keys, three tiles, the waves' sum.
 #include "attention_few.hpp"
 
 namespace hypno {
@@ -366,7 +366,10 @@ hipError_t run(const AttnArgs& a, hipStream_t s) {
 
 template <int DP, int kWaves>
 hipError_t run(const AttnArgs& a, hipStream_t s) {
-  // (a sequence with more rows than a pass goes through its keys once for each)
+  // (a sequence with more rows than a pass goes through its keys once for each.  A call with
+  // more tokens than sequences takes 16 rows for all of them: one sequence of two tokens among
+  // 64 of up to 8192 87 -> 96 us, of up to 2000 28 -> 39, a launch of the kernel for longer
+  // sequences among it)
   const bool one = a.group <= 8 && (a.selected || a.b.tokens <= a.b.batch);
   if (a.c.page_shift > kRunShift)
     return one ? run<DP, 32, 8, kWaves>(a, s) : run<DP, 32, 16, kWaves>(a, s);

@@ -15,7 +15,8 @@
 //
 // Bound: latency.  Bounds of the 131 pages of 8192 new 4-bit tokens (4.8 MB) 7.6 us, of 64
 // sequences' last pages 8.4: a sequence's place, its page and the keys are reads that depend
-// on each other.  Pages for one token of 2048 (4.2 MB) 12 us in two kernels, for 512 tokens of
+// on each other, six for 64 sequences (cu_q's end, its values 64 at a time, the sequence's
+// own beside its kv_len, the page, the keys).  Pages for one token of 2048 (4.2 MB) 12 us in two kernels, for 512 tokens of
 // 512 (their bounds 134 MB out of L2, 8 us of it) 20, for 2048 tokens 67, for 64 tokens of
 // 1150 each (151 MB) 46.
 #include "kv_cache.hpp"
@@ -635,8 +636,9 @@ SelectPlan select_plan(int heads, const KeyBounds& k, const KvBatch& b, int page
   return p;
 }
 
-// In one kernel, as for what else has no workspace: as many tokens a work-group as LDS has room for, and where these are one or
-// two, all of its waves look for one token's pages.
+// In one kernel, with or for want of a workspace: as many tokens a work-group as a product
+// has rows and LDS has room for.  Where these are one or two, or tokens are single, all of
+// its waves look for one token's pages.
 static void one_kernel(SelectPlan& p, const KvBatch& b) {
   p.splits = 1;
   p.tokens = std::max(1, std::min(16 / p.rows, kMaxScored / std::max(p.pitch, 1)));
